@@ -14,6 +14,7 @@ import argparse
 import concurrent.futures as cf
 import hashlib
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -47,6 +48,25 @@ def _headers() -> list[str]:
     hs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
     hs += [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE) if f.endswith(".h")]
     return sorted(hs)
+
+
+def _with_includes(src: str) -> list[str]:
+    """The source and every header of this repository it includes, directly or not."""
+    found, todo = set(), [src]
+    while todo:
+        p = todo.pop()
+        if p in found:
+            continue
+        found.add(p)
+        with open(p) as f:
+            names = re.findall(r'^\s*#\s*include\s+"([^"]+)"', f.read(), flags=re.M)
+        for name in names:
+            for folder in (os.path.dirname(p), INCLUDE, CSRC):
+                at = os.path.normpath(os.path.join(folder, name))
+                if os.path.exists(at):
+                    todo.append(at)
+                    break
+    return [src] + sorted(found - {src})
 
 
 def _fingerprint(flags: list[str]) -> str:
@@ -104,17 +124,12 @@ def build(force: bool = False, debug: bool = False, verbose: bool = False, jobs:
     srcs = _sources()
     objs = [os.path.join(BUILD_DIR, os.path.basename(s)[:-3] + ".o") for s in srcs]
 
-    hdr_hash = hashlib.sha256()
-    for p in _headers():
-        with open(p, "rb") as f:
-            hdr_hash.update(p.encode())
-            hdr_hash.update(f.read())
-    hdr_hash.update(" ".join(flags).encode())
-
     def obj_fingerprint(src: str) -> str:
-        h = hdr_hash.copy()
-        with open(src, "rb") as f:
-            h.update(f.read())
+        h = hashlib.sha256(" ".join(flags).encode())
+        for p in _with_includes(src):
+            with open(p, "rb") as f:
+                h.update(p.encode())
+                h.update(f.read())
         return h.hexdigest()
 
     def compile_one(pair):
