@@ -280,6 +280,70 @@ int po_matmul(const void* A, long long lda, long long sa, int trans_a, const voi
               long long M, long long N, long long K, float alpha, float beta, void* workspace,
               size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Language-model losses over a large vocabulary, with their gradients. No
+ * counterpart in the reference: what an optimised model's training step runs
+ * next to the optimizer. One row (token) t has the logits z = W h_t.
+ *
+ * Hard targets (teacher == NULL, top == 1), y = index[t], s = smoothing:
+ *   l  = lse(z) - (1 - s) z_y - s mean(z) + z_loss lse(z)^2
+ *   dz = (1 + 2 z_loss lse(z)) softmax(z) - (1 - s) onehot(y) - s / vocab
+ * Rows with y == ignore_index count for nothing.
+ * A teacher's top logits (teacher != NULL), over the entries k of the row
+ * with index[t][k] >= 0, a = temperature:
+ *   q  = softmax(teacher / a)
+ *   l  = a^2 sum_k q_k (log q_k - log softmax(z / a)[i_k])
+ *   dz = a (softmax(z / a) - q scattered to i)
+ * (equal indices add up). Rows without an entry above -inf count for nothing;
+ * what is stored beside a negative index is not looked at.
+ *
+ * A row that counts for nothing has loss 0 and gradient 0, whatever its
+ * hidden state holds, and is left out of the mean and of the products. With
+ * no counted row the loss and all gradients are 0. A row with an index
+ * outside [0, vocab) (other than ignore_index, or a negative one of a
+ * teacher's) has the loss NaN and gradient 0, and counts in the mean.
+ *
+ * hidden: tokens x dim, weight: vocab x dim, both of `dtype` (PO_BF16 /
+ * PO_F16 / PO_F32: split-tf32 products, fp32-grade), rows contiguous with the
+ * given pitches. index: tokens x top int64 (pitch index_ld); teacher: tokens
+ * x top of teacher_dtype (PO_F32 / PO_BF16 / PO_F16). top <= 1024.
+ * loss_rows (fp32 [tokens]) receives each row's loss; loss (nullable) their
+ * sum, divided by the counted rows when `mean`. dhidden (pitch dh_ld) and
+ * dweight (pitch dw_ld), nullable, receive the gradients of that loss in
+ * `dtype`; with row_grad (fp32 [tokens], nullable) the gradients of
+ * sum_t row_grad[t] l_t instead (`mean` must be 0).
+ * The logits are never stored: without gradients each tile of them leaves two
+ * numbers a row; with gradients at most chunk_rows rows at a time (0: a
+ * default by the workspace it takes) leave their scaled exponentials in the
+ * workspace, in 16 bits (32 for fp32).
+ * ---------------------------------------------------------------------- */
+size_t po_linear_loss_workspace_bytes(const void* weight, long long w_ld, int dtype, long long tokens, long long dim,
+                                      long long vocab, long long top, int want_dhidden, int want_dweight,
+                                      long long chunk_rows);
+int po_linear_loss(const void* hidden, long long h_ld, const void* weight, long long w_ld, int dtype,
+                   long long tokens, long long dim, long long vocab, const long long* index, long long index_ld,
+                   const void* teacher, long long teacher_ld, int teacher_dtype, long long top,
+                   long long ignore_index, float smoothing, float z_loss, float temperature, int mean,
+                   const float* row_grad, float* loss_rows, float* loss, void* dhidden, long long dh_ld,
+                   void* dweight, long long dw_ld, long long chunk_rows, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/* The teacher's form of po_linear_loss on logits that are there: logits and
+ * dlogits (nullable) tokens x vocab of `dtype` (PO_F32 / PO_BF16 / PO_F16)
+ * with any pitches; the logits are read once and dlogits written once
+ * (dlogits == logits, with equal pitches, is allowed). */
+size_t po_distill_logits_workspace_bytes(long long tokens);
+int po_distill_logits(const void* logits, long long ld, int dtype, long long tokens, long long vocab,
+                      const long long* index, long long index_ld, const void* teacher, long long teacher_ld,
+                      int teacher_dtype, long long top, float temperature, int mean, const float* row_grad,
+                      float* loss_rows, float* loss, void* dlogits, long long dl_ld, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* x[i] <- x[i] * *factor over n elements of `dtype` (PO_F32 / PO_BF16 /
+ * PO_F16), factor a device scalar; a factor of exactly 1 moves no data. The
+ * chain rule of a loss whose gradients were made with it. */
+int po_scale_inplace(void* x, int dtype, long long n, const float* factor, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

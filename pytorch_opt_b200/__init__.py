@@ -8,10 +8,12 @@ Muon, Shampoo, SOAP and KFAC optimizers of pytorch-opt:
   ``pytorch_opt.ops.native_build.load()``), plus KFAC and batched extras;
 * ``ops``     — the ``pytorch_opt.ops`` public API mirrored on that library;
 * ``muon``    — grouped multi-matrix Muon step (momentum, Newton–Schulz, update);
+* ``losses``  — losses over a large vocabulary with their gradients (linear cross
+  entropy, distillation from a teacher's top logits);
 * ``dist``    — FLOP-balanced sharding of matrices over ranks and the NCCL
   all-gather of their updates.
 """
 
-from . import ops, native  # noqa: F401
+from . import losses, native, ops  # noqa: F401
 
 __version__ = "0.1.0"

@@ -56,6 +56,13 @@ SIGNATURES = {
     "po_matmul_workspace_bytes": (_sz, [_ll, _ll, _ll, _ll, _i, _i]),
     "po_matmul": (_i, [_vp, _ll, _ll, _i, _vp, _ll, _ll, _i, _vp, _ll, _ll, _i, _i, _ll, _ll, _ll, _ll, _f, _f,
                        _vp, _sz, _vp]),
+    "po_linear_loss_workspace_bytes": (_sz, [_vp, _ll, _i, _ll, _ll, _ll, _ll, _i, _i, _ll]),
+    "po_linear_loss": (_i, [_vp, _ll, _vp, _ll, _i, _ll, _ll, _ll, _vp, _ll, _vp, _ll, _i, _ll, _ll, _f, _f, _f, _i,
+                            _vp, _vp, _vp, _vp, _ll, _vp, _ll, _ll, _vp, _sz, _vp]),
+    "po_distill_logits_workspace_bytes": (_sz, [_ll]),
+    "po_distill_logits": (_i, [_vp, _ll, _i, _ll, _ll, _vp, _ll, _vp, _ll, _i, _ll, _f, _i, _vp, _vp, _vp, _vp, _ll,
+                               _vp, _sz, _vp]),
+    "po_scale_inplace": (_i, [_vp, _i, _ll, _vp, _vp]),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,630 @@
+// The three products of a linear loss head on two-SM tcgen05 tiles: logits
+// H W^T with their softmax statistics taken in the epilogue, dH = dZ W and
+// dW = dZ^T H.
+//
+// Mainloop as in gemm_pair.cuh (cluster of two CTAs, 256 x 256 tile, 64 KB
+// stages of two 128-byte K atoms, dynamic tile queue), with three differences:
+//  * The extent that counts rows of H is read on the device (rows that count
+//    for nothing are packed away before, and their number never reaches the
+//    host), so tiles beyond it are not computed.
+//  * K may be split over tiles (few rows of H, a long vocabulary): each split
+//    stores its fp32 partial tile, a later kernel joins them in order.
+//  * The accumulator is drained into registers every `chunk` K blocks and
+//    summed there (fp32, round to nearest): the tensor core's own accumulator
+//    truncates, by -1.1e-5 of the sum at K = 4096, which the loss (a difference
+//    of two nearby logits) would show. A drain is 128 tcgen05.ld columns and
+//    128 adds a thread against 1024 tensor cycles a block, hidden behind the
+//    other accumulator's MMAs.
+//
+// Epilogue of the logits: each thread holds 128 columns of one row, so the
+// row's maximum and sum of exponentials over those columns need no exchange
+// between threads: 128 compares, 128 FMA + ex2, 128 adds. It leaves (max, sum)
+// per row and 128 columns, the logits at the row's target indices, and, when
+// gradients are wanted, exp(z - max) in 16 bits (fp16: the values are in
+// (0, 1], so its 11 bits cost less than the one rounding to the products' type
+// that follows; 32 bits for fp32 operands). Storing that costs 2 bytes a logit
+// once against 2 D operations a logit for computing it again.
+#pragma once
+
+#include "common.cuh"
+#include "gemm_pair.cuh"
+
+namespace po {
+
+enum HeadEpi : int { HEAD_STATS = 0, HEAD_STORE = 1 };
+enum HeadLimit : int { LIMIT_M = 0, LIMIT_K = 1 };  // which extent `count` bounds
+
+struct alignas(64) HeadParams {
+  CUtensorMap mapA[2];  // [0] = plain / hi, [1] = lo (fp32 operands)
+  CUtensorMap mapB[2];
+  int M, N, K;
+  int limit;         // HeadLimit
+  const int* count;  // device: counted rows of the whole call
+  int row0;          // first packed row of this launch
+  int tiles_n, splits, band;
+  int npass;         // 1, or 3: hi*hi, hi*lo, lo*hi
+  int chunk;         // K blocks summed inside the accumulator
+  uint32_t fmt;      // operand format of the instruction descriptor
+  unsigned int* sched;
+  int* err;
+  // HEAD_STATS
+  float scale2;       // log2(e) / temperature
+  float2* part;       // [row][nparts] (max, sum of 2^(z2 - max)) over 128 columns, z2 = scale2 * logit
+  int nparts;
+  float* zsum;        // [row][nparts] sum of the logits (nullable)
+  void* e;            // [row][e_ld] 2^(z2 - max) (nullable)
+  long long e_ld;
+  const int* rowmap;  // packed row -> row of the call
+  const int* ent;     // [row of the call][top] ascending target indices
+  int top;
+  float* zpick;       // [row of the call][top] z2 at those indices
+  // HEAD_STORE
+  const float* alpha;  // device scalar
+  const float* cin;    // fp32, added to row r (nullable)
+  long long cin_ld;
+  void* out;           // row r of the product goes to out row (rows ? rows[row0 + r] : r)
+  long long out_ld;
+  int out_dtype;       // PO_F32 / PO_BF16 / PO_F16
+  int vec;             // 32-byte vector access legal
+  const int* out_rows;
+  float* partial;      // splits > 1: [split][M][part_ld] fp32, instead of out
+  long long part_ld;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void st_global_32B(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+constexpr int HC = 128;  // columns of a tile one epilogue thread holds
+
+struct HeadTile {
+  int mt, nt, split, kb0, kb1;
+};
+
+// Extents of this launch after the device-side count.
+struct HeadExtent {
+  int m, tiles_m, nkb, total;
+};
+
+template <class C>
+__device__ __forceinline__ HeadExtent head_extent(const HeadParams& P) {
+  HeadExtent x;
+  const int left = max(0, __ldg(P.count) - P.row0);
+  x.m = P.limit == LIMIT_M ? min(P.M, left) : P.M;
+  const int k = P.limit == LIMIT_K ? min(P.K, left) : P.K;
+  x.tiles_m = (x.m + C::TM - 1) / C::TM;
+  x.nkb = (k + C::BK - 1) / C::BK;
+  x.total = x.tiles_m * P.tiles_n * P.splits;
+  return x;
+}
+
+// Splits outermost; in a split, bands of `band` row tiles, walked row tiles
+// first, so that tiles in flight share both operands' panels in L2.
+__device__ __forceinline__ HeadTile head_tile(const HeadParams& P, const HeadExtent& x, int t) {
+  HeadTile h;
+  const int per = x.tiles_m * P.tiles_n;
+  h.split = t / per;
+  const int r = t - h.split * per;
+  const int b = r / (P.band * P.tiles_n);
+  const int first = b * P.band;
+  const int rows = min(x.tiles_m - first, P.band);
+  const int in_band = r - b * P.band * P.tiles_n;
+  h.mt = first + in_band % rows;
+  h.nt = in_band / rows;
+  h.kb0 = static_cast<int>(static_cast<long long>(x.nkb) * h.split / P.splits);
+  h.kb1 = static_cast<int>(static_cast<long long>(x.nkb) * (h.split + 1) / P.splits);
+  return h;
+}
+
+// ------------------------------------------------------------- epilogues
+// x: accumulators of columns n0 .. n0 + 127 of packed row `row` (of this launch).
+template <bool F32E>
+__device__ __forceinline__ void stats_epilogue(const HeadParams& P, float (&x)[HC], bool live, int row, int n0,
+                                               int nt2, long long tk, int lo, int c) {
+  const int ncols = P.N - n0;
+  // Logits at the targets: c is the next target's column in this tile. One
+  // vote per 16 columns; a row has few targets, so most groups have none.
+#pragma unroll
+  for (int g = 0; g < HC / 16; ++g) {
+    while (__any_sync(0xffffffffu, c < 16 * g + 16)) {
+      if (c < 16 * g + 16) {
+        float v = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (c == 16 * g + j) v = x[16 * g + j];
+        P.zpick[tk + lo] = v * P.scale2;
+        ++lo;
+        c = lo < P.top ? __ldg(P.ent + tk + lo) - n0 : 0x7fffffff;
+      }
+    }
+  }
+  if (!live) return;
+  const long long at = static_cast<long long>(row) * P.nparts + nt2;
+  if (P.zsum != nullptr) {
+    // Columns past the vocabulary come from zero-filled rows of W: they add 0.
+    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < HC; j += 2) {
+      s0 += x[j];
+      s1 += x[j + 1];
+    }
+    P.zsum[at] = s0 + s1;
+  }
+  if (ncols < HC) {
+#pragma unroll
+    for (int j = 0; j < HC; ++j)
+      if (j >= ncols) x[j] = -INFINITY;
+  }
+  float m0 = x[0], m1 = x[1], m2 = x[2], m3 = x[3];
+#pragma unroll
+  for (int j = 4; j < HC; j += 4) {
+    m0 = fmaxf(m0, x[j]);
+    m1 = fmaxf(m1, x[j + 1]);
+    m2 = fmaxf(m2, x[j + 2]);
+    m3 = fmaxf(m3, x[j + 3]);
+  }
+  const float m = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * P.scale2;
+  const float off = m == -INFINITY ? 0.0f : -m;
+  float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
+#pragma unroll
+  for (int j = 0; j < HC; j += 4) {
+    x[j] = ex2(fmaf(x[j], P.scale2, off));
+    x[j + 1] = ex2(fmaf(x[j + 1], P.scale2, off));
+    x[j + 2] = ex2(fmaf(x[j + 2], P.scale2, off));
+    x[j + 3] = ex2(fmaf(x[j + 3], P.scale2, off));
+    s0 += x[j];
+    s1 += x[j + 1];
+    s2 += x[j + 2];
+    s3 += x[j + 3];
+  }
+  P.part[at] = make_float2(m, (s0 + s1) + (s2 + s3));
+  if (P.e == nullptr) return;
+  const long long base = static_cast<long long>(row) * P.e_ld + n0;  // e_ld is a multiple of 128
+  if (F32E) {
+    float* e = static_cast<float*>(P.e) + base;
+#pragma unroll
+    for (int j = 0; j < HC; j += 8) {
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(x[j + i]);
+      st_global_32B(e + j, v);
+    }
+  } else {
+    __half* e = static_cast<__half*>(P.e) + base;
+#pragma unroll
+    for (int j = 0; j < HC; j += 16) {
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = pack_f16x2(x[j + 2 * i], x[j + 2 * i + 1]);
+      st_global_32B(e + j, v);
+    }
+  }
+}
+
+__device__ __forceinline__ void store_epilogue(const HeadParams& P, float (&x)[HC], int row, int n0, int split) {
+  const int ncols = min(HC, P.N - n0);
+  if (P.splits > 1) {
+    float* o = P.partial + (static_cast<long long>(split) * P.M + row) * P.part_ld + n0;  // part_ld: multiple of 128
+#pragma unroll
+    for (int j = 0; j < HC; j += 8) {
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(x[j + i]);
+      st_global_32B(o + j, v);
+    }
+    return;
+  }
+  const float alpha = __ldg(P.alpha);
+#pragma unroll
+  for (int j = 0; j < HC; ++j) x[j] *= alpha;
+  if (P.cin != nullptr) {
+    const float* ci = P.cin + static_cast<long long>(row) * P.cin_ld + n0;
+    if (P.vec && ncols == HC) {
+#pragma unroll
+      for (int j = 0; j < HC; j += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(ci + j);
+        x[j] += f.x;
+        x[j + 1] += f.y;
+        x[j + 2] += f.z;
+        x[j + 3] += f.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < HC; ++j)
+        if (j < ncols) x[j] += ci[j];
+    }
+  }
+  const long long orow = P.out_rows != nullptr ? __ldg(P.out_rows + P.row0 + row) : row;
+  const long long base = orow * P.out_ld + n0;
+  if (P.out_dtype == PO_F32) {
+    float* o = static_cast<float*>(P.out) + base;
+#pragma unroll
+    for (int j = 0; j < HC; j += 8) {
+      if (P.vec && j + 8 <= ncols) {
+        uint32_t v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(x[j + i]);
+        st_global_32B(o + j, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (j + i < ncols) o[j + i] = x[j + i];
+      }
+    }
+    return;
+  }
+  const bool bf = P.out_dtype == PO_BF16;
+  uint16_t* o = static_cast<uint16_t*>(P.out) + base;
+#pragma unroll
+  for (int j = 0; j < HC; j += 16) {
+    uint32_t v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = bf ? pack_bf16x2(x[j + 2 * i], x[j + 2 * i + 1]) : pack_f16x2(x[j + 2 * i], x[j + 2 * i + 1]);
+    if (P.vec && j + 16 <= ncols) {
+      st_global_32B(o + j, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (j + i < ncols) o[j + i] = static_cast<uint16_t>(v[i / 2] >> (16 * (i & 1)));
+    }
+  }
+}
+
+// ---------------------------------------------------------------- kernel
+template <int KIND, bool A_MN, bool B_MN, int EPI>
+__global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid_constant__ HeadParams P) {
+  using C = PairCfg<KIND, 2>;
+  constexpr int BN = C::BN;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* tiles = smem;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE_BYTES);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* tfull = empty + C::STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
+  uint64_t* sfull = drain + 1;
+  uint64_t* sempty = sfull + kSchedSlots;
+  int* stile = reinterpret_cast<int*>(sempty + kSchedSlots);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(stile + kSchedSlots);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull + a, 1);
+      mbar_init(tempty + a, kPairEpilogueWarps);
+    }
+    mbar_init(drain, 1);
+    for (int i = 0; i < kSchedSlots; ++i) {
+      mbar_init(sfull + i, 1);
+      mbar_init(sempty + i, kSchedReaders);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&P.mapA[0]);
+    prefetch_tensormap(&P.mapB[0]);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_holder, C::TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  cluster_sync();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_holder;
+  const HeadExtent X = head_extent<C>(P);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ------------------------------------------------ TMA producer (both CTAs)
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      uint32_t armed = 0;
+      for (int j = 0; ok; ++j) {
+        int t;
+        if (leader) {
+          const int slot = j % kSchedSlots;
+          if (!mbar_wait_bounded_cluster(sempty + slot, ((j / kSchedSlots) & 1u) ^ 1u, abort_flag, P.err,
+                                         kErrTimeoutProducer))
+            break;
+          t = static_cast<int>(atomicAdd(P.sched, 1u));
+          stile[slot] = t;
+          st_shared_cluster_u32(mapa_shared(smem_u32(stile + slot), 1), static_cast<uint32_t>(t));
+          mbar_arrive(sfull + slot);
+          mbar_arrive_cluster(mapa_shared(smem_u32(sfull + slot), 1));
+        } else {
+          if (!sched_read(sfull, stile, j, abort_flag, P.err, kErrTimeoutProducer, t)) break;
+          sched_release(sempty, j);
+        }
+        if (t >= X.total) break;
+        const HeadTile h = head_tile(P, X, t);
+        const int nk = h.kb1 - h.kb0;
+        const int nv = P.npass * nk;
+        const int arow = h.mt * C::TM + static_cast<int>(rank) * 128;
+        const int brow = h.nt * BN + static_cast<int>(rank) * (BN / 2);
+        for (int v = 0; v < nv; ++v) {
+          const int pass = v / nk;
+          const int k0 = (h.kb0 + v - pass * nk) * C::BK;
+          if (!mbar_wait_bounded(empty + stage, phase ^ 1u, abort_flag, P.err, kErrTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          if (leader) {
+            mbar_arrive_expect_tx(full + stage, 2 * C::STAGE_BYTES);
+            armed = (armed & ~(0x101u << stage)) | (1u << stage) | (phase << (8 + stage));
+          }
+          const uint32_t bar = mapa_shared(smem_u32(full + stage), 0);
+          const CUtensorMap* ma = &P.mapA[pass == 2 ? 1 : 0];
+          const CUtensorMap* mb = &P.mapB[pass == 1 ? 1 : 0];
+          uint8_t* sa = tiles + stage * C::STAGE_BYTES;
+          uint8_t* sb = sa + C::A_BYTES;
+          if (!A_MN) {
+#pragma unroll
+            for (int a = 0; a < C::ATOMS; ++a) tma_load_3d_pair(sa + a * 128 * 128, ma, bar, k0 + a * C::AK, arow, 0);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 128 * C::ES / 128; ++i)
+              tma_load_3d_pair(sa + i * C::BK * 128, ma, bar, arow + i * (128 / C::ES), k0, 0);
+          }
+          if (!B_MN) {
+#pragma unroll
+            for (int a = 0; a < C::ATOMS; ++a)
+              tma_load_3d_pair(sb + a * (BN / 2) * 128, mb, bar, k0 + a * C::AK, brow, 0);
+          } else {
+#pragma unroll
+            for (int i = 0; i < (BN / 2) * C::ES / 128; ++i)
+              tma_load_3d_pair(sb + i * C::BK * 128, mb, bar, brow + i * (128 / C::ES), k0, 0);
+          }
+          if (++stage == C::STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok && leader) {
+        // Once the last arming of each stage completes, no load of either CTA is in flight.
+        for (int s = 0; s < C::STAGES; ++s) {
+          if (!(armed & (1u << s))) continue;
+          const uint32_t par = (armed >> (8 + s)) & 1u;
+          const unsigned long long t0 = global_timer_ns();
+          while (!mbar_try_wait(full + s, par)) {
+            if (global_timer_ns() - t0 > kWaitTimeoutNs) {
+              atomicCAS(P.err, 0, kErrTimeoutDrain);
+              break;
+            }
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      // ------------------------------------------------ MMA issuer (leader CTA)
+      const uint32_t idesc = make_idesc(0, C::TM, BN, A_MN ? 1u : 0u, B_MN ? 1u : 0u) | (P.fmt << 7) | (P.fmt << 10);
+      constexpr uint32_t A_STEP = A_MN ? C::MMA_K * 128 : 32;
+      constexpr uint32_t B_STEP = B_MN ? C::MMA_K * 128 : 32;
+      constexpr uint32_t A_LBO = A_MN ? C::BK * 128 : 16;
+      constexpr uint32_t B_LBO = B_MN ? C::BK * 128 : 16;
+      constexpr bool MN32 = (KIND == KIND_TF32);
+      constexpr uint32_t A_LAY = (A_MN && MN32) ? kSwizzle128BAtom32B : kSwizzle128B;
+      constexpr uint32_t B_LAY = (B_MN && MN32) ? kSwizzle128BAtom32B : kSwizzle128B;
+      constexpr uint32_t A_SBO = (A_MN && MN32) ? 512 : 1024;
+      constexpr uint32_t B_SBO = (B_MN && MN32) ? 512 : 1024;
+      int stage = 0;
+      uint32_t phase = 0;
+      int ucount = 0;  // accumulators filled
+      bool ok = true;
+      for (int j = 0; ok; ++j) {
+        int t;
+        if (!sched_read(sfull, stile, j, abort_flag, P.err, kErrTimeoutMma, t)) break;
+        sched_release(sempty, j);
+        if (t >= X.total) break;
+        const HeadTile h = head_tile(P, X, t);
+        const int nv = P.npass * (h.kb1 - h.kb0);
+        for (int v0 = 0; v0 < nv && ok; v0 += P.chunk, ++ucount) {
+          const int acc = ucount & 1;
+          if (!mbar_wait_bounded_cluster(tempty + acc, ((ucount >> 1) & 1u) ^ 1u, abort_flag, P.err,
+                                         kErrTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t dtmem = tmem_base + static_cast<uint32_t>(acc * BN);
+          const int v1 = min(nv, v0 + P.chunk);
+          for (int v = v0; v < v1; ++v) {
+            if (!mbar_wait_bounded(full + stage, phase, abort_flag, P.err, kErrTimeoutMma)) {
+              ok = false;
+              break;
+            }
+            const uint32_t sa = smem_u32(tiles + stage * C::STAGE_BYTES);
+            const uint32_t sb = sa + C::A_BYTES;
+#pragma unroll
+            for (int ks = 0; ks < C::KSTEPS; ++ks) {
+              constexpr int PER = C::KSTEPS / C::ATOMS;
+              const uint32_t aoff = A_MN ? ks * A_STEP : (ks / PER) * (128 * 128) + (ks % PER) * 32;
+              const uint32_t boff = B_MN ? ks * B_STEP : (ks / PER) * ((BN / 2) * 128) + (ks % PER) * 32;
+              const uint64_t ad = make_sw128_desc(sa + aoff, A_LBO, A_SBO, A_LAY);
+              const uint64_t bd = make_sw128_desc(sb + boff, B_LBO, B_SBO, B_LAY);
+              const uint32_t accumulate = (v > v0 || ks > 0) ? 1u : 0u;
+              if (KIND == KIND_BF16) mma_f16_pair(dtmem, ad, bd, idesc, accumulate);
+              else mma_tf32_pair(dtmem, ad, bd, idesc, accumulate);
+            }
+            mma_commit_pair_mc(empty + stage, 0x3);
+            if (++stage == C::STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+          if (ok) mma_commit_pair_mc(tfull + acc, 0x3);
+        }
+      }
+      mma_commit_pair(drain);
+      const unsigned long long t0 = global_timer_ns();
+      while (!mbar_try_wait(drain, 0)) {
+        if (global_timer_ns() - t0 > kWaitTimeoutNs) {
+          atomicCAS(P.err, 0, kErrTimeoutDrain);
+          break;
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------ epilogue (both CTAs)
+    const int q = warp & 3;
+    const int half = (warp - 2) >> 2;
+    const uint32_t tcol = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * HC);
+    int ucount = 0;
+    bool ok = true;
+    for (int j = 0; ok; ++j) {
+      int t;
+      const bool got = sched_read(sfull, stile, j, abort_flag, P.err, kErrTimeoutEpilogue, t);
+      if (!__all_sync(0xffffffffu, got)) break;
+      __syncwarp();
+      if (lane == 0) sched_release(sempty, j);
+      if (t >= X.total) break;
+      const HeadTile h = head_tile(P, X, t);
+      const int nv = P.npass * (h.kb1 - h.kb0);
+      const int row = h.mt * C::TM + static_cast<int>(rank) * 128 + q * 32 + lane;
+      const int n0 = h.nt * BN + half * HC;
+      const bool live = row < X.m && n0 < P.N;
+      long long tk = 0;
+      int lo = 0, c = 0x7fffffff;
+      if (EPI == HEAD_STATS && live) {
+        // First target of this row at or after column n0.
+        tk = static_cast<long long>(__ldg(P.rowmap + P.row0 + row)) * P.top;
+        int hi = P.top;
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (__ldg(P.ent + tk + mid) < n0) lo = mid + 1;
+          else hi = mid;
+        }
+        if (lo < P.top) c = __ldg(P.ent + tk + lo) - n0;
+      }
+      float x[HC];
+#pragma unroll
+      for (int i = 0; i < HC; ++i) x[i] = 0.0f;
+      for (int v0 = 0; v0 < nv; v0 += P.chunk, ++ucount) {
+        const int acc = ucount & 1;
+        const bool ready =
+            mbar_wait_bounded_sleep(tfull + acc, (ucount >> 1) & 1u, abort_flag, P.err, kErrTimeoutEpilogue);
+        if (!__all_sync(0xffffffffu, ready)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+#pragma unroll
+        for (int i = 0; i < HC / 32; ++i) {
+          uint32_t r[32];
+          tmem_ld_32x32(tcol + static_cast<uint32_t>(acc * BN + i * 32), r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) x[32 * i + k] += __uint_as_float(r[k]);
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(tempty + acc), 0));
+      }
+      if (!ok) break;
+      if (EPI == HEAD_STATS) {
+        stats_epilogue<KIND == KIND_TF32>(P, x, live, row, n0, 2 * h.nt + half, tk, lo, c);
+        __syncwarp();
+      } else if (live) {
+        store_epilogue(P, x, row, n0, h.split);
+      }
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before_sync();
+  cluster_sync();  // every MMA drained and every TMEM read done in both CTAs
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
+  }
+  if (threadIdx.x == 0) {
+    // The last CTA to finish re-arms the queue for the next launch.
+    __threadfence();
+    if (atomicAdd(P.sched + 1, 1u) == gridDim.x - 1) {
+      atomicExch(P.sched, 0u);
+      atomicExch(P.sched + 1, 0u);
+    }
+  }
+}
+
+// The tile counts here are upper bounds: the kernel reads the real extent.
+template <int KIND, bool A_MN, bool B_MN, int EPI>
+int launch_head(const HeadParams& P, int max_tiles, cudaStream_t stream) {
+  using C = PairCfg<KIND, 2>;
+  auto kern = head_gemm_kernel<KIND, A_MN, B_MN, EPI>;
+  static int max_pairs[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return set_error(PO_ERR_CUDA, "device ordinal out of range");
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kGemmThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (max_pairs[dev] == 0) {
+    int r = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES),
+                       "cudaFuncSetAttribute");
+    if (r) return r;
+    cfg.gridDim = dim3(2 * (sm_count() / 2), 1, 1);
+    int n = 0;
+    r = check_cuda(cudaOccupancyMaxActiveClusters(&n, kern, &cfg), "cudaOccupancyMaxActiveClusters");
+    if (r) return r;
+    if (n <= 0) return set_error(PO_ERR_CUDA, "loss head: no cluster of two CTAs fits on this device");
+    max_pairs[dev] = n;
+  }
+  const int pairs = max_tiles < max_pairs[dev] ? max_tiles : max_pairs[dev];
+  cfg.gridDim = dim3(2 * pairs, 1, 1);
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, P), "loss head launch");
+}
+
+// logits + statistics (both operands K-major); dH = dZ W (W MN-major); dW = dZ^T H (both MN-major).
+enum HeadProduct : int { HEAD_LOGITS = 0, HEAD_DHIDDEN = 1, HEAD_DWEIGHT = 2 };
+template <int KIND>
+int dispatch_head(int product, const HeadParams& P, int max_tiles, cudaStream_t s) {
+  if (product == HEAD_LOGITS) return launch_head<KIND, false, false, HEAD_STATS>(P, max_tiles, s);
+  if (product == HEAD_DHIDDEN) return launch_head<KIND, false, true, HEAD_STORE>(P, max_tiles, s);
+  return launch_head<KIND, true, true, HEAD_STORE>(P, max_tiles, s);
+}
+extern template int dispatch_head<KIND_BF16>(int, const HeadParams&, int, cudaStream_t);
+extern template int dispatch_head<KIND_TF32>(int, const HeadParams&, int, cudaStream_t);
+
+}  // namespace po

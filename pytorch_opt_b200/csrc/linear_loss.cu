@@ -1,0 +1,959 @@
+// Losses of a linear head over a large vocabulary, with their gradients:
+// softmax cross entropy against a target, and the divergence from a teacher's
+// top logits (po_linear_loss).
+//
+//   z = H W^T,  l_t = loss(z_t),  dZ = dl/dz,  dH = dZ W,  dW = dZ^T H
+//
+// Launches of one call (T rows, V vocabulary, D features):
+//   targets  a teacher's rows only: q, sum q log q, indices sorted; row status
+//   pack     counted rows of H packed together (a row that counts for nothing
+//            costs no product, and whatever it holds reaches no sum); their
+//            number stays on the device
+//   logits   tensor-core product, softmax statistics in its epilogue
+//            (head_gemm.cuh): 2 T V D operations
+//   finish   joins each row's V / 128 statistics, writes the losses
+// and with gradients
+//   rescale  exp(z - max of 128 columns) -> dZ in the products' type, in place:
+//            one read and one write of T V 2-byte values
+//   dH, dW   two more products of 2 T V D operations
+// The products bound all but the smallest calls (6 T V D operations with
+// gradients). Taking the softmax apart into the tile-local exponential and a
+// late factor is what makes the logits' product run once: dZ needs each row's
+// sum over the whole vocabulary, which is known only after all tiles, and the
+// alternative to the rescale pass (4 bytes a logit) is computing the logits
+// again (2 D operations a logit).
+//
+// Nothing here allocates, synchronises or depends on timing: partial sums are
+// joined in a fixed order.
+#include <cudaTypedefs.h>
+
+#include <climits>
+#include <cmath>
+#include <cstring>
+#include <mutex>
+
+#include "head_gemm.cuh"
+#include "losses.cuh"
+
+namespace po {
+namespace {
+
+// Rows of packed operands are zero up to a multiple of this (a K block of the
+// 16-bit products), so that dW's last K block adds nothing.
+constexpr int kRowPad = 128;
+// Values of the fp16 gradient operand are 2^10 of dZ / upstream: |dZ| is at
+// most 1 + 2 z_loss lse, and softmax values down to 6e-8 stay normal. bf16
+// and tf32 have fp32's range and need no factor.
+constexpr float kF16Scale = 1024.0f;
+
+// Device-side state of a call.
+struct CallState {
+  int count;         // counted rows
+  int counted_mean;  // rows that the mean divides by
+  int done;          // blocks of the finishing kernel that are through
+  float alpha;       // factor of the gradient products
+  float grad_max;    // max |row_grad|
+};
+
+struct Targets {
+  const long long* index;
+  long long index_ld;
+  const void* teacher;
+  long long teacher_ld;
+  int teacher_dtype;
+  int top;
+  long long ignore_index;
+};
+
+// ---------------------------------------------------------------- targets
+// One block a row: q = softmax(teacher / a) over the entries with index >= 0,
+// sum q log q, and (index, q) sorted by index (a bitonic network over `width`
+// = the next power of two; empty entries sort last as INT_MAX, q = 0).
+__global__ void teacher_targets_kernel(Targets tg, long long V, float inv_temp, int width, int* __restrict__ status,
+                                       int* __restrict__ ent, float* __restrict__ q, float* __restrict__ qlogq) {
+  extern __shared__ float sm[];
+  int* si = reinterpret_cast<int*>(sm);
+  float* sl = sm + width;
+  __shared__ float buf[32];
+  const long long t = blockIdx.x;
+  float m = -INFINITY;
+  bool bad = false, nan = false;
+  for (int k = threadIdx.x; k < width; k += blockDim.x) {
+    int i = INT_MAX;
+    float l = -INFINITY;
+    if (k < tg.top) {
+      const long long x = tg.index[t * tg.index_ld + k];
+      if (x >= V) bad = true;
+      else if (x >= 0) {
+        i = static_cast<int>(x);
+        l = load_as_f32(tg.teacher, tg.teacher_dtype, t * tg.teacher_ld + k) * inv_temp;
+        nan |= isnan(l);
+      }
+    }
+    si[k] = i;
+    sl[k] = l;
+    m = fmaxf(m, l);
+  }
+  bad = __syncthreads_or(bad);
+  nan = __syncthreads_or(nan);
+  m = block_max(m, buf);
+  const int st = bad ? ROW_BAD : (m > -INFINITY || nan ? ROW_COUNTED : ROW_IGNORED);
+  float sum = 0.0f;
+  for (int k = threadIdx.x; k < width; k += blockDim.x)
+    if (si[k] != INT_MAX) sum += expf(sl[k] - m);
+  sum = block_sum(sum, buf);
+  const float logsum = logf(sum);
+  float c = 0.0f;
+  for (int k = threadIdx.x; k < width; k += blockDim.x) {
+    float p = 0.0f;
+    if (si[k] != INT_MAX && st == ROW_COUNTED) {
+      const float lq = sl[k] - m - logsum;
+      p = expf(sl[k] - m) / sum;
+      if (p != 0.0f) c += p * lq;  // NaN passes
+    }
+    sl[k] = p;
+  }
+  c = block_sum(c, buf);
+  if (threadIdx.x == 0) {
+    status[t] = st;
+    qlogq[t] = c;
+  }
+  // Sort by index; the network is fixed, so equal indices land the same way each time.
+  for (int size = 2; size <= width; size <<= 1) {
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      __syncthreads();
+      for (int k = threadIdx.x; k < width / 2; k += blockDim.x) {
+        const int a = 2 * k - (k & (stride - 1)), b = a + stride;
+        const bool up = (a & size) == 0;
+        const int ia = si[a], ib = si[b];
+        if ((ia > ib) == up && ia != ib) {
+          si[a] = ib;
+          si[b] = ia;
+          const float f = sl[a];
+          sl[a] = sl[b];
+          sl[b] = f;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < tg.top; k += blockDim.x) {
+    ent[t * tg.top + k] = si[k];
+    q[t * tg.top + k] = sl[k];
+  }
+}
+
+// max |row_grad| into state->grad_max (1 when there is nothing to scale by).
+__global__ void grad_max_kernel(const float* __restrict__ g, long long T, CallState* st) {
+  __shared__ float buf[32];
+  float m = 0.0f;
+  for (long long t = threadIdx.x; t < T; t += blockDim.x) m = fmaxf(m, fabsf(g[t]));
+  m = block_max(m, buf);
+  if (threadIdx.x == 0) st->grad_max = (m > 0.0f && m < INFINITY) ? m : 1.0f;
+}
+
+// ------------------------------------------------------------------- pack
+struct PackArgs {
+  const void* hidden;
+  long long h_ld;
+  long long T;
+  int D, ldp;  // packed pitch (elements)
+  int vec;     // 16-byte rows on both sides
+  Targets tg;
+  long long V;
+  const int* status;  // teacher's rows (nullable: decided by the target here)
+  int* ent;           // targets (written here without a teacher)
+  int* rowmap;
+  void* packed;
+  float* packed_lo;  // fp32: low halves of the tf32 pairs
+  long long rows_alloc;
+  void* dhidden;
+  long long dh_ld;
+  float* loss_rows;
+  CallState* st;
+  unsigned int* sched;
+  float alpha;
+  int mean, has_row_grad;
+};
+
+__device__ __forceinline__ int row_status(const PackArgs& a, long long t, int& target) {
+  if (a.status != nullptr) return a.status[t];
+  const long long y = a.tg.index[t * a.tg.index_ld];
+  if (y == a.tg.ignore_index) return ROW_IGNORED;
+  if (y < 0 || y >= a.V) return ROW_BAD;
+  target = static_cast<int>(y);
+  return ROW_COUNTED;
+}
+
+__device__ __forceinline__ float tf32_rna(float v) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
+  return __uint_as_float(r);
+}
+
+constexpr int kPackRows = 32;
+
+// A block takes 32 rows; their places follow from the number of counted rows
+// before them, which it counts itself (T statuses, read from L2) instead of
+// waiting for another launch.
+template <int DT>
+__global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
+  using T = typename ElemOf<DT>::T;
+  __shared__ int buf[32];
+  __shared__ int s_place[kPackRows];
+  const long long first = static_cast<long long>(blockIdx.x) * kPackRows;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int before = 0, bad_before = 0, y = 0;
+  const bool last = blockIdx.x == gridDim.x - 1;
+  for (long long t = threadIdx.x; t < first; t += blockDim.x) {
+    const int s = row_status(a, t, y);
+    before += s == ROW_COUNTED;
+    bad_before += s == ROW_BAD;
+  }
+  before = block_sum(before, buf);
+  if (last) bad_before = block_sum(bad_before, buf);
+  if (warp == 0) {
+    const long long t = first + lane;
+    int s = ROW_IGNORED;
+    if (t < a.T) s = row_status(a, t, y);
+    const unsigned votes = __ballot_sync(0xffffffffu, s == ROW_COUNTED);
+    const unsigned bad = __ballot_sync(0xffffffffu, s == ROW_BAD);
+    const int place = before + __popc(votes & ((1u << lane) - 1u));
+    s_place[lane] = s == ROW_COUNTED ? place : -1;
+    if (s == ROW_COUNTED) {
+      a.rowmap[place] = static_cast<int>(t);
+      if (a.status == nullptr) a.ent[t] = y;
+    } else if (t < a.T) {
+      a.loss_rows[t] = s == ROW_BAD ? NAN : 0.0f;
+      if (a.status == nullptr) a.ent[t] = INT_MAX;
+    }
+    if (last && lane == 0) {
+      const int n = before + __popc(votes), all = n + bad_before + __popc(bad);
+      a.st->count = n;
+      a.st->counted_mean = all;
+      a.st->done = 0;
+      float alpha = a.alpha;
+      if (a.mean) alpha /= static_cast<float>(all > 0 ? all : 1);
+      if (a.has_row_grad) alpha *= a.st->grad_max;
+      a.st->alpha = alpha;
+      buf[0] = n;
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x < 2) a.sched[threadIdx.x] = 0u;
+  __syncthreads();
+  T zero;
+  from_f32(0.0f, zero);
+  for (int r = warp; r < kPackRows; r += blockDim.x >> 5) {
+    const long long t = first + r;
+    if (t >= a.T) break;
+    const int place = s_place[r];
+    if (place < 0) {
+      if (a.dhidden != nullptr) {
+        T* o = static_cast<T*>(a.dhidden) + t * a.dh_ld;
+        for (int i = lane; i < a.D; i += 32) o[i] = zero;
+      }
+      continue;
+    }
+    const T* src = static_cast<const T*>(a.hidden) + t * a.h_ld;
+    T* dst = static_cast<T*>(a.packed) + static_cast<long long>(place) * a.ldp;
+    if (DT == PO_F32) {
+      float* lo = a.packed_lo + static_cast<long long>(place) * a.ldp;
+      for (int i = lane; i < a.D; i += 32) {
+        const float v = to_f32(src[i]), h = tf32_rna(v);
+        from_f32(h, dst[i]);
+        lo[i] = tf32_rna(v - h);
+      }
+    } else if (a.vec) {
+      for (int i = lane; i < a.D / 8; i += 32)
+        reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
+    } else {
+      for (int i = lane; i < a.D; i += 32) dst[i] = src[i];
+    }
+  }
+  if (last) {  // zero rows that complete dW's last K block
+    const long long n = buf[0];
+    long long end = (n + kRowPad - 1) / kRowPad * kRowPad;
+    if (end > a.rows_alloc) end = a.rows_alloc;
+    for (long long i = n * a.ldp + threadIdx.x; i < end * a.ldp; i += blockDim.x) {
+      static_cast<T*>(a.packed)[i] = zero;
+      if (DT == PO_F32) a.packed_lo[i] = 0.0f;
+    }
+  }
+}
+
+// Copy of W with a pitch that TMA takes (16-bit), or as tf32 (hi, lo) pairs.
+template <int DT>
+__global__ void __launch_bounds__(256) stage_weight_kernel(const void* w, long long w_ld, long long V, int D, int ldp,
+                                                           void* out, float* lo) {
+  using T = typename ElemOf<DT>::T;
+  for (long long v = blockIdx.x; v < V; v += gridDim.x) {
+    const T* src = static_cast<const T*>(w) + v * w_ld;
+    T* dst = static_cast<T*>(out) + v * ldp;
+    for (int i = threadIdx.x; i < D; i += blockDim.x) {
+      if (DT == PO_F32) {
+        const float x = to_f32(src[i]), h = tf32_rna(x);
+        from_f32(h, dst[i]);
+        lo[v * ldp + i] = tf32_rna(x - h);
+      } else {
+        dst[i] = src[i];
+      }
+    }
+  }
+}
+
+// ----------------------------------------------------------------- finish
+struct FinishArgs {
+  const float2* part;
+  const float* zsum;
+  int nparts;
+  int row0;
+  const int* rowmap;
+  const float* zpick;
+  const int* ent;
+  const float* q;      // nullable: hard targets
+  const float* qlogq;
+  int top;
+  float smoothing, z_loss, temperature, inv_vocab;
+  float4* stat;        // [row of this launch] max, 1 / sum, log2 sum 2^z2
+  float* loss_rows;
+  float* loss;         // nullable; written by the last block of the last launch
+  long long T;
+  int mean, final_launch;
+  CallState* st;
+};
+
+// One block a packed row: lse = log2 sum 2^z2 from the row's partial
+// statistics, and the loss; the last block to finish sums the losses of all
+// rows in a fixed order (fp64).
+__global__ void __launch_bounds__(128) finish_kernel(FinishArgs a) {
+  __shared__ float buf[32];
+  __shared__ double dbuf[32];
+  __shared__ int s_last;
+  const int row = blockIdx.x;
+  if (a.row0 + row < a.st->count) {
+    const float2* p = a.part + static_cast<long long>(row) * a.nparts;
+    float m = -INFINITY, s = 0.0f;
+    for (int i = threadIdx.x; i < a.nparts; i += blockDim.x) {
+      const float2 v = p[i];
+      if (v.x > m) {
+        s *= ex2(m - v.x);
+        m = v.x;
+      }
+      s += v.x == -INFINITY ? v.y : v.y * ex2(v.x - m);  // an empty part holds 0, or a NaN to keep
+    }
+    const float mm = block_max(m, buf);
+    s = block_sum(m == -INFINITY ? s : s * ex2(m - mm), buf);
+    const float log2s = log2f(s), lse2 = mm + log2s;
+    const long long t = a.rowmap[a.row0 + row];
+    float zs = 0.0f;
+    if (a.zsum != nullptr) {
+      for (int i = threadIdx.x; i < a.nparts; i += blockDim.x) zs += a.zsum[static_cast<long long>(row) * a.nparts + i];
+      zs = block_sum(zs, buf);
+    }
+    float loss;
+    if (a.q == nullptr) {
+      const float lse = lse2 * kLn2;
+      loss = kLn2 * ((mm - a.zpick[t]) + log2s) + a.z_loss * lse * lse;
+      if (a.smoothing != 0.0f) loss += a.smoothing * (kLn2 * a.zpick[t] - zs * a.inv_vocab);
+    } else {
+      float c = 0.0f;
+      for (int k = threadIdx.x; k < a.top; k += blockDim.x) {
+        const float q = a.q[t * a.top + k];
+        if (q != 0.0f) c += q * ((mm - a.zpick[t * a.top + k]) + log2s);
+      }
+      c = block_sum(c, buf);
+      loss = a.temperature * a.temperature * (a.qlogq[t] + kLn2 * c);
+    }
+    if (threadIdx.x == 0) {
+      a.stat[row] = make_float4(mm, 1.0f / s, lse2, 0.0f);
+      a.loss_rows[t] = loss;
+    }
+  }
+  if (a.loss == nullptr || !a.final_launch) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = atomicAdd(&a.st->done, 1) == static_cast<int>(gridDim.x) - 1;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  double sum = 0.0;
+  for (long long t = threadIdx.x; t < a.T; t += blockDim.x) sum += static_cast<double>(__ldcg(a.loss_rows + t));
+  sum = block_sum(sum, dbuf);
+  if (threadIdx.x == 0) {
+    if (a.mean) sum /= static_cast<double>(a.st->counted_mean > 0 ? a.st->counted_mean : 1);
+    *a.loss = static_cast<float>(sum);
+  }
+}
+
+// ---------------------------------------------------------------- rescale
+struct RescaleArgs {
+  void* e;        // fp16 (fp32) in, dZ of the operand type out
+  float* lo;      // fp32: low halves
+  long long e_ld;
+  long long V;
+  const float2* part;
+  int nparts;
+  const float4* stat;
+  int row0, rows;
+  const int* rowmap;
+  const int* ent;
+  const float* q;
+  const float* zpick;
+  int top;
+  const float* row_grad;  // nullable
+  float smoothing, z_loss, inv_vocab, scale;
+  const CallState* st;
+};
+
+constexpr int kSegment = 8192;  // columns a block rescales
+
+template <int DT>
+__device__ __forceinline__ void put_dz(const RescaleArgs& a, long long off, float v) {
+  if (DT == PO_F32) {
+    const float h = tf32_rna(v);
+    static_cast<float*>(a.e)[off] = h;
+    a.lo[off] = tf32_rna(v - h);
+  } else {
+    typename ElemOf<DT>::T o;
+    from_f32(v, o);
+    static_cast<typename ElemOf<DT>::T*>(a.e)[off] = o;
+  }
+}
+
+// dZ = w ((1 + 2 c lse) p - s/V - target distribution), w the row's share of
+// the upstream gradient; the constant upstream factor is in the products'
+// alpha, so that rounding dZ to 16 bits sees w = 1 in all but the per-row
+// case. Bound by memory: 4 bytes a logit in 16-bit types.
+template <int DT>
+__global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
+  const int row = blockIdx.x / nseg;
+  const int seg = blockIdx.x - row * nseg;
+  const int left = a.st->count - a.row0;
+  const long long base = static_cast<long long>(row) * a.e_ld;
+  const int c0 = seg * kSegment;
+  const int c1 = min(static_cast<long long>(c0) + kSegment, a.e_ld);
+  if (row >= left) {
+    if (left <= 0 || row >= (left + kRowPad - 1) / kRowPad * kRowPad) return;
+    for (int c = c0 + threadIdx.x; c < c1; c += blockDim.x) put_dz<DT>(a, base + c, 0.0f);
+    return;
+  }
+  const long long t = a.rowmap[a.row0 + row];
+  const float4 stat = a.stat[row];
+  const float mm = stat.x;
+  const float w = a.scale * (a.row_grad != nullptr ? a.row_grad[t] / a.st->grad_max : 1.0f);
+  const float coef = w * (1.0f + 2.0f * a.z_loss * kLn2 * stat.z);
+  const float pcoef = coef * stat.y;
+  const float flat = w * a.smoothing * a.inv_vocab;
+  const float2* part = a.part + static_cast<long long>(row) * a.nparts;
+  if (DT == PO_F32) {
+#pragma unroll 2
+    for (int c = c0 + threadIdx.x * 4; c < c1; c += 256 * 4) {
+      const float m = part[c >> 7].x;
+      const float f = m == -INFINITY ? (pcoef == pcoef ? 0.0f : pcoef) : pcoef * ex2(m - mm);
+      const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(a.e) + base + c);
+      const float x[4] = {fmaf(v.x, f, -flat), fmaf(v.y, f, -flat), fmaf(v.z, f, -flat), fmaf(v.w, f, -flat)};
+      float4 h, l;
+      h.x = tf32_rna(x[0]), l.x = tf32_rna(x[0] - h.x);
+      h.y = tf32_rna(x[1]), l.y = tf32_rna(x[1] - h.y);
+      h.z = tf32_rna(x[2]), l.z = tf32_rna(x[2] - h.z);
+      h.w = tf32_rna(x[3]), l.w = tf32_rna(x[3] - h.w);
+      *reinterpret_cast<float4*>(static_cast<float*>(a.e) + base + c) = h;
+      *reinterpret_cast<float4*>(a.lo + base + c) = l;
+    }
+  } else {
+    uint4 raw[4];
+    float ms[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = c0 + (i * 256 + static_cast<int>(threadIdx.x)) * 8;
+      if (c < c1) {
+        raw[i] = *reinterpret_cast<const uint4*>(static_cast<const __half*>(a.e) + base + c);
+        ms[i] = part[c >> 7].x;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = c0 + (i * 256 + static_cast<int>(threadIdx.x)) * 8;
+      if (c >= c1) break;
+      const float m = ms[i];
+      const float f = m == -INFINITY ? (pcoef == pcoef ? 0.0f : pcoef) : pcoef * ex2(m - mm);
+      const __half2* hv = reinterpret_cast<const __half2*>(&raw[i]);
+      uint32_t o[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 v = __half22float2(hv[k]);
+        const float x0 = fmaf(v.x, f, -flat), x1 = fmaf(v.y, f, -flat);
+        o[k] = DT == PO_BF16 ? pack_bf16x2(x0, x1) : pack_f16x2(x0, x1);
+      }
+      *reinterpret_cast<uint4*>(static_cast<__half*>(a.e) + base + c) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  }
+  // The targets' columns again, with the target distribution taken off before
+  // the one rounding (p from the fp32 logit).
+  __syncthreads();
+  for (int k = threadIdx.x; k < a.top; k += blockDim.x) {
+    const int* ent = a.ent + t * a.top;
+    const int c = ent[k];
+    if (c < c0 || c >= c1 || (k > 0 && ent[k - 1] == c)) continue;
+    float goal = 0.0f;
+    if (a.q == nullptr) goal = 1.0f - a.smoothing;
+    else
+      for (int j = k; j < a.top && ent[j] == c; ++j) goal += a.q[t * a.top + j];
+    put_dz<DT>(a, base + c, pcoef * ex2(a.zpick[t * a.top + k] - mm) - flat - w * goal);
+  }
+}
+
+// ------------------------------------------------------------------- join
+// out[rows[row0 + r] or r][c] = alpha sum_s partial[s][r][c], in order of s.
+template <int DT>
+__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ partial, int splits, int M, long long pld,
+                                                   int N, const float* alpha, const int* count, int row0, int limit_rows,
+                                                   const int* rows, void* out, long long ld) {
+  const int r = blockIdx.x;
+  if (limit_rows && row0 + r >= *count) return;
+  const float al = *alpha;
+  typename ElemOf<DT>::T* o =
+      static_cast<typename ElemOf<DT>::T*>(out) + (rows != nullptr ? rows[row0 + r] : r) * ld;
+  for (int c = (blockIdx.y * 256 + threadIdx.x) * 4; c < N; c += gridDim.y * 1024) {
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k = 0; k < splits; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(partial + (static_cast<long long>(k) * M + r) * pld + c);
+      s.x += v.x;
+      s.y += v.y;
+      s.z += v.z;
+      s.w += v.w;
+    }
+    const float x[4] = {s.x * al, s.y * al, s.z * al, s.w * al};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < N) from_f32(x[i], o[c + i]);
+  }
+}
+
+// Zeroes a rows x cols matrix (no counted row can reach it).
+template <int DT>
+__global__ void zero_kernel(void* out, long long ld, long long rows, long long cols) {
+  typename ElemOf<DT>::T z;
+  from_f32(0.0f, z);
+  for (long long r = blockIdx.x; r < rows; r += gridDim.x)
+    for (long long c = threadIdx.x; c < cols; c += blockDim.x)
+      static_cast<typename ElemOf<DT>::T*>(out)[r * ld + c] = z;
+}
+
+// ------------------------------------------------------------------- host
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// rows x cols matrix of `dtype`, pitch ld; boxes of box_cols x box_rows, zeros outside.
+int encode(CUtensorMap* map, const void* ptr, int dtype, long long rows, long long cols, long long ld, int box_cols,
+           int box_rows, bool mn) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return set_error(PO_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const int es = dtype_size(dtype);
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), 1};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * es), static_cast<cuuint64_t>(ld * es * rows)};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapDataType t = dtype == PO_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : dtype == PO_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUtensorMapSwizzle swz =
+      mn && es == 4 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B;
+  const CUresult r = fn(map, t, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? PO_OK : set_error(PO_ERR_CUDA, "linear_loss: cuTensorMapEncodeTiled failed");
+}
+
+// One operand of a product: hi (and lo) matrices, stored K-major [MN][K] or
+// MN-major [K][MN].
+struct HeadOperand {
+  const void* p[2];
+  int dtype;
+  long long rows, cols, ld;
+  bool kmajor;
+};
+
+int encode_operand(CUtensorMap map[2], const HeadOperand& o) {
+  const int es = dtype_size(o.dtype);
+  const int w = 128 / es;
+  for (int i = 0; i < 2; ++i) {
+    const void* p = o.p[i] != nullptr ? o.p[i] : o.p[0];
+    // K-major: 128 bytes of K x 128 rows; MN-major: 128 bytes of MN x a stage's 2 w rows of K.
+    const int r = o.kmajor ? encode(&map[i], p, o.dtype, o.rows, o.cols, o.ld, w, 128, false)
+                           : encode(&map[i], p, o.dtype, o.rows, o.cols, o.ld, w, 2 * w, true);
+    if (r) return r;
+  }
+  return PO_OK;
+}
+
+// Splits of K for a store product: the tiles' waves over the pairs, each tile
+// paying its K blocks and about 3 more to fill and drain, plus the join's
+// traffic (8 bytes a value and split at ~5 TB/s, in blocks of ~0.6 us).
+int choose_splits(long long tiles, int nkb, long long M, long long N) {
+  const long long pairs = sm_count() / 2;
+  int best = 1;
+  double best_cost = 1e300;
+  for (int s = 1; s <= 32 && s <= (nkb + 3) / 4; ++s) {
+    const double waves = static_cast<double>((tiles * s + pairs - 1) / pairs);
+    double cost = waves * (static_cast<double>((nkb + s - 1) / s) + 3.0);
+    if (s > 1) cost += 5.0 + static_cast<double>(s) * static_cast<double>(M) * static_cast<double>(N) * 8.0 / 3.0e6;
+    if (cost < best_cost * 0.98) {
+      best_cost = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+// Sizes and places of one call.
+struct Plan {
+  long long T, D, V, top;
+  int dtype, es;
+  bool f32, soft, grads, want_dh, want_dw;
+  long long chunk;    // rows a pass of the products takes
+  int nchunks;
+  long long rows_alloc;
+  long long ldp;      // pitch of packed H and staged W
+  bool stage_w;
+  int nparts;
+  long long e_ld;
+  int bk;
+  int splits_dh, splits_dw;
+  bool dw_acc;
+  // workspace
+  CallState* st;
+  unsigned int* sched;
+  int* rowmap;
+  int* status;
+  int* ent;
+  float* q;
+  float* qlogq;
+  float* zpick;
+  float4* stat;
+  float2* part;
+  float* zsum;
+  void* packed;
+  float* packed_lo;
+  void* w;
+  float* w_lo;
+  void* e;
+  float* e_lo;
+  float* partial;
+  float* dw_accum;
+  size_t bytes;
+};
+
+// Rows a pass keeps in the workspace by default: as many as leave 2 GiB of
+// exponentials (8191 rows of 128 thousand columns in 16 bits).
+constexpr long long kDefaultChunkBytes = 2LL << 30;
+
+int make_plan(Plan& p, const void* weight, long long w_ld, int dtype, long long T, long long D, long long V,
+              long long top, bool soft, bool want_dh, bool want_dw, long long chunk_rows, void* ws, size_t ws_bytes) {
+  memset(&p, 0, sizeof(p));
+  p.T = T, p.D = D, p.V = V, p.top = top, p.dtype = dtype, p.es = dtype_size(dtype);
+  p.f32 = dtype == PO_F32;
+  p.soft = soft;
+  p.want_dh = want_dh, p.want_dw = want_dw, p.grads = want_dh || want_dw;
+  p.ldp = round_up(D, 64);
+  p.stage_w = p.f32 || reinterpret_cast<uintptr_t>(weight) % 16 != 0 || (w_ld * p.es) % 16 != 0;
+  p.nparts = cdiv(V, 128);
+  p.e_ld = round_up(V, 128);
+  p.bk = p.f32 ? 64 : 128;
+  long long most = chunk_rows;
+  if (most <= 0) {
+    // Without gradients a row leaves 8 bytes per 128 columns.
+    const long long per_row = p.grads ? p.e_ld * (p.f32 ? 8 : 2) : static_cast<long long>(p.nparts) * 8;
+    most = kDefaultChunkBytes / per_row;
+  }
+  most = most / 256 * 256;
+  if (most < 256) most = 256;
+  p.nchunks = static_cast<int>((T + most - 1) / most);
+  p.chunk = p.nchunks == 1 ? T : round_up((T + p.nchunks - 1) / p.nchunks, 256);
+  p.rows_alloc = round_up(T, kRowPad);
+  const long long mt = (p.chunk + 255) / 256, nd = (D + 255) / 256, nv = (V + 255) / 256;
+  const int npass = p.f32 ? 3 : 1;
+  p.splits_dh = want_dh ? choose_splits(mt * nd, npass * cdiv(V, p.bk), p.chunk, D) : 1;
+  p.dw_acc = want_dw && p.nchunks > 1;
+  p.splits_dw = want_dw && !p.dw_acc ? choose_splits(nv * nd, npass * cdiv(p.chunk, p.bk), V, D) : 1;
+
+  Arena ar(ws, ws_bytes);
+  auto i32 = [&](long long n) { return static_cast<int*>(ar.take(static_cast<size_t>(n) * 4)); };
+  auto f32 = [&](long long n) { return static_cast<float*>(ar.take(static_cast<size_t>(n) * 4)); };
+  p.st = static_cast<CallState*>(ar.take(sizeof(CallState)));
+  p.sched = static_cast<unsigned int*>(ar.take(8));
+  p.rowmap = i32(T);
+  p.ent = i32(T * top);
+  p.zpick = f32(T * top);
+  if (soft) {
+    p.status = i32(T);
+    p.q = f32(T * top);
+    p.qlogq = f32(T);
+  }
+  p.stat = static_cast<float4*>(ar.take(static_cast<size_t>(p.chunk) * 16));
+  p.part = static_cast<float2*>(ar.take(static_cast<size_t>(p.chunk) * p.nparts * 8));
+  p.zsum = f32(soft ? 1 : p.chunk * p.nparts);
+  p.packed = ar.take(static_cast<size_t>(p.rows_alloc) * p.ldp * p.es);
+  if (p.f32) p.packed_lo = f32(p.rows_alloc * p.ldp);
+  if (p.stage_w) {
+    p.w = ar.take(static_cast<size_t>(V) * p.ldp * p.es);
+    if (p.f32) p.w_lo = f32(V * p.ldp);
+  }
+  if (p.grads) {
+    const long long rows = round_up(p.chunk, kRowPad);
+    p.e = ar.take(static_cast<size_t>(rows) * p.e_ld * p.es);
+    if (p.f32) p.e_lo = f32(rows * p.e_ld);
+    const long long pld = round_up(D, 128);
+    long long partial = 0;
+    if (p.splits_dh > 1) partial = p.splits_dh * p.chunk * pld;
+    if (p.splits_dw > 1 && p.splits_dw * V * pld > partial) partial = p.splits_dw * V * pld;
+    if (partial > 0) p.partial = f32(partial);
+    if (p.dw_acc && !p.f32) p.dw_accum = f32(V * round_up(D, 8));
+  }
+  p.bytes = ar.used;
+  return ar.overflow() ? set_error(PO_ERR_WORKSPACE, "linear_loss: workspace too small") : PO_OK;
+}
+
+int join(int dtype, const float* partial, int splits, int M, long long pld, int N, const Plan& p, int row0,
+         bool limit_rows, const int* rows, void* out, long long ld, cudaStream_t s) {
+  const dim3 grid(M, N > 4096 ? 4 : 1);
+  if (dtype == PO_F32)
+    join_kernel<PO_F32><<<grid, 256, 0, s>>>(partial, splits, M, pld, N, &p.st->alpha, &p.st->count, row0, limit_rows, rows, out, ld);
+  else if (dtype == PO_BF16)
+    join_kernel<PO_BF16><<<grid, 256, 0, s>>>(partial, splits, M, pld, N, &p.st->alpha, &p.st->count, row0, limit_rows, rows, out, ld);
+  else
+    join_kernel<PO_F16><<<grid, 256, 0, s>>>(partial, splits, M, pld, N, &p.st->alpha, &p.st->count, row0, limit_rows, rows, out, ld);
+  return check_cuda(cudaGetLastError(), "linear_loss join");
+}
+
+int run_head(const Plan& p, int product, HeadParams& P, const HeadOperand& A, const HeadOperand& B, int splits,
+             cudaStream_t s) {
+  int r;
+  if ((r = encode_operand(P.mapA, A))) return r;
+  if ((r = encode_operand(P.mapB, B))) return r;
+  P.count = &p.st->count;
+  P.sched = p.sched;
+  P.err = device_error_word();
+  if (P.err == nullptr) return set_error(PO_ERR_CUDA, "device error word unavailable");
+  P.fmt = p.f32 ? 2u : (p.dtype == PO_BF16 ? 1u : 0u);
+  P.npass = p.f32 ? 3 : 1;
+  P.splits = splits;
+  P.tiles_n = cdiv(P.N, 256);
+  const int tiles_m = cdiv(P.M, 256);
+  const long long tiles = static_cast<long long>(tiles_m) * P.tiles_n * splits;
+  if (tiles > INT_MAX / 2) return set_error(PO_ERR_ARG, "linear_loss: too many tiles");
+  return p.f32 ? dispatch_head<KIND_TF32>(product, P, static_cast<int>(tiles), s)
+               : dispatch_head<KIND_BF16>(product, P, static_cast<int>(tiles), s);
+}
+
+// K blocks summed inside the tensor core's accumulator. Losses: 256 of K, a
+// truncation of under 1e-6 of a logit. Gradients in 16-bit types round to
+// 2^-9: 2048 of K.
+constexpr int kChunkStats16 = 2, kChunkStats32 = 2, kChunkGrad16 = 16, kChunkGrad32 = 2;
+
+bool vec32(const void* p, long long ld, int es) {
+  return reinterpret_cast<uintptr_t>(p) % 32 == 0 && (ld * es) % 32 == 0;
+}
+
+}  // namespace
+}  // namespace po
+
+using namespace po;
+
+extern "C" size_t po_linear_loss_workspace_bytes(const void* weight, long long w_ld, int dtype, long long tokens,
+                                                 long long dim, long long vocab, long long top, int want_dhidden,
+                                                 int want_dweight, long long chunk_rows) {
+  if (tokens <= 0 || dim <= 0 || vocab <= 0 || top <= 0 || dtype_size(dtype) == 0) return 0;
+  Plan p;
+  // A teacher's rows need the larger workspace of the two kinds of targets but for zsum: size for both.
+  size_t best = 0;
+  for (int soft = 0; soft < 2; ++soft) {
+    make_plan(p, weight, w_ld, dtype, tokens, dim, vocab, top, soft != 0, want_dhidden != 0, want_dweight != 0,
+              chunk_rows, nullptr, 0);
+    if (p.bytes > best) best = p.bytes;
+  }
+  return best + 256;
+}
+
+extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* weight, long long w_ld, int dtype,
+                              long long tokens, long long dim, long long vocab, const long long* index,
+                              long long index_ld, const void* teacher, long long teacher_ld, int teacher_dtype,
+                              long long top, long long ignore_index, float smoothing, float z_loss, float temperature,
+                              int mean, const float* row_grad, float* loss_rows, float* loss, void* dhidden,
+                              long long dh_ld, void* dweight, long long dw_ld, long long chunk_rows, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  if (dtype != PO_F32 && dtype != PO_BF16 && dtype != PO_F16)
+    return set_error(PO_ERR_ARG, "linear_loss: dtype must be fp32, bf16 or fp16");
+  if (tokens < 0 || dim <= 0 || vocab <= 0) return set_error(PO_ERR_ARG, "linear_loss: bad size");
+  if (tokens > (1 << 26) || dim > (1 << 24) || vocab > (1 << 28))
+    return set_error(PO_ERR_ARG, "linear_loss: size too large");
+  const bool soft = teacher != nullptr;
+  if (top < 1 || top > kMaxTop || (!soft && top != 1))
+    return set_error(PO_ERR_ARG, "linear_loss: top must be 1 to 1024 (1 without a teacher)");
+  if (soft && teacher_dtype != PO_F32 && teacher_dtype != PO_BF16 && teacher_dtype != PO_F16)
+    return set_error(PO_ERR_ARG, "linear_loss: teacher dtype must be fp32, bf16 or fp16");
+  if (!(temperature > 0.0f) || !std::isfinite(temperature) || (!soft && temperature != 1.0f))
+    return set_error(PO_ERR_ARG, "linear_loss: temperature must be positive (1 without a teacher)");
+  if (!(smoothing >= 0.0f && smoothing <= 1.0f) || !std::isfinite(z_loss) || (soft && (smoothing != 0.0f || z_loss != 0.0f)))
+    return set_error(PO_ERR_ARG, "linear_loss: smoothing must be in [0, 1] and z_loss finite (both 0 with a teacher)");
+  if (row_grad != nullptr && (mean || (dhidden == nullptr && dweight == nullptr)))
+    return set_error(PO_ERR_ARG, "linear_loss: row_grad goes with gradients of the sum");
+  if (h_ld < dim || w_ld < dim || (tokens > 1 && (index_ld < top || (soft && teacher_ld < top))) ||
+      (dhidden != nullptr && dh_ld < dim) || (dweight != nullptr && dw_ld < dim))
+    return set_error(PO_ERR_ARG, "linear_loss: a pitch is smaller than its row");
+  if (weight == nullptr || (tokens > 0 && (hidden == nullptr || index == nullptr || loss_rows == nullptr)))
+    return set_error(PO_ERR_ARG, "linear_loss: null operand");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int sms = sm_count();
+  if (tokens == 0) {
+    if (loss != nullptr)
+      if (int r = check_cuda(cudaMemsetAsync(loss, 0, 4, s), "linear_loss")) return r;
+    if (dweight != nullptr) {
+      if (dtype == PO_F32) zero_kernel<PO_F32><<<8 * sms, 256, 0, s>>>(dweight, dw_ld, vocab, dim);
+      else zero_kernel<PO_BF16><<<8 * sms, 256, 0, s>>>(dweight, dw_ld, vocab, dim);
+      return check_cuda(cudaGetLastError(), "linear_loss zero");
+    }
+    return PO_OK;
+  }
+  if (workspace == nullptr) return set_error(PO_ERR_WORKSPACE, "linear_loss: workspace too small");
+  Plan p;
+  int r = make_plan(p, weight, w_ld, dtype, tokens, dim, vocab, top, soft, dhidden != nullptr, dweight != nullptr,
+                    chunk_rows, workspace, workspace_bytes);
+  if (r) return r;
+  const int T = static_cast<int>(tokens), D = static_cast<int>(dim), V = static_cast<int>(vocab);
+  const Targets tg{index, index_ld, teacher, teacher_ld, teacher_dtype, static_cast<int>(top), ignore_index};
+
+  if (soft) {
+    int width = 2;
+    while (width < top) width <<= 1;
+    const int threads = width < 64 ? 32 : (width > 256 ? 128 : width / 2);
+    teacher_targets_kernel<<<T, threads, width * 8, s>>>(tg, vocab, 1.0f / temperature, width, p.status, p.ent, p.q, p.qlogq);
+    if ((r = check_cuda(cudaGetLastError(), "linear_loss targets"))) return r;
+  }
+  if (row_grad != nullptr) {
+    grad_max_kernel<<<1, 1024, 0, s>>>(row_grad, tokens, p.st);
+    if ((r = check_cuda(cudaGetLastError(), "linear_loss grad_max"))) return r;
+  }
+  const float gscale = dtype == PO_F16 ? kF16Scale : 1.0f;
+  PackArgs pa{};
+  pa.hidden = hidden, pa.h_ld = h_ld, pa.T = tokens, pa.D = D, pa.ldp = static_cast<int>(p.ldp);
+  pa.vec = !p.f32 && D % 8 == 0 && reinterpret_cast<uintptr_t>(hidden) % 16 == 0 && h_ld % 8 == 0;
+  pa.tg = tg, pa.V = vocab, pa.status = p.status, pa.ent = p.ent, pa.rowmap = p.rowmap;
+  pa.packed = p.packed, pa.packed_lo = p.packed_lo, pa.rows_alloc = p.rows_alloc;
+  pa.dhidden = dhidden, pa.dh_ld = dh_ld, pa.loss_rows = loss_rows, pa.st = p.st, pa.sched = p.sched;
+  pa.alpha = temperature / gscale, pa.mean = mean, pa.has_row_grad = row_grad != nullptr;
+  const int pblocks = cdiv(T, kPackRows);
+  if (dtype == PO_F32) pack_kernel<PO_F32><<<pblocks, 256, 0, s>>>(pa);
+  else if (dtype == PO_BF16) pack_kernel<PO_BF16><<<pblocks, 256, 0, s>>>(pa);
+  else pack_kernel<PO_F16><<<pblocks, 256, 0, s>>>(pa);
+  if ((r = check_cuda(cudaGetLastError(), "linear_loss pack"))) return r;
+
+  const void* w = weight;
+  long long wld = w_ld;
+  if (p.stage_w) {
+    if (p.f32) stage_weight_kernel<PO_F32><<<8 * sms, 256, 0, s>>>(weight, w_ld, vocab, D, static_cast<int>(p.ldp), p.w, p.w_lo);
+    else stage_weight_kernel<PO_BF16><<<8 * sms, 256, 0, s>>>(weight, w_ld, vocab, D, static_cast<int>(p.ldp), p.w, nullptr);
+    if ((r = check_cuda(cudaGetLastError(), "linear_loss stage"))) return r;
+    w = p.w;
+    wld = p.ldp;
+  }
+
+  for (int c = 0; c < p.nchunks; ++c) {
+    const long long row0 = c * p.chunk;
+    const int rows = static_cast<int>(tokens - row0 < p.chunk ? tokens - row0 : p.chunk);
+    const size_t hoff = static_cast<size_t>(row0) * p.ldp;
+    const void* hp = static_cast<const char*>(p.packed) + hoff * p.es;
+    const float* hlo = p.f32 ? p.packed_lo + hoff : nullptr;
+    const long long krows = round_up(rows, kRowPad);
+    const HeadOperand Hk{{hp, hlo}, dtype, rows, dim, p.ldp, true};
+    const HeadOperand Wk{{w, p.w_lo}, dtype, vocab, dim, wld, true};
+    {
+      HeadParams P;
+      memset(&P, 0, sizeof(P));
+      P.M = rows, P.N = V, P.K = D, P.limit = LIMIT_M, P.row0 = static_cast<int>(row0);
+      // All row tiles of a vocabulary tile run together (W is read once) as
+      // long as their panels of H take at most 48 MB of L2.
+      const int mt = cdiv(rows, 256);
+      const long long panel = 256LL * p.ldp * p.es * (p.f32 ? 2 : 1);
+      const int fit = static_cast<int>((48LL << 20) / panel > 1 ? (48LL << 20) / panel : 1);
+      P.band = cdiv(mt, cdiv(mt, fit));
+      P.chunk = p.f32 ? kChunkStats32 : kChunkStats16;
+      P.scale2 = kLog2e / temperature;
+      P.part = p.part, P.nparts = p.nparts, P.zsum = smoothing != 0.0f ? p.zsum : nullptr;
+      P.e = p.e, P.e_ld = p.e_ld, P.rowmap = p.rowmap, P.ent = p.ent, P.top = static_cast<int>(top), P.zpick = p.zpick;
+      if ((r = run_head(p, HEAD_LOGITS, P, Hk, Wk, 1, s))) return r;
+    }
+    FinishArgs fa{};
+    fa.part = p.part, fa.zsum = smoothing != 0.0f ? p.zsum : nullptr, fa.nparts = p.nparts, fa.row0 = static_cast<int>(row0);
+    fa.rowmap = p.rowmap, fa.zpick = p.zpick, fa.ent = p.ent, fa.q = soft ? p.q : nullptr, fa.qlogq = p.qlogq;
+    fa.top = static_cast<int>(top), fa.smoothing = smoothing, fa.z_loss = z_loss, fa.temperature = temperature;
+    fa.inv_vocab = 1.0f / static_cast<float>(vocab), fa.stat = p.stat, fa.loss_rows = loss_rows, fa.loss = loss;
+    fa.T = tokens, fa.mean = mean, fa.final_launch = c == p.nchunks - 1, fa.st = p.st;
+    finish_kernel<<<rows, 128, 0, s>>>(fa);
+    if ((r = check_cuda(cudaGetLastError(), "linear_loss finish"))) return r;
+    if (!p.grads) continue;
+
+    RescaleArgs ra{};
+    ra.e = p.e, ra.lo = p.e_lo, ra.e_ld = p.e_ld, ra.V = vocab, ra.part = p.part, ra.nparts = p.nparts, ra.stat = p.stat;
+    ra.row0 = static_cast<int>(row0), ra.rows = rows, ra.rowmap = p.rowmap, ra.ent = p.ent, ra.q = soft ? p.q : nullptr;
+    ra.zpick = p.zpick, ra.top = static_cast<int>(top), ra.row_grad = row_grad, ra.smoothing = smoothing;
+    ra.z_loss = z_loss, ra.inv_vocab = 1.0f / static_cast<float>(vocab), ra.scale = gscale, ra.st = p.st;
+    const int nseg = cdiv(p.e_ld, kSegment);
+    const long long rblocks = krows * nseg;
+    if (rblocks > INT_MAX) return set_error(PO_ERR_ARG, "linear_loss: chunk too large");
+    if (dtype == PO_F32) rescale_kernel<PO_F32><<<static_cast<int>(rblocks), 256, 0, s>>>(ra, nseg);
+    else if (dtype == PO_BF16) rescale_kernel<PO_BF16><<<static_cast<int>(rblocks), 256, 0, s>>>(ra, nseg);
+    else rescale_kernel<PO_F16><<<static_cast<int>(rblocks), 256, 0, s>>>(ra, nseg);
+    if ((r = check_cuda(cudaGetLastError(), "linear_loss rescale"))) return r;
+
+    const long long pld = round_up(dim, 128);
+    if (p.want_dh) {
+      HeadParams P;
+      memset(&P, 0, sizeof(P));
+      P.M = rows, P.N = D, P.K = V, P.limit = LIMIT_M, P.row0 = static_cast<int>(row0), P.band = 8;
+      P.chunk = p.f32 ? kChunkGrad32 : kChunkGrad16;
+      P.alpha = &p.st->alpha, P.out = dhidden, P.out_ld = dh_ld, P.out_dtype = dtype, P.vec = vec32(dhidden, dh_ld, p.es);
+      P.out_rows = p.rowmap, P.partial = p.partial, P.part_ld = pld;
+      const HeadOperand A{{p.e, p.e_lo}, dtype, rows, vocab, p.e_ld, true};
+      const HeadOperand B{{w, p.w_lo}, dtype, vocab, dim, wld, false};
+      if ((r = run_head(p, HEAD_DHIDDEN, P, A, B, p.splits_dh, s))) return r;
+      if (p.splits_dh > 1 &&
+          (r = join(dtype, p.partial, p.splits_dh, rows, pld, D, p, static_cast<int>(row0), true, p.rowmap, dhidden, dh_ld, s)))
+        return r;
+    }
+    if (p.want_dw) {
+      HeadParams P;
+      memset(&P, 0, sizeof(P));
+      P.M = V, P.N = D, P.K = rows, P.limit = LIMIT_K, P.row0 = static_cast<int>(row0), P.band = 8;
+      P.chunk = p.f32 ? kChunkGrad32 : kChunkGrad16;
+      P.alpha = &p.st->alpha, P.partial = p.partial, P.part_ld = pld;
+      const bool to_acc = p.dw_acc && !p.f32;  // fp32 gradients add up in place
+      const bool last = c == p.nchunks - 1;
+      float* acc = to_acc ? p.dw_accum : static_cast<float*>(dweight);
+      const long long acc_ld = to_acc ? round_up(dim, 8) : dw_ld;
+      P.cin = p.dw_acc && c > 0 ? acc : nullptr;
+      P.cin_ld = acc_ld;
+      const bool mid = to_acc && !last;
+      P.out = mid ? static_cast<void*>(acc) : dweight;
+      P.out_ld = mid ? acc_ld : dw_ld;
+      P.out_dtype = mid ? PO_F32 : dtype;
+      P.vec = vec32(P.out, P.out_ld, dtype_size(P.out_dtype)) && (P.cin == nullptr || vec32(P.cin, acc_ld, 4));
+      // Rows past the counted ones are zero up to a K block in both operands.
+      const HeadOperand A{{p.e, p.e_lo}, dtype, krows, vocab, p.e_ld, false};
+      const HeadOperand B{{hp, hlo}, dtype, p.rows_alloc - row0 < krows ? p.rows_alloc - row0 : krows, dim, p.ldp, false};
+      if ((r = run_head(p, HEAD_DWEIGHT, P, A, B, p.splits_dw, s))) return r;
+      if (p.splits_dw > 1 && (r = join(dtype, p.partial, p.splits_dw, V, pld, D, p, 0, false, nullptr, dweight, dw_ld, s)))
+        return r;
+    }
+  }
+  return PO_OK;
+}

@@ -1,0 +1,82 @@
+// Device helpers shared by the loss kernels: typed loads and stores, block
+// reductions in a fixed order, and a teacher's distribution over one row's
+// entries.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace po {
+
+constexpr int kMaxTop = 1024;  // entries a teacher's row may have
+
+template <int DT>
+struct ElemOf;
+template <>
+struct ElemOf<PO_F32> {
+  using T = float;
+};
+template <>
+struct ElemOf<PO_BF16> {
+  using T = __nv_bfloat16;
+};
+template <>
+struct ElemOf<PO_F16> {
+  using T = __half;
+};
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ void from_f32(float v, float& o) { o = v; }
+__device__ __forceinline__ void from_f32(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void from_f32(float v, __half& o) { o = __float2half_rn(v); }
+
+__device__ __forceinline__ float load_as_f32(const void* p, int dtype, long long i) {
+  if (dtype == PO_F32) return static_cast<const float*>(p)[i];
+  if (dtype == PO_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ T warp_sum(T v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// Over the whole block (any multiple of 32 threads up to 1024); every thread
+// gets the result. `buf`: 32 values of shared memory, free again on return.
+__device__ __forceinline__ float block_max(float v, float* buf) {
+  v = warp_max(v);
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+  __syncthreads();
+  const int nw = blockDim.x >> 5;
+  v = warp_max(static_cast<int>(threadIdx.x & 31) < nw ? buf[threadIdx.x & 31] : -INFINITY);
+  __syncthreads();
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ T block_sum(T v, T* buf) {
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+  __syncthreads();
+  const int nw = blockDim.x >> 5;
+  v = warp_sum(static_cast<int>(threadIdx.x & 31) < nw ? buf[threadIdx.x & 31] : T(0));
+  __syncthreads();
+  return v;
+}
+
+// What a row is to the loss.
+enum RowStatus : int { ROW_IGNORED = 0, ROW_COUNTED = 1, ROW_BAD = 2 };
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+}  // namespace po

@@ -1,0 +1,275 @@
+"""Losses of language-model training over a large vocabulary, with their gradients.
+
+Three functions of CUDA tensors (bf16, fp16 or fp32), differentiable by
+``torch.autograd``; the kernels are those of ``po_linear_loss`` and
+``po_distill_logits`` (``include/pytorch_opt_b200.h``):
+
+* ``linear_cross_entropy(hidden, weight, target)`` — softmax cross entropy of
+  ``hidden @ weight.T`` without that product as a tensor: per-token losses
+  leave two numbers a row and 128 columns, gradients the scaled exponentials
+  of one chunk of rows in 16 bits while the call runs;
+* ``linear_distillation(hidden, weight, teacher_index, teacher_logits)`` — the
+  divergence of the same product's softmax from a teacher's top logits;
+* ``distillation(logits, teacher_index, teacher_logits)`` — the same for
+  student logits that are there already.
+
+Rows that count for nothing (``ignore_index``, no teacher's entry) have loss
+and gradient 0, are left out of the mean, and cost no product. With a scalar
+reduction the gradients are made together with the loss (the softmax is not
+computed a second time) whenever an input requires grad; with
+``reduction="none"`` they are made in the backward pass from the upstream
+gradient of each row. Errors are ``RuntimeError`` as in ``native``; there is no
+CPU path.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_REDUCTIONS = ("mean", "sum", "none")
+MAX_TOP = 1024
+
+
+def _check_tensors(name: str, *tensors) -> torch.device:
+    dev = None
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise RuntimeError(f"{name}: expected a tensor, got {type(t).__name__}")
+        if not t.is_cuda:
+            raise RuntimeError("pytorch_opt_b200 runs on CUDA tensors only (there is no CPU path)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RuntimeError("all tensors must be on the same CUDA device")
+    return dev
+
+
+def _check_reduction(name: str, reduction: str) -> None:
+    if reduction not in _REDUCTIONS:
+        raise RuntimeError(f"{name}: reduction must be mean|sum|none, got {reduction}")
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """The tensor as rows of its last axis, each contiguous (a copy only if they are not)."""
+    x = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
+    if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+    return x
+
+
+def _pitch(x: torch.Tensor) -> int:
+    """Elements from one row to the next."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _linear_loss(hidden, weight, index, teacher, ignore_index, smoothing, z_loss, temperature, mean, scalar, row_grad,
+                 want_dh, want_dw, chunk_rows):
+    """One call of po_linear_loss: (per-row losses, scalar loss, dhidden, dweight)."""
+    tokens, dim = hidden.shape
+    vocab, top = weight.shape[0], index.shape[1]
+    dev = hidden.device
+    code = _lib.DTYPE_CODE[hidden.dtype]
+    with torch.cuda.device(dev):
+        lib = _lib.load()
+        losses = torch.empty(tokens, dtype=torch.float32, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev) if scalar else None
+        dh = torch.empty(tokens, dim, dtype=hidden.dtype, device=dev) if want_dh else None
+        dw = torch.empty(vocab, dim, dtype=weight.dtype, device=dev) if want_dw else None
+        nbytes = lib.po_linear_loss_workspace_bytes(weight.data_ptr(), _pitch(weight), code, tokens, dim, vocab, top,
+                                                    int(want_dh), int(want_dw), chunk_rows)
+        ws = _lib.workspace(nbytes, dev)
+        _lib.check(lib.po_linear_loss(
+            hidden.data_ptr(), _pitch(hidden), weight.data_ptr(), _pitch(weight), code, tokens, dim, vocab,
+            index.data_ptr(), _pitch(index), teacher.data_ptr() if teacher is not None else None,
+            _pitch(teacher) if teacher is not None else 0,
+            _lib.DTYPE_CODE[teacher.dtype] if teacher is not None else 0, top, ignore_index, smoothing, z_loss,
+            temperature, int(mean), row_grad.data_ptr() if row_grad is not None else None, losses.data_ptr(),
+            loss.data_ptr() if scalar else None, dh.data_ptr() if want_dh else None, dim,
+            dw.data_ptr() if want_dw else None, dim, chunk_rows, ws.data_ptr(), nbytes, _lib.stream_ptr(dev)),
+            "po_linear_loss")
+    return losses, loss, dh, dw
+
+
+def _distill_logits(logits, index, teacher, temperature, mean, scalar, row_grad, want_grad):
+    """One call of po_distill_logits: (per-row losses, scalar loss, dlogits)."""
+    tokens, vocab = logits.shape
+    dev = logits.device
+    with torch.cuda.device(dev):
+        lib = _lib.load()
+        losses = torch.empty(tokens, dtype=torch.float32, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev) if scalar else None
+        dz = torch.empty(tokens, vocab, dtype=logits.dtype, device=dev) if want_grad else None
+        nbytes = lib.po_distill_logits_workspace_bytes(tokens)
+        ws = _lib.workspace(nbytes, dev) if scalar else None
+        _lib.check(lib.po_distill_logits(
+            logits.data_ptr(), _pitch(logits), _lib.DTYPE_CODE[logits.dtype], tokens, vocab, index.data_ptr(),
+            _pitch(index), teacher.data_ptr(), _pitch(teacher), _lib.DTYPE_CODE[teacher.dtype], index.shape[1],
+            temperature, int(mean), row_grad.data_ptr() if row_grad is not None else None, losses.data_ptr(),
+            loss.data_ptr() if scalar else None, dz.data_ptr() if want_grad else None, vocab,
+            ws.data_ptr() if scalar else None, nbytes if scalar else 0, _lib.stream_ptr(dev)), "po_distill_logits")
+    return losses, loss, dz
+
+
+def _scaled(grad: torch.Tensor | None, factor: torch.Tensor) -> torch.Tensor | None:
+    """``grad`` times a device scalar, in place; a factor of 1 (``loss.backward()``) moves no data."""
+    if grad is not None:
+        with torch.cuda.device(grad.device):
+            _lib.check(_lib.load().po_scale_inplace(grad.data_ptr(), _lib.DTYPE_CODE[grad.dtype], grad.numel(),
+                                                    factor.data_ptr(), _lib.stream_ptr(grad.device)),
+                       "po_scale_inplace")
+    return grad
+
+
+class _LinearLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, index, teacher, opts):
+        reduction, chunk_rows, *terms = opts
+        scalar = reduction != "none"
+        want = ctx.needs_input_grad[:2] if scalar else (False, False)
+        losses, loss, dh, dw = _linear_loss(hidden, weight, index, teacher, *terms, reduction == "mean", scalar, None,
+                                            *want, chunk_rows)
+        ctx.opts = opts
+        if scalar:
+            ctx.grads = (dh, dw)
+            return loss
+        ctx.save_for_backward(hidden, weight, index, teacher)
+        return losses
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, up):
+        reduction, chunk_rows, *terms = ctx.opts
+        up = up.float().contiguous()
+        if reduction != "none":
+            if ctx.grads is None:
+                raise RuntimeError("the gradients of this loss were handed out already: one backward pass per loss")
+            (dh, dw), ctx.grads = ctx.grads, None
+            return _scaled(dh, up), _scaled(dw, up), None, None, None
+        hidden, weight, index, teacher = ctx.saved_tensors
+        _, _, dh, dw = _linear_loss(hidden, weight, index, teacher, *terms, False, False, up, *ctx.needs_input_grad[:2],
+                                    chunk_rows)
+        return dh, dw, None, None, None
+
+
+class _Distillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, index, teacher, reduction, temperature):
+        scalar = reduction != "none"
+        losses, loss, dz = _distill_logits(logits, index, teacher, temperature, reduction == "mean", scalar, None,
+                                           scalar and ctx.needs_input_grad[0])
+        ctx.scalar, ctx.temperature = scalar, temperature
+        if scalar:
+            ctx.grad = dz
+            return loss
+        ctx.save_for_backward(logits, index, teacher)
+        return losses
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, up):
+        up = up.float().contiguous()
+        if ctx.scalar:
+            if ctx.grad is None:
+                raise RuntimeError("the gradient of this loss was handed out already: one backward pass per loss")
+            dz, ctx.grad = ctx.grad, None
+            return _scaled(dz, up), None, None, None, None
+        logits, index, teacher = ctx.saved_tensors
+        return _distill_logits(logits, index, teacher, ctx.temperature, False, False, up, True)[2], None, None, None, None
+
+
+def _check_head(name: str, hidden: torch.Tensor, weight: torch.Tensor) -> None:
+    if hidden.dtype not in _DTYPES or weight.dtype != hidden.dtype:
+        raise RuntimeError(f"{name}: hidden and weight must both be bf16, fp16 or fp32, got {hidden.dtype} and "
+                           f"{weight.dtype}")
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or not weight.numel():
+        raise RuntimeError(f"{name}: expects hidden (..., dim) and weight (vocab, dim), got {tuple(hidden.shape)} and "
+                           f"{tuple(weight.shape)}")
+
+
+def _check_teacher(name: str, lead, index: torch.Tensor, teacher: torch.Tensor, temperature: float):
+    if index.dtype not in (torch.int64, torch.int32):
+        raise RuntimeError(f"{name}: teacher_index must be int64 or int32, got {index.dtype}")
+    if teacher.dtype not in _DTYPES:
+        raise RuntimeError(f"{name}: teacher_logits must be fp32, bf16 or fp16, got {teacher.dtype}")
+    if index.dim() < 1 or index.shape != teacher.shape or index.shape[:-1] != lead:
+        raise RuntimeError(f"{name}: teacher_index and teacher_logits must be (..., top) over the same tokens, got "
+                           f"{tuple(index.shape)} and {tuple(teacher.shape)} for {tuple(lead)}")
+    if not 1 <= index.shape[-1] <= MAX_TOP:
+        raise RuntimeError(f"{name}: 1 to {MAX_TOP} entries a token, got {index.shape[-1]}")
+    if not (temperature > 0 and temperature < float("inf")):
+        raise RuntimeError(f"{name}: temperature must be positive, got {temperature}")
+    return _rows(index.long()), _rows(teacher.detach())
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100,
+                         label_smoothing: float = 0.0, z_loss: float = 0.0, reduction: str = "mean",
+                         chunk_rows: int = 0) -> torch.Tensor:
+    """Softmax cross entropy of the logits ``hidden @ weight.T`` (fp32 result).
+
+    ``hidden`` (..., dim), ``weight`` (vocab, dim), ``target`` (...) of indices.
+    A token's loss is ``lse(z) - (1 - s) z_y - s mean(z) + z_loss lse(z)^2``
+    with s = ``label_smoothing``. Tokens with ``target == ignore_index`` count
+    for nothing; "mean" divides by the others (0 if there are none). A target
+    outside the vocabulary makes its loss NaN and its gradient 0.
+    ``chunk_rows``: tokens whose exponentials may lie in the workspace at once
+    while gradients are made (0: as many as fit 2 GiB).
+    """
+    name = "linear_cross_entropy"
+    _check_tensors(name, hidden, weight, target)
+    _check_reduction(name, reduction)
+    _check_head(name, hidden, weight)
+    if target.dtype not in (torch.int64, torch.int32) or target.shape != hidden.shape[:-1]:
+        raise RuntimeError(f"{name}: target must be int64 or int32 of shape {tuple(hidden.shape[:-1])}, got "
+                           f"{target.dtype} {tuple(target.shape)}")
+    if not 0.0 <= label_smoothing <= 1.0 or not abs(z_loss) < float("inf"):
+        raise RuntimeError(f"{name}: label_smoothing must be in [0, 1] and z_loss finite")
+    if chunk_rows < 0:
+        raise RuntimeError(f"{name}: chunk_rows must not be negative")
+    lead = hidden.shape[:-1]
+    out = _LinearLoss.apply(_rows(hidden), _rows(weight), target.long().reshape(-1, 1), None,
+                            (reduction, int(chunk_rows), int(ignore_index), float(label_smoothing), float(z_loss), 1.0))
+    return out.reshape(lead) if reduction == "none" else out
+
+
+def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_index: torch.Tensor,
+                        teacher_logits: torch.Tensor, *, temperature: float = 1.0, reduction: str = "mean",
+                        chunk_rows: int = 0) -> torch.Tensor:
+    """Divergence of ``softmax(hidden @ weight.T / a)`` from a teacher's top logits (fp32 result).
+
+    ``teacher_index`` and ``teacher_logits`` (..., top): where a token's index
+    is negative there is no entry. With q the softmax of the entries' logits
+    divided by a = ``temperature``, a token's loss is ``a^2 sum_k q_k (log q_k
+    - log p_k)``, p the student's softmax over the whole vocabulary. Tokens
+    without an entry count for nothing. An index past the vocabulary makes its
+    token's loss NaN and its gradient 0. ``chunk_rows`` as in
+    ``linear_cross_entropy``.
+    """
+    name = "linear_distillation"
+    _check_tensors(name, hidden, weight, teacher_index, teacher_logits)
+    _check_reduction(name, reduction)
+    _check_head(name, hidden, weight)
+    if chunk_rows < 0:
+        raise RuntimeError(f"{name}: chunk_rows must not be negative")
+    lead = hidden.shape[:-1]
+    index, teacher = _check_teacher(name, lead, teacher_index, teacher_logits, temperature)
+    out = _LinearLoss.apply(_rows(hidden), _rows(weight), index, teacher,
+                            (reduction, int(chunk_rows), 0, 0.0, 0.0, float(temperature)))
+    return out.reshape(lead) if reduction == "none" else out
+
+
+def distillation(logits: torch.Tensor, teacher_index: torch.Tensor, teacher_logits: torch.Tensor, *,
+                 temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
+    """``linear_distillation`` for student logits (..., vocab) that are there already (fp32 result)."""
+    name = "distillation"
+    _check_tensors(name, logits, teacher_index, teacher_logits)
+    _check_reduction(name, reduction)
+    if logits.dtype not in _DTYPES or logits.dim() < 1 or logits.shape[-1] < 1:
+        raise RuntimeError(f"{name}: logits must be (..., vocab) of bf16, fp16 or fp32, got {logits.dtype} "
+                           f"{tuple(logits.shape)}")
+    lead = logits.shape[:-1]
+    index, teacher = _check_teacher(name, lead, teacher_index, teacher_logits, temperature)
+    out = _Distillation.apply(_rows(logits), index, teacher, reduction, float(temperature))
+    return out.reshape(lead) if reduction == "none" else out
