@@ -12,14 +12,12 @@
 //  * The accumulator is drained into registers every `chunk` K blocks and
 //    summed there (fp32, round to nearest): the tensor core's own accumulator
 //    truncates, by -1.1e-5 of the sum at K = 4096, which the loss (a difference
-//    of two nearby logits) would show. A drain is 128 tcgen05.ld columns and
-//    128 adds a thread against 1024 tensor cycles a block, hidden behind the
-//    other accumulator's MMAs.
+//    of two nearby logits) would show. A drain is 64 columns loaded and added
+//    by each thread, hidden behind the other accumulator's MMAs.
 //
-// Epilogue of the logits: each thread holds 128 columns of one row, so the
-// row's maximum and sum of exponentials over those columns need no exchange
-// between threads: 128 compares, 128 FMA + ex2, 128 adds. It leaves (max, sum)
-// per row and 128 columns, the logits at the row's target indices, and, when
+// Epilogue of the logits: each thread holds 64 columns of one row, so the
+// row's maximum and sum of exponentials over the tile's 256 columns take two
+// exchanges between four threads. It leaves (max, sum) per row and tile, the logits at the row's target indices, and, when
 // gradients are wanted, exp(z - max) in 16 bits (fp16: the values are in
 // (0, 1], so its 11 bits cost less than the one rounding to the products' type
 // that follows; 32 bits for fp32 operands). Storing that costs 2 bytes a logit
@@ -49,7 +47,7 @@ struct alignas(64) HeadParams {
   int* err;
   // HEAD_STATS
   float scale2;       // log2(e) / temperature
-  float2* part;       // [row][nparts] (max, sum of 2^(z2 - max)) over 128 columns, z2 = scale2 * logit
+  float2* part;       // [row][nparts] (max, sum of 2^(z2 - max)) over 256 columns, z2 = scale2 * logit
   int nparts;
   float* zsum;        // [row][nparts] sum of the logits (nullable)
   void* e;            // [row][e_ld] 2^(z2 - max) (nullable)
@@ -70,6 +68,17 @@ struct alignas(64) HeadParams {
   float* partial;      // splits > 1: [split][M][part_ld] fp32, instead of out
   long long part_ld;
 };
+
+// Arrival on a barrier of either CTA of the pair that orders what the barrier
+// guards (a tile index read from shared memory, TMEM reads behind their tcgen05
+// fence) but not this thread's global stores: at cluster scope a release would
+// wait for the tile's stores to reach L2 (a third of the epilogue's stalls).
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void head_sched_release(uint64_t* sempty, int j) {
+  mbar_arrive_pair(mapa_shared(smem_u32(sempty + j % kSchedSlots), 0));
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -92,7 +101,16 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-constexpr int HC = 128;  // columns of a tile one epilogue thread holds
+// Sixteen epilogue warps a CTA, four to each TMEM lane quarter: four warps a
+// scheduler hide the latencies of TMEM loads, ex2 and stores where two (with
+// 128 columns a thread) did not.
+constexpr int kHeadEpiWarps = 16;
+constexpr int HC = 64;  // columns of a tile one epilogue thread holds
+constexpr int kShareFloats = 3 * 128;  // a lane quarter's maxima, sums and logit sums
+constexpr int kHeadSmemExtra = 4 * kShareFloats * 4;
+constexpr int kHeadThreads = 64 + 32 * kHeadEpiWarps;
+// Readers of a slot of the tile queue: leader MMA issuer and epilogue warps, peer producer and epilogue warps.
+constexpr int kHeadReaders = 2 + 2 * kHeadEpiWarps;
 
 struct HeadTile {
   int mt, nt, split, kb0, kb1;
@@ -133,11 +151,49 @@ __device__ __forceinline__ HeadTile head_tile(const HeadParams& P, const HeadExt
   return h;
 }
 
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// Stores 128 bytes of each of the warp's 32 rows. v: this thread's row, as four
+// blocks of 32 bytes. Four lanes first exchange blocks (two butterfly rounds),
+// so that each store instruction writes whole 128-byte lines of eight rows
+// instead of 32-byte pieces of 32 rows. row_ptr(r): where row r of the warp
+// goes, null where it does not.
+template <class RowPtr>
+__device__ __forceinline__ void store_lines(uint32_t (&v)[32], int lane, RowPtr row_ptr) {
+#pragma unroll
+  for (int round = 0; round < 2; ++round) {
+    const int x = 1 << round;
+    const bool hi = (lane & x) != 0;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int a = round == 0 ? 2 * p : p, b = a + x;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, hi ? v[8 * a + i] : v[8 * b + i], x);
+        if (hi) v[8 * a + i] = got;
+        else v[8 * b + i] = got;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = v[8 * i + k];
+    char* at = row_ptr((lane & ~3) + i);
+    if (at != nullptr) st_global_32B(at + (lane & 3) * 32, w);
+  }
+}
+
 // ------------------------------------------------------------- epilogues
-// x: accumulators of columns n0 .. n0 + 127 of packed row `row` (of this launch).
+// x: accumulators of columns n0 .. n0 + HC - 1 of packed row `row` (of this launch).
+// `share`: this lane quarter's rows of shared memory, [column group][row].
 template <bool F32E>
 __device__ __forceinline__ void stats_epilogue(const HeadParams& P, float (&x)[HC], bool live, int row, int n0,
-                                               int nt2, long long tk, int lo, int c) {
+                                               int nt, long long tk, int lo, int c, float* share, int group, int q,
+                                               int lane, int m_rows) {
   const int ncols = P.N - n0;
   // Logits at the targets: c is the next target's column in this tile. One
   // vote per 16 columns; a row has few targets, so most groups have none.
@@ -155,8 +211,8 @@ __device__ __forceinline__ void stats_epilogue(const HeadParams& P, float (&x)[H
       }
     }
   }
-  if (!live) return;
-  const long long at = static_cast<long long>(row) * P.nparts + nt2;
+  const long long at = static_cast<long long>(row) * P.nparts + nt;
+  float zs = 0.0f;
   if (P.zsum != nullptr) {
     // Columns past the vocabulary come from zero-filled rows of W: they add 0.
     float s0 = 0.0f, s1 = 0.0f;
@@ -165,7 +221,7 @@ __device__ __forceinline__ void stats_epilogue(const HeadParams& P, float (&x)[H
       s0 += x[j];
       s1 += x[j + 1];
     }
-    P.zsum[at] = s0 + s1;
+    zs = s0 + s1;
   }
   if (ncols < HC) {
 #pragma unroll
@@ -180,7 +236,10 @@ __device__ __forceinline__ void stats_epilogue(const HeadParams& P, float (&x)[H
     m2 = fmaxf(m2, x[j + 2]);
     m3 = fmaxf(m3, x[j + 3]);
   }
-  const float m = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * P.scale2;
+  // The four warps of this lane quarter share the row's maximum over the tile.
+  share[group * 32 + lane] = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+  bar_sync(1 + q, 128);
+  const float m = fmaxf(fmaxf(share[lane], share[32 + lane]), fmaxf(share[64 + lane], share[96 + lane])) * P.scale2;
   const float off = m == -INFINITY ? 0.0f : -m;
   float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
 #pragma unroll
@@ -194,47 +253,51 @@ __device__ __forceinline__ void stats_epilogue(const HeadParams& P, float (&x)[H
     s2 += x[j + 2];
     s3 += x[j + 3];
   }
-  P.part[at] = make_float2(m, (s0 + s1) + (s2 + s3));
-  if (P.e == nullptr) return;
-  const long long base = static_cast<long long>(row) * P.e_ld + n0;  // e_ld is a multiple of 128
-  if (F32E) {
-    float* e = static_cast<float*>(P.e) + base;
+  share[128 + group * 32 + lane] = (s0 + s1) + (s2 + s3);
+  share[256 + group * 32 + lane] = zs;
+  bar_sync(1 + q, 128);
+  if (group == 0 && live) {
+    const float* g = share + 128 + lane;
+    P.part[at] = make_float2(m, (g[0] + g[32]) + (g[64] + g[96]));
+    if (P.zsum != nullptr) P.zsum[at] = (g[128] + g[160]) + (g[192] + g[224]);
+  }
+  if (P.e == nullptr || ncols <= 0) return;
+  // e_ld is a multiple of 256: whole lines, on 128-byte boundaries.
+  const int row_w = row - lane;
+  constexpr int ES = F32E ? 4 : 2;
+  char* base = static_cast<char*>(P.e) + (static_cast<long long>(row_w) * P.e_ld + n0) * ES;
 #pragma unroll
-    for (int j = 0; j < HC; j += 8) {
-      uint32_t v[8];
+  for (int part = 0; part < ES / 2; ++part) {
+    uint32_t v[32];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(x[j + i]);
-      st_global_32B(e + j, v);
-    }
-  } else {
-    __half* e = static_cast<__half*>(P.e) + base;
-#pragma unroll
-    for (int j = 0; j < HC; j += 16) {
-      uint32_t v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = pack_f16x2(x[j + 2 * i], x[j + 2 * i + 1]);
-      st_global_32B(e + j, v);
-    }
+    for (int i = 0; i < 32; ++i)
+      v[i] = F32E ? __float_as_uint(x[32 * part + i]) : pack_f16x2(x[2 * i], x[2 * i + 1]);
+    store_lines(v, lane, [&](int r) { return row_w + r < m_rows ? base + r * P.e_ld * ES + part * 128 : nullptr; });
   }
 }
 
-__device__ __forceinline__ void store_epilogue(const HeadParams& P, float (&x)[HC], int row, int n0, int split) {
+__device__ __forceinline__ void store_epilogue(const HeadParams& P, float (&x)[HC], int row, int n0, int split,
+                                               int lane, int m_rows) {
   const int ncols = min(HC, P.N - n0);
+  const int row_w = row - lane;
   if (P.splits > 1) {
-    float* o = P.partial + (static_cast<long long>(split) * P.M + row) * P.part_ld + n0;  // part_ld: multiple of 128
+    // part_ld is a multiple of 256: whole lines, on 128-byte boundaries.
+    char* base =
+        reinterpret_cast<char*>(P.partial + (static_cast<long long>(split) * P.M + row_w) * P.part_ld + n0);
 #pragma unroll
-    for (int j = 0; j < HC; j += 8) {
-      uint32_t v[8];
+    for (int part = 0; part < 2; ++part) {
+      uint32_t v[32];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(x[j + i]);
-      st_global_32B(o + j, v);
+      for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(x[32 * part + i]);
+      store_lines(v, lane, [&](int r) { return row_w + r < m_rows ? base + r * P.part_ld * 4 + part * 128 : nullptr; });
     }
     return;
   }
+  const bool live = row < m_rows;
   const float alpha = __ldg(P.alpha);
 #pragma unroll
   for (int j = 0; j < HC; ++j) x[j] *= alpha;
-  if (P.cin != nullptr) {
+  if (P.cin != nullptr && live) {
     const float* ci = P.cin + static_cast<long long>(row) * P.cin_ld + n0;
     if (P.vec && ncols == HC) {
 #pragma unroll
@@ -251,46 +314,52 @@ __device__ __forceinline__ void store_epilogue(const HeadParams& P, float (&x)[H
         if (j < ncols) x[j] += ci[j];
     }
   }
+  const bool bf = P.out_dtype == PO_BF16;
+  if (P.vec && ncols == HC) {
+    const int es = P.out_dtype == PO_F32 ? 4 : 2;
+    char* base = static_cast<char*>(P.out) + static_cast<long long>(n0) * es;
+    const auto row_ptr = [&](int r) -> char* {
+      if (row_w + r >= m_rows) return nullptr;
+      const long long o = P.out_rows != nullptr ? __ldg(P.out_rows + P.row0 + row_w + r) : row_w + r;
+      return base + o * P.out_ld * es;
+    };
+    uint32_t v[32];
+    if (P.out_dtype == PO_F32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(x[i]);
+      store_lines(v, lane, row_ptr);
+      base += 128;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(x[32 + i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = bf ? pack_bf16x2(x[2 * i], x[2 * i + 1]) : pack_f16x2(x[2 * i], x[2 * i + 1]);
+    }
+    store_lines(v, lane, row_ptr);
+    return;
+  }
+  if (!live) return;
   const long long orow = P.out_rows != nullptr ? __ldg(P.out_rows + P.row0 + row) : row;
   const long long base = orow * P.out_ld + n0;
   if (P.out_dtype == PO_F32) {
     float* o = static_cast<float*>(P.out) + base;
 #pragma unroll
-    for (int j = 0; j < HC; j += 8) {
-      if (P.vec && j + 8 <= ncols) {
-        uint32_t v[8];
+    for (int j = 0; j < HC; ++j)
+      if (j < ncols) o[j] = x[j];
+  } else {
+    uint16_t* o = static_cast<uint16_t*>(P.out) + base;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(x[j + i]);
-        st_global_32B(o + j, v);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (j + i < ncols) o[j + i] = x[j + i];
-      }
-    }
-    return;
-  }
-  const bool bf = P.out_dtype == PO_BF16;
-  uint16_t* o = static_cast<uint16_t*>(P.out) + base;
-#pragma unroll
-  for (int j = 0; j < HC; j += 16) {
-    uint32_t v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = bf ? pack_bf16x2(x[j + 2 * i], x[j + 2 * i + 1]) : pack_f16x2(x[j + 2 * i], x[j + 2 * i + 1]);
-    if (P.vec && j + 16 <= ncols) {
-      st_global_32B(o + j, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (j + i < ncols) o[j + i] = static_cast<uint16_t>(v[i / 2] >> (16 * (i & 1)));
+    for (int j = 0; j < HC; j += 2) {
+      const uint32_t v = bf ? pack_bf16x2(x[j], x[j + 1]) : pack_f16x2(x[j], x[j + 1]);
+      if (j < ncols) o[j] = static_cast<uint16_t>(v);
+      if (j + 1 < ncols) o[j + 1] = static_cast<uint16_t>(v >> 16);
     }
   }
 }
 
 // ---------------------------------------------------------------- kernel
 template <int KIND, bool A_MN, bool B_MN, int EPI>
-__global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid_constant__ HeadParams P) {
+__global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid_constant__ HeadParams P) {
   using C = PairCfg<KIND, 2>;
   constexpr int BN = C::BN;
 
@@ -307,6 +376,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
   int* stile = reinterpret_cast<int*>(sempty + kSchedSlots);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(stile + kSchedSlots);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  float* shares = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES + 512);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -320,12 +390,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull + a, 1);
-      mbar_init(tempty + a, kPairEpilogueWarps);
+      mbar_init(tempty + a, 2 * kHeadEpiWarps);
     }
     mbar_init(drain, 1);
     for (int i = 0; i < kSchedSlots; ++i) {
       mbar_init(sfull + i, 1);
-      mbar_init(sempty + i, kSchedReaders);
+      mbar_init(sempty + i, kHeadReaders);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -365,7 +435,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
           mbar_arrive_cluster(mapa_shared(smem_u32(sfull + slot), 1));
         } else {
           if (!sched_read(sfull, stile, j, abort_flag, P.err, kErrTimeoutProducer, t)) break;
-          sched_release(sempty, j);
+          head_sched_release(sempty, j);
         }
         if (t >= X.total) break;
         const HeadTile h = head_tile(P, X, t);
@@ -447,7 +517,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
       for (int j = 0; ok; ++j) {
         int t;
         if (!sched_read(sfull, stile, j, abort_flag, P.err, kErrTimeoutMma, t)) break;
-        sched_release(sempty, j);
+        head_sched_release(sempty, j);
         if (t >= X.total) break;
         const HeadTile h = head_tile(P, X, t);
         const int nv = P.npass * (h.kb1 - h.kb0);
@@ -500,8 +570,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
   } else {
     // ------------------------------------------------------ epilogue (both CTAs)
     const int q = warp & 3;
-    const int half = (warp - 2) >> 2;
-    const uint32_t tcol = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * HC);
+    const int group = (warp - 2) >> 2;
+    float* share = shares + q * kShareFloats;
+    const uint32_t tcol = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(group * HC);
     int ucount = 0;
     bool ok = true;
     for (int j = 0; ok; ++j) {
@@ -509,13 +580,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
       const bool got = sched_read(sfull, stile, j, abort_flag, P.err, kErrTimeoutEpilogue, t);
       if (!__all_sync(0xffffffffu, got)) break;
       __syncwarp();
-      if (lane == 0) sched_release(sempty, j);
+      if (lane == 0) head_sched_release(sempty, j);
       if (t >= X.total) break;
       const HeadTile h = head_tile(P, X, t);
       const int nv = P.npass * (h.kb1 - h.kb0);
       const int row = h.mt * C::TM + static_cast<int>(rank) * 128 + q * 32 + lane;
-      const int n0 = h.nt * BN + half * HC;
-      const bool live = row < X.m && n0 < P.N;
+      const int n0 = h.nt * BN + group * HC;
+      const bool live = row < X.m;
       long long tk = 0;
       int lo = 0, c = 0x7fffffff;
       if (EPI == HEAD_STATS && live) {
@@ -542,23 +613,23 @@ __global__ void __launch_bounds__(kGemmThreads, 1) head_gemm_kernel(const __grid
         }
         tc_fence_after_sync();
 #pragma unroll
-        for (int i = 0; i < HC / 32; ++i) {
-          uint32_t r[32];
-          tmem_ld_32x32(tcol + static_cast<uint32_t>(acc * BN + i * 32), r);
+        for (int i = 0; i < HC / 16; ++i) {
+          uint32_t r[16];
+          tmem_ld_32x16(tcol + static_cast<uint32_t>(acc * BN + i * 16), r);
           tmem_ld_wait();
 #pragma unroll
-          for (int k = 0; k < 32; ++k) x[32 * i + k] += __uint_as_float(r[k]);
+          for (int k = 0; k < 16; ++k) x[16 * i + k] += __uint_as_float(r[k]);
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(tempty + acc), 0));
+        if (lane == 0) mbar_arrive_pair(mapa_shared(smem_u32(tempty + acc), 0));
       }
       if (!ok) break;
       if (EPI == HEAD_STATS) {
-        stats_epilogue<KIND == KIND_TF32>(P, x, live, row, n0, 2 * h.nt + half, tk, lo, c);
+        stats_epilogue<KIND == KIND_TF32>(P, x, live, row, n0, h.nt, tk, lo, c, share, group, q, lane, X.m);
         __syncwarp();
-      } else if (live) {
-        store_epilogue(P, x, row, n0, h.split);
+      } else if (n0 < P.N) {
+        store_epilogue(P, x, row, n0, h.split, lane, X.m);
       }
     }
   }
@@ -595,13 +666,14 @@ int launch_head(const HeadParams& P, int max_tiles, cudaStream_t stream) {
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(kGemmThreads, 1, 1);
-  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.blockDim = dim3(kHeadThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES + kHeadSmemExtra;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (max_pairs[dev] == 0) {
-    int r = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES),
+    int r = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            C::SMEM_BYTES + kHeadSmemExtra),
                        "cudaFuncSetAttribute");
     if (r) return r;
     cfg.gridDim = dim3(2 * (sm_count() / 2), 1, 1);

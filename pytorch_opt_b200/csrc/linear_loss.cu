@@ -11,9 +11,9 @@
 //            number stays on the device
 //   logits   tensor-core product, softmax statistics in its epilogue
 //            (head_gemm.cuh): 2 T V D operations
-//   finish   joins each row's V / 128 statistics, writes the losses
+//   finish   joins each row's V / 256 statistics, writes the losses
 // and with gradients
-//   rescale  exp(z - max of 128 columns) -> dZ in the products' type, in place:
+//   rescale  exp(z - max of 256 columns) -> dZ in the products' type, in place:
 //            one read and one write of T V 2-byte values
 //   dH, dW   two more products of 2 T V D operations
 // The products bound all but the smallest calls (6 T V D operations with
@@ -158,7 +158,7 @@ struct PackArgs {
   long long h_ld;
   long long T;
   int D, ldp;  // packed pitch (elements)
-  int vec;     // 16-byte rows on both sides
+  int vec;     // 16-byte vectors on both sides
   Targets tg;
   long long V;
   const int* status;  // teacher's rows (nullable: decided by the target here)
@@ -166,7 +166,6 @@ struct PackArgs {
   int* rowmap;
   void* packed;
   float* packed_lo;  // fp32: low halves of the tf32 pairs
-  long long rows_alloc;
   void* dhidden;
   long long dh_ld;
   float* loss_rows;
@@ -190,64 +189,61 @@ __device__ __forceinline__ float tf32_rna(float v) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
   return __uint_as_float(r);
 }
+// Four fp32 values as a tf32 (hi, lo) pair.
+__device__ __forceinline__ void split_vec(const uint4& v, float4* hi, float4* lo) {
+  const float x[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
+  float h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    h[i] = tf32_rna(x[i]);
+    l[i] = tf32_rna(x[i] - h[i]);
+  }
+  *hi = make_float4(h[0], h[1], h[2], h[3]);
+  *lo = make_float4(l[0], l[1], l[2], l[3]);
+}
 
-constexpr int kPackRows = 32;
 
-// A block takes 32 rows; their places follow from the number of counted rows
-// before them, which it counts itself (T statuses, read from L2) instead of
-// waiting for another launch.
+constexpr int kPackWarps = 8;
+
+// A warp copies a row; a block takes `groups` times 8 consecutive rows. Their
+// places follow from the number of counted rows before them, which the block
+// counts itself (T statuses, read from L2) instead of waiting for another
+// launch; the host keeps blocks x T / 2 reads small.
 template <int DT>
-__global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
+__global__ void __launch_bounds__(32 * kPackWarps) pack_kernel(PackArgs a, int groups) {
   using T = typename ElemOf<DT>::T;
   __shared__ int buf[32];
-  __shared__ int s_place[kPackRows];
-  const long long first = static_cast<long long>(blockIdx.x) * kPackRows;
+  const long long first = static_cast<long long>(blockIdx.x) * groups * kPackWarps;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int before = 0, bad_before = 0, y = 0;
   const bool last = blockIdx.x == gridDim.x - 1;
+  int before = 0, bad = 0, y = 0;
   for (long long t = threadIdx.x; t < first; t += blockDim.x) {
     const int s = row_status(a, t, y);
     before += s == ROW_COUNTED;
-    bad_before += s == ROW_BAD;
+    bad += s == ROW_BAD;
   }
   before = block_sum(before, buf);
-  if (last) bad_before = block_sum(bad_before, buf);
-  if (warp == 0) {
-    const long long t = first + lane;
-    int s = ROW_IGNORED;
-    if (t < a.T) s = row_status(a, t, y);
-    const unsigned votes = __ballot_sync(0xffffffffu, s == ROW_COUNTED);
-    const unsigned bad = __ballot_sync(0xffffffffu, s == ROW_BAD);
-    const int place = before + __popc(votes & ((1u << lane) - 1u));
-    s_place[lane] = s == ROW_COUNTED ? place : -1;
-    if (s == ROW_COUNTED) {
-      a.rowmap[place] = static_cast<int>(t);
-      if (a.status == nullptr) a.ent[t] = y;
-    } else if (t < a.T) {
-      a.loss_rows[t] = s == ROW_BAD ? NAN : 0.0f;
-      if (a.status == nullptr) a.ent[t] = INT_MAX;
-    }
-    if (last && lane == 0) {
-      const int n = before + __popc(votes), all = n + bad_before + __popc(bad);
-      a.st->count = n;
-      a.st->counted_mean = all;
-      a.st->done = 0;
-      float alpha = a.alpha;
-      if (a.mean) alpha /= static_cast<float>(all > 0 ? all : 1);
-      if (a.has_row_grad) alpha *= a.st->grad_max;
-      a.st->alpha = alpha;
-      buf[0] = n;
-    }
-  }
+  if (last) bad = block_sum(bad, buf);
   if (blockIdx.x == 0 && threadIdx.x < 2) a.sched[threadIdx.x] = 0u;
-  __syncthreads();
   T zero;
   from_f32(0.0f, zero);
-  for (int r = warp; r < kPackRows; r += blockDim.x >> 5) {
-    const long long t = first + r;
-    if (t >= a.T) break;
-    const int place = s_place[r];
-    if (place < 0) {
+  for (int g = 0; g < groups; ++g) {
+    const long long t0 = first + g * kPackWarps, t = t0 + warp;
+    int s = ROW_IGNORED;
+    if (lane < kPackWarps && t0 + lane < a.T) s = row_status(a, t0 + lane, y);
+    const unsigned votes = __ballot_sync(0xffffffffu, s == ROW_COUNTED);
+    const unsigned bads = __ballot_sync(0xffffffffu, s == ROW_BAD);
+    const bool counted = (votes >> warp) & 1u;
+    const int place = before + __popc(votes & ((1u << warp) - 1u));
+    if (lane == warp && t < a.T) {
+      if (counted) a.rowmap[place] = static_cast<int>(t);
+      else a.loss_rows[t] = s == ROW_BAD ? NAN : 0.0f;
+      if (a.status == nullptr) a.ent[t] = counted ? y : INT_MAX;
+    }
+    before += __popc(votes);
+    bad += __popc(bads);
+    if (t >= a.T) continue;
+    if (!counted) {
       if (a.dhidden != nullptr) {
         T* o = static_cast<T*>(a.dhidden) + t * a.dh_ld;
         for (int i = lane; i < a.D; i += 32) o[i] = zero;
@@ -256,36 +252,74 @@ __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
     }
     const T* src = static_cast<const T*>(a.hidden) + t * a.h_ld;
     T* dst = static_cast<T*>(a.packed) + static_cast<long long>(place) * a.ldp;
-    if (DT == PO_F32) {
-      float* lo = a.packed_lo + static_cast<long long>(place) * a.ldp;
-      for (int i = lane; i < a.D; i += 32) {
-        const float v = to_f32(src[i]), h = tf32_rna(v);
-        from_f32(h, dst[i]);
-        lo[i] = tf32_rna(v - h);
+    float* lo = DT == PO_F32 ? a.packed_lo + static_cast<long long>(place) * a.ldp : nullptr;
+    constexpr int VEC = 16 / sizeof(T);
+    if (a.vec) {
+      const int n = a.D / VEC;
+      for (int i0 = lane; i0 < n; i0 += 128) {  // four loads in flight
+        uint4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (i0 + 32 * u < n) v[u] = reinterpret_cast<const uint4*>(src)[i0 + 32 * u];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (i0 + 32 * u >= n) continue;
+          if (DT == PO_F32) split_vec(v[u], reinterpret_cast<float4*>(dst) + i0 + 32 * u, reinterpret_cast<float4*>(lo) + i0 + 32 * u);
+          else reinterpret_cast<uint4*>(dst)[i0 + 32 * u] = v[u];
+        }
       }
-    } else if (a.vec) {
-      for (int i = lane; i < a.D / 8; i += 32)
-        reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
     } else {
-      for (int i = lane; i < a.D; i += 32) dst[i] = src[i];
+      for (int i = lane; i < a.D; i += 32) {
+        if (DT == PO_F32) {
+          const float v = to_f32(src[i]), h = tf32_rna(v);
+          from_f32(h, dst[i]);
+          lo[i] = tf32_rna(v - h);
+        } else {
+          dst[i] = src[i];
+        }
+      }
     }
   }
-  if (last) {  // zero rows that complete dW's last K block
-    const long long n = buf[0];
-    long long end = (n + kRowPad - 1) / kRowPad * kRowPad;
-    if (end > a.rows_alloc) end = a.rows_alloc;
-    for (long long i = n * a.ldp + threadIdx.x; i < end * a.ldp; i += blockDim.x) {
-      static_cast<T*>(a.packed)[i] = zero;
-      if (DT == PO_F32) a.packed_lo[i] = 0.0f;
-    }
+  if (last && threadIdx.x == 0) {
+    const int all = before + bad;
+    a.st->count = before;
+    a.st->counted_mean = all;
+    a.st->done = 0;
+    float alpha = a.alpha;
+    if (a.mean) alpha /= static_cast<float>(all > 0 ? all : 1);
+    if (a.has_row_grad) alpha *= a.st->grad_max;
+    a.st->alpha = alpha;
   }
 }
 
 // Copy of W with a pitch that TMA takes (16-bit), or as tf32 (hi, lo) pairs.
 template <int DT>
 __global__ void __launch_bounds__(256) stage_weight_kernel(const void* w, long long w_ld, long long V, int D, int ldp,
-                                                           void* out, float* lo) {
+                                                           void* out, float* lo, int vec) {
   using T = typename ElemOf<DT>::T;
+  if (DT == PO_F32 && vec) {
+    // A thread splits 4 values; two loads in flight.
+    const int n = D / 4;
+    const long long total = V * n, step = static_cast<long long>(gridDim.x) * blockDim.x;
+    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += 2 * step) {
+      uint4 x[2];
+      long long v[2];
+      int c[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (i + u * step >= total) continue;
+        v[u] = (i + u * step) / n;
+        c[u] = static_cast<int>(i + u * step - v[u] * n);
+        x[u] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const float*>(w) + v[u] * w_ld) + c[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (i + u * step < total)
+          split_vec(x[u], reinterpret_cast<float4*>(static_cast<float*>(out) + v[u] * ldp) + c[u],
+                    reinterpret_cast<float4*>(lo + v[u] * ldp) + c[u]);
+    }
+    return;
+  }
   for (long long v = blockIdx.x; v < V; v += gridDim.x) {
     const T* src = static_cast<const T*>(w) + v * w_ld;
     T* dst = static_cast<T*>(out) + v * ldp;
@@ -320,11 +354,15 @@ struct FinishArgs {
   long long T;
   int mean, final_launch;
   CallState* st;
+  uint4* packed;       // 16-byte words of H's packed rows of this launch (and of their low halves, nullable)
+  uint4* packed_lo;
+  int row_words;
 };
 
 // One block a packed row: lse = log2 sum 2^z2 from the row's partial
 // statistics, and the loss; the last block to finish sums the losses of all
-// rows in a fixed order (fp64).
+// rows in a fixed order (fp64). Rows past the counted ones are zeroed up to a
+// K block of dW, where they meet the zeros of dZ.
 __global__ void __launch_bounds__(128) finish_kernel(FinishArgs a) {
   __shared__ float buf[32];
   __shared__ double dbuf[32];
@@ -333,13 +371,21 @@ __global__ void __launch_bounds__(128) finish_kernel(FinishArgs a) {
   if (a.row0 + row < a.st->count) {
     const float2* p = a.part + static_cast<long long>(row) * a.nparts;
     float m = -INFINITY, s = 0.0f;
-    for (int i = threadIdx.x; i < a.nparts; i += blockDim.x) {
-      const float2 v = p[i];
-      if (v.x > m) {
-        s *= ex2(m - v.x);
-        m = v.x;
+    for (int i0 = threadIdx.x; i0 < a.nparts; i0 += 4 * blockDim.x) {
+      float2 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * blockDim.x;
+        v[u] = i < a.nparts ? p[i] : make_float2(-INFINITY, 0.0f);
       }
-      s += v.x == -INFINITY ? v.y : v.y * ex2(v.x - m);  // an empty part holds 0, or a NaN to keep
+      const float c = fmaxf(fmaxf(v[0].x, v[1].x), fmaxf(v[2].x, v[3].x));
+      if (c > m) {
+        s *= ex2(m - c);
+        m = c;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        s += v[u].x == -INFINITY ? v[u].y : v[u].y * ex2(v[u].x - m);  // an empty part holds 0, or a NaN to keep
     }
     const float mm = block_max(m, buf);
     s = block_sum(m == -INFINITY ? s : s * ex2(m - mm), buf);
@@ -367,6 +413,15 @@ __global__ void __launch_bounds__(128) finish_kernel(FinishArgs a) {
     if (threadIdx.x == 0) {
       a.stat[row] = make_float4(mm, 1.0f / s, lse2, 0.0f);
       a.loss_rows[t] = loss;
+    }
+  } else if (a.packed != nullptr) {
+    const int left = a.st->count - a.row0;
+    if (left > 0 && row < (left + kRowPad - 1) / kRowPad * kRowPad) {
+      const uint4 none = make_uint4(0, 0, 0, 0);
+      for (int i = threadIdx.x; i < a.row_words; i += blockDim.x) {
+        a.packed[static_cast<long long>(row) * a.row_words + i] = none;
+        if (a.packed_lo != nullptr) a.packed_lo[static_cast<long long>(row) * a.row_words + i] = none;
+      }
     }
   }
   if (a.loss == nullptr || !a.final_launch) return;
@@ -448,7 +503,7 @@ __global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
   if (DT == PO_F32) {
 #pragma unroll 2
     for (int c = c0 + threadIdx.x * 4; c < c1; c += 256 * 4) {
-      const float m = part[c >> 7].x;
+      const float m = part[c >> 8].x;
       const float f = m == -INFINITY ? (pcoef == pcoef ? 0.0f : pcoef) : pcoef * ex2(m - mm);
       const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(a.e) + base + c);
       const float x[4] = {fmaf(v.x, f, -flat), fmaf(v.y, f, -flat), fmaf(v.z, f, -flat), fmaf(v.w, f, -flat)};
@@ -468,7 +523,7 @@ __global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
       const int c = c0 + (i * 256 + static_cast<int>(threadIdx.x)) * 8;
       if (c < c1) {
         raw[i] = *reinterpret_cast<const uint4*>(static_cast<const __half*>(a.e) + base + c);
-        ms[i] = part[c >> 7].x;
+        ms[i] = part[c >> 8].x;
       }
     }
 #pragma unroll
@@ -666,12 +721,12 @@ int make_plan(Plan& p, const void* weight, long long w_ld, int dtype, long long 
   p.want_dh = want_dh, p.want_dw = want_dw, p.grads = want_dh || want_dw;
   p.ldp = round_up(D, 64);
   p.stage_w = p.f32 || reinterpret_cast<uintptr_t>(weight) % 16 != 0 || (w_ld * p.es) % 16 != 0;
-  p.nparts = cdiv(V, 128);
-  p.e_ld = round_up(V, 128);
+  p.nparts = cdiv(V, 256);
+  p.e_ld = round_up(V, 256);
   p.bk = p.f32 ? 64 : 128;
   long long most = chunk_rows;
   if (most <= 0) {
-    // Without gradients a row leaves 8 bytes per 128 columns.
+    // Without gradients a row leaves 8 bytes per 256 columns.
     const long long per_row = p.grads ? p.e_ld * (p.f32 ? 8 : 2) : static_cast<long long>(p.nparts) * 8;
     most = kDefaultChunkBytes / per_row;
   }
@@ -712,7 +767,7 @@ int make_plan(Plan& p, const void* weight, long long w_ld, int dtype, long long 
     const long long rows = round_up(p.chunk, kRowPad);
     p.e = ar.take(static_cast<size_t>(rows) * p.e_ld * p.es);
     if (p.f32) p.e_lo = f32(rows * p.e_ld);
-    const long long pld = round_up(D, 128);
+    const long long pld = round_up(D, 256);
     long long partial = 0;
     if (p.splits_dh > 1) partial = p.splits_dh * p.chunk * pld;
     if (p.splits_dw > 1 && p.splits_dw * V * pld > partial) partial = p.splits_dw * V * pld;
@@ -755,10 +810,13 @@ int run_head(const Plan& p, int product, HeadParams& P, const HeadOperand& A, co
                : dispatch_head<KIND_BF16>(product, P, static_cast<int>(tiles), s);
 }
 
-// K blocks summed inside the tensor core's accumulator. Losses: 256 of K, a
-// truncation of under 1e-6 of a logit. Gradients in 16-bit types round to
-// 2^-9: 2048 of K.
-constexpr int kChunkStats16 = 2, kChunkStats32 = 2, kChunkGrad16 = 16, kChunkGrad32 = 2;
+// K blocks summed inside the tensor core's accumulator. Relative error of a
+// mean loss at D = 768 / 4096 with 2, 4, 8 blocks (256, 512, 1024 of K):
+// 2.3e-7 / 1.6e-7, 4.1e-7 / 3.1e-7, 6.9e-7 / 6.7e-7; time of the 4096 x 128256
+// x 4096 logits 4.33, 3.59, 3.38 ms before the epilogue's other steps, 3.40
+// and 3.39 ms (4, 8 blocks) after them. fp32 gradients: 5.3e-7, 6.7e-7 and
+// 1.1e-6 with 2, 4, 8 blocks (64 of K each); 16-bit ones round to 2^-9.
+constexpr int kChunkStats16 = 4, kChunkStats32 = 4, kChunkGrad16 = 16, kChunkGrad32 = 4;
 
 bool vec32(const void* p, long long ld, int es) {
   return reinterpret_cast<uintptr_t>(p) % 32 == 0 && (ld * es) % 32 == 0;
@@ -846,22 +904,22 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
   const float gscale = dtype == PO_F16 ? kF16Scale : 1.0f;
   PackArgs pa{};
   pa.hidden = hidden, pa.h_ld = h_ld, pa.T = tokens, pa.D = D, pa.ldp = static_cast<int>(p.ldp);
-  pa.vec = !p.f32 && D % 8 == 0 && reinterpret_cast<uintptr_t>(hidden) % 16 == 0 && h_ld % 8 == 0;
+  pa.vec = D * p.es % 16 == 0 && reinterpret_cast<uintptr_t>(hidden) % 16 == 0 && h_ld * p.es % 16 == 0;
   pa.tg = tg, pa.V = vocab, pa.status = p.status, pa.ent = p.ent, pa.rowmap = p.rowmap;
-  pa.packed = p.packed, pa.packed_lo = p.packed_lo, pa.rows_alloc = p.rows_alloc;
+  pa.packed = p.packed, pa.packed_lo = p.packed_lo;
   pa.dhidden = dhidden, pa.dh_ld = dh_ld, pa.loss_rows = loss_rows, pa.st = p.st, pa.sched = p.sched;
   pa.alpha = temperature / gscale, pa.mean = mean, pa.has_row_grad = row_grad != nullptr;
-  const int pblocks = cdiv(T, kPackRows);
-  if (dtype == PO_F32) pack_kernel<PO_F32><<<pblocks, 256, 0, s>>>(pa);
-  else if (dtype == PO_BF16) pack_kernel<PO_BF16><<<pblocks, 256, 0, s>>>(pa);
-  else pack_kernel<PO_F16><<<pblocks, 256, 0, s>>>(pa);
+  const int groups = cdiv(T, 2048 * kPackWarps), pblocks = cdiv(T, groups * kPackWarps);
+  if (dtype == PO_F32) pack_kernel<PO_F32><<<pblocks, 32 * kPackWarps, 0, s>>>(pa, groups);
+  else if (dtype == PO_BF16) pack_kernel<PO_BF16><<<pblocks, 32 * kPackWarps, 0, s>>>(pa, groups);
+  else pack_kernel<PO_F16><<<pblocks, 32 * kPackWarps, 0, s>>>(pa, groups);
   if ((r = check_cuda(cudaGetLastError(), "linear_loss pack"))) return r;
 
   const void* w = weight;
   long long wld = w_ld;
   if (p.stage_w) {
-    if (p.f32) stage_weight_kernel<PO_F32><<<8 * sms, 256, 0, s>>>(weight, w_ld, vocab, D, static_cast<int>(p.ldp), p.w, p.w_lo);
-    else stage_weight_kernel<PO_BF16><<<8 * sms, 256, 0, s>>>(weight, w_ld, vocab, D, static_cast<int>(p.ldp), p.w, nullptr);
+    if (p.f32) stage_weight_kernel<PO_F32><<<8 * sms, 256, 0, s>>>(weight, w_ld, vocab, D, static_cast<int>(p.ldp), p.w, p.w_lo, dim % 4 == 0 && w_ld % 4 == 0 && reinterpret_cast<uintptr_t>(weight) % 16 == 0);
+    else stage_weight_kernel<PO_BF16><<<8 * sms, 256, 0, s>>>(weight, w_ld, vocab, D, static_cast<int>(p.ldp), p.w, nullptr, 0);
     if ((r = check_cuda(cudaGetLastError(), "linear_loss stage"))) return r;
     w = p.w;
     wld = p.ldp;
@@ -898,7 +956,12 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
     fa.top = static_cast<int>(top), fa.smoothing = smoothing, fa.z_loss = z_loss, fa.temperature = temperature;
     fa.inv_vocab = 1.0f / static_cast<float>(vocab), fa.stat = p.stat, fa.loss_rows = loss_rows, fa.loss = loss;
     fa.T = tokens, fa.mean = mean, fa.final_launch = c == p.nchunks - 1, fa.st = p.st;
-    finish_kernel<<<rows, 128, 0, s>>>(fa);
+    if (p.want_dw) {
+      fa.packed = static_cast<uint4*>(p.packed) + hoff * p.es / 16;
+      fa.packed_lo = p.f32 ? reinterpret_cast<uint4*>(p.packed_lo + hoff) : nullptr;
+      fa.row_words = static_cast<int>(p.ldp * p.es / 16);
+    }
+    finish_kernel<<<static_cast<int>(p.want_dw ? krows : rows), 128, 0, s>>>(fa);
     if ((r = check_cuda(cudaGetLastError(), "linear_loss finish"))) return r;
     if (!p.grads) continue;
 
@@ -915,7 +978,7 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
     else rescale_kernel<PO_F16><<<static_cast<int>(rblocks), 256, 0, s>>>(ra, nseg);
     if ((r = check_cuda(cudaGetLastError(), "linear_loss rescale"))) return r;
 
-    const long long pld = round_up(dim, 128);
+    const long long pld = round_up(dim, 256);
     if (p.want_dh) {
       HeadParams P;
       memset(&P, 0, sizeof(P));

@@ -6,7 +6,7 @@ Three functions of CUDA tensors (bf16, fp16 or fp32), differentiable by
 
 * ``linear_cross_entropy(hidden, weight, target)`` — softmax cross entropy of
   ``hidden @ weight.T`` without that product as a tensor: per-token losses
-  leave two numbers a row and 128 columns, gradients the scaled exponentials
+  leave two numbers a row and 256 columns, gradients the scaled exponentials
   of one chunk of rows in 16 bits while the call runs;
 * ``linear_distillation(hidden, weight, teacher_index, teacher_logits)`` — the
   divergence of the same product's softmax from a teacher's top logits;
