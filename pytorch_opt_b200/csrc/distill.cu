@@ -6,11 +6,10 @@
 //
 // Bound by memory: each logit is read once and each gradient written once (4
 // bytes a logit in 16-bit types). A row's sum has to be known before its first
-// gradient is written, so a row stays on the chip in between: a cluster of up
-// to 8 CTAs shares one row, each CTA keeps its segment in shared memory, and
-// the CTAs exchange their (max, sum) through distributed shared memory. Short
-// segments keep several CTAs on an SM, so that one loads while another writes;
-// a single long row is spread over 8 SMs.
+// gradient is written, so a row is read twice, the second time from L2: one CTA
+// a row keeps about 300 rows in work, 76 MB at 128 thousand 16-bit columns.
+// Where there are too few rows for that, a cluster of up to 8 CTAs shares one
+// and exchanges (max, sum) through distributed shared memory.
 #include <climits>
 #include <cmath>
 
@@ -44,8 +43,7 @@ struct DistillArgs {
   float* loss_rows;
   float* loss;
   DistillState* st;
-  int seg;     // elements a CTA takes
-  int cached;  // the segment stays in shared memory
+  int seg;  // elements a CTA takes
 };
 
 // Whether the row has an entry with mass; bad indices are found here too.
@@ -75,220 +73,323 @@ __global__ void __launch_bounds__(256) count_rows_kernel(DistillArgs a) {
   if (lane == 0 && n > 0) atomicAdd(&a.st->count, n);
 }
 
-__device__ __forceinline__ float4 ld_cluster_f4(const float4* p, uint32_t rank) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(mapa_shared(smem_u32(p), rank))
-               : "memory");
-  return v;
-}
 __device__ __forceinline__ uint32_t cluster_nctarank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st_cluster_f2(const float2* p, uint32_t rank, float x, float y) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(mapa_shared(smem_u32(p), rank)), "f"(x), "f"(y)
+               : "memory");
+}
 
-// (m, s) <- (m, s) joined with 2^(scale2 x); the sum is kept relative to the
-// maximum, which is subtracted before the scaling: z - m is exact where it matters.
-template <int N>
-__device__ __forceinline__ void online_add(const float (&x)[N], float scale2, float& m, float& s) {
-  float c = x[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) c = fmaxf(c, x[i]);
+// Two fp32 operations an instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// The warp's (m, s) joined: sums of 2^(scale2 z) relative to their maxima. An
+// empty one holds (-inf, 0), or a NaN sum, which is kept.
+__device__ __forceinline__ void warp_join(float scale2, float& m, float& s) {
+  const float top = warp_max(m);
+  s = warp_sum(m == -INFINITY ? s : s * ex2((m - top) * scale2));
+  m = top;
+}
+
+// Largest of a vector's values: the 16-bit types compare two at a time.
+template <int DT>
+__device__ __forceinline__ float max16(const uint4& v) {
+  if constexpr (DT == PO_F32) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  } else if constexpr (DT == PO_BF16) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  } else {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+}
+
+// (m, s) <- (m, s) joined with a vector of logits.
+template <int DT>
+__device__ __forceinline__ void online_add(const uint4& raw, float scale2, float& m, float& s) {
+  constexpr int N = DT == PO_F32 ? 4 : 8;
+  const float c = max16<DT>(raw);
   if (c > m) {
     s *= ex2((m - c) * scale2);
     m = c;
   }
-  const float off = m == -INFINITY ? 0.0f : m;
-  float add = 0.0f;
+  // The scaled maximum is rounded once and every exponential sees the same
+  // rounding: at most 2^-24 of m scale2, the size of the logits' own.
+  const float off = m == -INFINITY ? 0.0f : -m * scale2;
+  const uint64_t off2 = pack2(off, off), sc2 = pack2(scale2, scale2);
+  float x[N];
+  unpack16<DT>(raw, x);
+  uint64_t add = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) add += ex2((x[i] - off) * scale2);
-  s += add;
+  for (int i = 0; i < N; i += 2) {
+    const float2 e = unpack2(fma2(pack2(x[i], x[i + 1]), sc2, off2));
+    add = add2(add, pack2(ex2(e.x), ex2(e.y)));
+  }
+  const float2 a = unpack2(add);
+  s += a.x + a.y;
 }
 
-constexpr int kDistillThreads = 256;
+// Threads a CTA has at most (and one warp more), and CTAs an SM should hold.
+// With gradients 512 and 2: the rows in work (256 KB each at 128 thousand
+// 16-bit columns) stay in L2 between their two reads; 2048 such rows 224 us,
+// with 256 threads 257 us. Without: 256 and 5, 94 us against 107 us.
+constexpr int kGradThreads = 512, kEvalThreads = 256;
+constexpr int kMaxPairs = 8 * kGradThreads / 32;
 
+// A CTA's part of one row: the vectors of its segment lie on 16-byte
+// boundaries of the logits; the first holds `mis` elements that belong to
+// someone else, and so may the last. Whole vectors j0 .. j1 - 1 go to the
+// threads in turn, the up to two others (read and written element by element)
+// to threads 0 and 1.
+template <typename T>
+struct Segment {
+  static constexpr int VEC = 16 / sizeof(T);
+  const T* z0;
+  int mis, end, j0, j1, edge;
+  __device__ __forceinline__ Segment(const T* row, int s0, int s1) {
+    mis = static_cast<int>((reinterpret_cast<uintptr_t>(row + s0) / sizeof(T)) % VEC);
+    z0 = row + s0 - mis;
+    end = s1 - s0 + mis;
+    j0 = mis > 0 ? 1 : 0;
+    j1 = end / VEC;
+    const int nvec = (end + VEC - 1) / VEC;
+    edge = -1;
+    if (threadIdx.x == 0 && j0 > 0 && nvec > 0) edge = 0;
+    if (threadIdx.x == 1 && j1 < nvec && j1 >= j0) edge = j1;
+  }
+  __device__ __forceinline__ uint4 load_edge() const {  // others' elements read as -inf
+    uint4 raw;
+    T* o = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int c = edge * VEC + i;
+      from_f32(-INFINITY, o[i]);
+      if (c >= mis && c < end) o[i] = z0[c];
+    }
+    return raw;
+  }
+  __device__ __forceinline__ void put(T* out0, int j, const uint4& v) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int c = j * VEC + i;
+      if (c >= mis && c < end) out0[c] = reinterpret_cast<const T*>(&v)[i];
+    }
+  }
+};
+
+// In each of a row's CTAs
+//   the last warp takes the teacher's entries, their distribution and the
+//   logits there (three dependent loads, which would hold up the row if a
+//   warp with a share of the segment made them);
+//   the others run over their vectors of the segment (each thread its own)
+//   and hand each warp's (max, sum) to every CTA of the row;
+//   after one barrier of the row's CTAs every thread joins the row's pairs in
+//   the same order and writes its own vectors' gradients, while the last warp
+//   of the first CTA writes the loss.
 template <int DT, bool GRAD>
-__global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a) {
+__global__ void __launch_bounds__((GRAD ? kGradThreads : kEvalThreads) + 32, GRAD ? 2 : 5)
+    distill_kernel(DistillArgs a) {
   using T = typename ElemOf<DT>::T;
   constexpr int VEC = 16 / sizeof(T);
   extern __shared__ __align__(16) uint8_t sm[];
-  __shared__ float buf[32];
+  __shared__ float2 s_pairs[kMaxPairs];  // (max, sum) of every warp of the row's CTAs
   __shared__ double dbuf[32];
-  __shared__ __align__(16) float4 s_share;
-  __shared__ int s_last;
+  __shared__ float s_qlogq;
+  __shared__ int s_status, s_last;
   const uint32_t cs = cluster_nctarank(), rank = cluster_ctarank();
   const long long t = blockIdx.x / cs;
-  int* si = reinterpret_cast<int*>(sm);            // entries' indices (-1: none)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nthreads = blockDim.x - 32, nwarps = nthreads >> 5;
+  const bool teacher_warp = warp == nwarps;
+  int* si = reinterpret_cast<int*>(sm);              // entries' indices (-1: none)
   float* sq = reinterpret_cast<float*>(si + a.top);  // q
   float* sz = sq + a.top;                            // logits at the entries
-  T* cache = reinterpret_cast<T*>(sm + (static_cast<size_t>(a.top) * 12 + 15) / 16 * 16);
   const float scale2 = kLog2e / a.temperature;
-
   const T* z = static_cast<const T*>(a.z) + t * a.ld;
   const int s0 = min(static_cast<long long>(rank) * a.seg, static_cast<long long>(a.V));
   const int s1 = min(static_cast<long long>(s0) + a.seg, static_cast<long long>(a.V));
-  // Vectors lie on 16-byte boundaries of the logits; the first holds `mis`
-  // elements that belong to someone else (never read).
-  const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(z + s0) / sizeof(T)) % VEC);
-  const int nvec = (s1 - s0 + mis + VEC - 1) / VEC;
-
-  // Teacher's distribution (every CTA of the row for itself).
-  float tm = -INFINITY;
-  bool bad = false, mass = false;
-  for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
-    long long x;
-    float l;
-    const int e = entry_status(a, t, k, x, l);
-    bad |= e == ROW_BAD;
-    mass |= e == ROW_COUNTED;
-    const bool there = x >= 0 && x < a.V;
-    si[k] = there ? static_cast<int>(x) : -1;
-    l = there ? l / a.temperature : -INFINITY;
-    sq[k] = l;
-    sz[k] = there ? to_f32(z[x]) : 0.0f;
-    tm = fmaxf(tm, l);
-  }
-  bad = __syncthreads_or(bad);
-  mass = __syncthreads_or(mass);
+  const Segment<T> g(z, s0, s1);
+  const uint4* src = reinterpret_cast<const uint4*>(g.z0);
+  if (cs > 1) cluster_arrive_relaxed();  // this CTA runs: its shared memory may be written
 
   float m = -INFINITY, s = 0.0f;
-  float qlogq = 0.0f;
-  if (mass && !bad) {
-    // Segment: running maximum and sum, four vectors in flight a thread.
-    const T* z0 = z + s0 - mis;
-    for (int j0 = threadIdx.x; j0 < nvec; j0 += 4 * kDistillThreads) {
-      uint4 raw[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int j = j0 + u * kDistillThreads;
-        if (j >= nvec) continue;
-        if ((j > 0 || mis == 0) && (j + 1) * VEC <= s1 - s0 + mis) {
-          raw[u] = __ldcs(reinterpret_cast<const uint4*>(z0) + j);
-        } else {
-          T* o = reinterpret_cast<T*>(&raw[u]);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const int c = j * VEC + i;
-            from_f32(-INFINITY, o[i]);
-            if (c >= mis && c < s1 - s0 + mis) o[i] = z0[c];
-          }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int j = j0 + u * kDistillThreads;
-        if (j >= nvec) continue;
-        float x[VEC];
-        const T* o = reinterpret_cast<const T*>(&raw[u]);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) x[i] = to_f32(o[i]);
-        online_add(x, scale2, m, s);
-        if (GRAD && a.cached) reinterpret_cast<uint4*>(cache)[j] = raw[u];
-      }
+  if (teacher_warp) {
+    const float inv_temp = 1.0f / a.temperature;
+    float tm = -INFINITY;
+    int bad = 0, mass = 0;
+#pragma unroll 4
+    for (int k = lane; k < a.top; k += 32) {
+      const long long x = a.index[t * a.index_ld + k];
+      const float l = load_as_f32(a.teacher, a.teacher_dtype, t * a.teacher_ld + k) * inv_temp;
+      const bool there = x >= 0 && x < a.V;
+      bad |= x >= a.V;
+      mass |= there && !(l == -INFINITY);
+      si[k] = there ? static_cast<int>(x) : -1;
+      sq[k] = there ? l : -INFINITY;
+      sz[k] = there ? to_f32(z[x]) : 0.0f;
+      if (there) tm = fmaxf(tm, l);
     }
-    const float mm = block_max(m, buf);
-    s = block_sum(m == -INFINITY ? s : s * ex2((m - mm) * scale2), buf);
-    m = mm;
-    // q and sum q log q
-    tm = block_max(tm, buf);
+    bad = __any_sync(0xffffffffu, bad);
+    mass = __any_sync(0xffffffffu, mass);
+    tm = warp_max(tm);
     float sum = 0.0f;
-    for (int k = threadIdx.x; k < a.top; k += kDistillThreads)
-      if (si[k] >= 0) sum += expf(sq[k] - tm);
-    sum = block_sum(sum, buf);
-    const float logsum = logf(sum);
-    for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
+    for (int k = lane; k < a.top; k += 32) {
+      const float e = si[k] >= 0 ? expf(sq[k] - tm) : 0.0f;
+      sum += e;
+    }
+    sum = warp_sum(sum);
+    const float logsum = logf(sum), inv_sum = 1.0f / sum;
+    float c = 0.0f;
+    for (int k = lane; k < a.top; k += 32) {
       float q = 0.0f;
       if (si[k] >= 0) {
-        q = expf(sq[k] - tm) / sum;
-        if (q != 0.0f) qlogq += q * (sq[k] - tm - logsum);
+        q = expf(sq[k] - tm) * inv_sum;
+        if (q != 0.0f) c += q * (sq[k] - tm - logsum);
       }
       sq[k] = q;
     }
-    qlogq = block_sum(qlogq, buf);
-    // Join the row's CTAs, each in rank order.
-    if (cs > 1) {
-      if (threadIdx.x == 0) s_share = make_float4(m, s, 0.0f, 0.0f);
-      cluster_sync();
-      float gm = -INFINITY, gs = 0.0f;
-      float4 v[8];
-#pragma unroll
-      for (uint32_t r = 0; r < 8; ++r)
-        if (r < cs) {
-          v[r] = ld_cluster_f4(&s_share, r);
-          gm = fmaxf(gm, v[r].x);
-        }
-#pragma unroll
-      for (uint32_t r = 0; r < 8; ++r)
-        if (r < cs) gs += v[r].x == -INFINITY ? v[r].y : v[r].y * ex2((v[r].x - gm) * scale2);
-      m = gm;
-      s = gs;
+    c = warp_sum(c);
+    if (lane == 0) {
+      s_qlogq = c;
+      s_status = bad ? ROW_BAD : (mass ? ROW_COUNTED : ROW_IGNORED);
     }
+  } else {
+    for (int j = g.j0 + threadIdx.x; j < g.j1; j += 4 * nthreads) {  // four loads in flight
+      uint4 raw[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (j + u * nthreads < g.j1) raw[u] = GRAD ? __ldcg(src + j + u * nthreads) : __ldcs(src + j + u * nthreads);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (j + u * nthreads < g.j1) online_add<DT>(raw[u], scale2, m, s);
+    }
+    if (g.edge >= 0) online_add<DT>(g.load_edge(), scale2, m, s);
+    warp_join(scale2, m, s);
   }
-  const float logs = logf(s);  // log sum exp(z / a) = m / a + logs
+  // Every warp's pair to every CTA of the row; one barrier for the row (and
+  // for what the teacher's warp left in shared memory).
+  if (cs > 1) {
+    cluster_wait();
+    if (lane < cs && !teacher_warp) st_cluster_f2(s_pairs + rank * nwarps + warp, lane, m, s);
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    if (lane == 0 && !teacher_warp) s_pairs[warp] = make_float2(m, s);
+    __syncthreads();
+  }
+  {
+    const int npairs = static_cast<int>(cs) * nwarps;
+    float2 p[kMaxPairs / 32];
+    m = -INFINITY;
+    s = 0.0f;
+#pragma unroll
+    for (int u = 0; u < kMaxPairs / 32; ++u) {
+      p[u] = lane + 32 * u < npairs ? s_pairs[lane + 32 * u] : make_float2(-INFINITY, 0.0f);
+      m = fmaxf(m, p[u].x);
+    }
+#pragma unroll
+    for (int u = 0; u < kMaxPairs / 32; ++u) s += p[u].x == -INFINITY ? p[u].y : p[u].y * ex2((p[u].x - m) * scale2);
+    warp_join(scale2, m, s);
+  }
+  const int status = s_status;
+  const bool live = status == ROW_COUNTED;
 
-  if (rank == 0) {
-    float c = 0.0f;
-    if (mass && !bad)
-      for (int k = threadIdx.x; k < a.top; k += kDistillThreads)
+  if (teacher_warp) {
+    if (rank == 0) {
+      float c = 0.0f;
+      const float logs = logf(s);  // log sum exp(z / a) = m / a + logs
+      for (int k = lane; k < a.top; k += 32)
         if (sq[k] != 0.0f) c += sq[k] * ((m - sz[k]) / a.temperature + logs);
-    c = block_sum(c, buf);
-    if (threadIdx.x == 0) {
-      float loss = 0.0f;
-      if (bad) loss = NAN;
-      else if (mass) loss = a.temperature * a.temperature * (qlogq + c);
-      a.loss_rows[t] = loss;
+      c = warp_sum(c);
+      if (lane == 0) {
+        a.loss_rows[t] = live ? a.temperature * a.temperature * (s_qlogq + c) : (status == ROW_BAD ? NAN : 0.0f);
+        if (a.loss != nullptr) {
+          __threadfence();
+          s_last = atomicAdd(&a.st->done, 1u) == static_cast<unsigned int>(a.T) - 1;
+        }
+      }
     }
-  }
-
-  if (GRAD) {
+  } else if (GRAD) {
     T* out = static_cast<T*>(a.dz) + t * a.dz_ld;
+    T* out0 = out + s0 - g.mis;
+    uint4* dst = reinterpret_cast<uint4*>(out0);
+    const bool vec = reinterpret_cast<uintptr_t>(out0) % 16 == 0;
     float w = 0.0f;
-    if (mass && !bad) {
+    if (live) {
       w = a.temperature;
       if (a.mean) w /= static_cast<float>(a.st->count);
       if (a.row_grad != nullptr) w *= a.row_grad[t];
     }
-    const float ws = w / s;
-    const T* z0 = z + s0 - mis;
-    T* out0 = out + s0 - mis;
-    const bool vec = (reinterpret_cast<uintptr_t>(out0) % 16) == 0;
-    const bool live = mass && !bad;
-    for (int j = threadIdx.x; j < nvec; j += kDistillThreads) {
-      const bool whole = (j > 0 || mis == 0) && (j + 1) * VEC <= s1 - s0 + mis;
-      uint4 raw = make_uint4(0, 0, 0, 0), res = make_uint4(0, 0, 0, 0);
-      const T* o = reinterpret_cast<const T*>(&raw);
-      T* d = reinterpret_cast<T*>(&res);
-      if (live) {
-        if (a.cached) {
-          raw = reinterpret_cast<const uint4*>(cache)[j];
-        } else if (whole) {
-          raw = reinterpret_cast<const uint4*>(z0)[j];
-        } else {
+    const float ws = w / s, off = -m * scale2;
+    const auto grad = [&](const uint4& raw) {
+      const uint64_t off2 = pack2(off, off), sc2 = pack2(scale2, scale2), w2 = pack2(ws, ws);
+      float x[VEC];
+      unpack16<DT>(raw, x);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const int c = j * VEC + i;
-            if (c >= mis && c < s1 - s0 + mis) reinterpret_cast<T*>(&raw)[i] = z0[c];
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) from_f32(ws * ex2((to_f32(o[i]) - m) * scale2), d[i]);
+      for (int i = 0; i < VEC; i += 2) {
+        const float2 e = unpack2(fma2(pack2(x[i], x[i + 1]), sc2, off2));
+        const float2 p = unpack2(mul2(pack2(ex2(e.x), ex2(e.y)), w2));
+        x[i] = p.x;
+        x[i + 1] = p.y;
       }
-      if (whole && vec) {
-        __stcs(reinterpret_cast<uint4*>(out0) + j, res);
-      } else {
+      return pack16<DT>(x);
+    };
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    // The second read of the segment comes from L2: the rows that are being
+    // worked on fit there.
+    if (!vec) {
+      for (int j = g.j0 + threadIdx.x; j < g.j1; j += nthreads) g.put(out0, j, live ? grad(src[j]) : none);
+    } else if (!live) {
+      for (int j = g.j0 + threadIdx.x; j < g.j1; j += nthreads) __stcs(dst + j, none);
+    } else {
+      for (int j = g.j0 + threadIdx.x; j < g.j1; j += 4 * nthreads) {
+        uint4 raw[4];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const int c = j * VEC + i;
-          if (c >= mis && c < s1 - s0 + mis) out0[c] = d[i];
-        }
+        for (int u = 0; u < 4; ++u)
+          if (j + u * nthreads < g.j1) raw[u] = __ldcs(src + j + u * nthreads);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (j + u * nthreads < g.j1) __stcs(dst + j + u * nthreads, grad(raw[u]));
       }
     }
+    if (g.edge >= 0) g.put(out0, g.edge, live ? grad(g.load_edge()) : none);
     // The entries' places again, with q taken off before the one rounding.
-    __syncthreads();
+    asm volatile("bar.sync 1, %0;" ::"r"(nthreads) : "memory");
     if (live) {
-      for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
+      for (int k = threadIdx.x; k < a.top; k += nthreads) {
         const int c = si[k];
         if (c < s0 || c >= s1) continue;
         float goal = 0.0f;
@@ -298,22 +399,18 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
           first = first && j >= k;
           goal += sq[j];
         }
-        if (first) from_f32(w * (ex2((sz[k] - m) * scale2) / s - goal), out[c]);
+        if (first) from_f32(ws * ex2(fmaf(sz[k], scale2, off)) - w * goal, out[c]);
       }
     }
   }
-  if (cs > 1 && mass && !bad) cluster_sync();  // no CTA leaves while another reads its share
 
+  // The last row to finish sums the losses of all rows in a fixed order.
   if (a.loss == nullptr || rank != 0) return;
-  if (threadIdx.x == 0) {
-    __threadfence();
-    s_last = atomicAdd(&a.st->done, 1u) == static_cast<unsigned int>(a.T) - 1;
-  }
   __syncthreads();
   if (!s_last) return;
   __threadfence();
   double sum = 0.0;
-  for (long long r = threadIdx.x; r < a.T; r += kDistillThreads) sum += static_cast<double>(__ldcg(a.loss_rows + r));
+  for (long long r = threadIdx.x; r < a.T; r += blockDim.x) sum += static_cast<double>(__ldcg(a.loss_rows + r));
   sum = block_sum(sum, dbuf);
   if (threadIdx.x == 0) {
     if (a.mean) sum /= static_cast<double>(a.st->count > 0 ? a.st->count : 1);
@@ -322,18 +419,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
 }
 
 template <int DT, bool GRAD>
-int launch_distill(const DistillArgs& a, int cs, size_t smem, cudaStream_t s) {
-  auto kern = distill_kernel<DT, GRAD>;
-  static bool configured[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return set_error(PO_ERR_CUDA, "device ordinal out of range");
-  if (!configured[dev]) {
-    const int r = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 120 << 10),
-                             "cudaFuncSetAttribute");
-    if (r) return r;
-    configured[dev] = true;
-  }
+int launch_distill(const DistillArgs& a, int cs, int threads, cudaStream_t s) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -341,12 +427,12 @@ int launch_distill(const DistillArgs& a, int cs, size_t smem, cudaStream_t s) {
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3(static_cast<unsigned>(a.T * cs), 1, 1);
-  cfg.blockDim = dim3(kDistillThreads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3(threads + 32, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(a.top) * 12;
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern, a), "distill launch");
+  cfg.numAttrs = cs > 1 ? 1 : 0;
+  return check_cuda(cudaLaunchKernelEx(&cfg, distill_kernel<DT, GRAD>, a), "distill launch");
 }
 
 template <int DT>
@@ -414,22 +500,22 @@ extern "C" int po_distill_logits(const void* logits, long long ld, int dtype, lo
     count_rows_kernel<<<blocks, 256, 0, s>>>(a);
     if (int r = check_cuda(cudaGetLastError(), "distill_logits count")) return r;
   }
-  // CTAs a row: segments of at most 32 KB (several CTAs on an SM), and all 8
-  // when there are too few rows to fill the SMs otherwise.
+  // CTAs a row: one, unless there are too few rows to fill the SMs.
   const int es = dtype_size(dtype);
   int cs = 1;
-  while (cs < 8 && (vocab * es > cs * (32LL << 10) || (tokens * cs < 2 * sm_count() && vocab > cs * 2048LL))) cs *= 2;
+  while (cs < 8 && tokens * cs < 2 * sm_count() && vocab > cs * 2048LL) cs *= 2;
   const int vec = 16 / es;
   a.seg = static_cast<int>(round_up((vocab + cs - 1) / cs, vec));
-  const size_t entries = (static_cast<size_t>(top) * 12 + 15) / 16 * 16;
-  const size_t seg_bytes = static_cast<size_t>(a.seg + 2 * vec) * es;
-  a.cached = dlogits != nullptr && seg_bytes <= (96u << 10);
-  const size_t smem = entries + (a.cached ? seg_bytes : 0);
+  // About sixteen vectors a thread.
+  const long long nvec = (a.seg + vec - 1) / vec + 1;
+  int threads = static_cast<int>(round_up((nvec + 15) / 16, 32));
   const bool g = dlogits != nullptr;
-  if (dtype == PO_F32) return g ? launch_distill<PO_F32, true>(a, cs, smem, s) : launch_distill<PO_F32, false>(a, cs, smem, s);
+  const int most = g ? kGradThreads : kEvalThreads;
+  threads = threads < 64 ? 64 : (threads > most ? most : threads);
+  if (dtype == PO_F32) return g ? launch_distill<PO_F32, true>(a, cs, threads, s) : launch_distill<PO_F32, false>(a, cs, threads, s);
   if (dtype == PO_BF16)
-    return g ? launch_distill<PO_BF16, true>(a, cs, smem, s) : launch_distill<PO_BF16, false>(a, cs, smem, s);
-  return g ? launch_distill<PO_F16, true>(a, cs, smem, s) : launch_distill<PO_F16, false>(a, cs, smem, s);
+    return g ? launch_distill<PO_BF16, true>(a, cs, threads, s) : launch_distill<PO_BF16, false>(a, cs, threads, s);
+  return g ? launch_distill<PO_F16, true>(a, cs, threads, s) : launch_distill<PO_F16, false>(a, cs, threads, s);
 }
 
 extern "C" int po_scale_inplace(void* x, int dtype, long long n, const float* factor, void* stream) {

@@ -34,6 +34,42 @@ __device__ __forceinline__ void from_f32(float v, float& o) { o = v; }
 __device__ __forceinline__ void from_f32(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void from_f32(float v, __half& o) { o = __float2half_rn(v); }
 
+// 16 bytes of a type as floats and back, two 16-bit values an instruction.
+template <int DT>
+__device__ __forceinline__ void unpack16(const uint4& v, float (&x)[DT == PO_F32 ? 4 : 8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == PO_F32) {
+      x[i] = __uint_as_float(w[i]);
+    } else if constexpr (DT == PO_BF16) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+}
+template <int DT>
+__device__ __forceinline__ uint4 pack16(const float (&x)[DT == PO_F32 ? 4 : 8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == PO_F32) {
+      w[i] = __float_as_uint(x[i]);
+    } else if constexpr (DT == PO_BF16) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 __device__ __forceinline__ float load_as_f32(const void* p, int dtype, long long i) {
   if (dtype == PO_F32) return static_cast<const float*>(p)[i];
   if (dtype == PO_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
