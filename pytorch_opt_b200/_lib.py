@@ -6,6 +6,7 @@ fails loudly: there is no CPU or library fallback behind these entry points.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -121,7 +122,20 @@ def gemm_profile(enable: bool, read: bool = True) -> dict | None:
     return {name: int(out[i]) for i, name in enumerate(GEMM_PROFILE_SLOTS)}
 
 
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """``torch.cuda.device(device)``, or nothing where that is the current device already."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device: torch.device | None = None) -> int:
+    if _raw_stream is not None and device is not None and device.index is not None:
+        return _raw_stream(device.index)  # the same pointer without a Stream object around it
     return torch.cuda.current_stream(device).cuda_stream
 
 

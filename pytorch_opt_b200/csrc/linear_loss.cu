@@ -642,7 +642,11 @@ int encode_operand(CUtensorMap map[2], const HeadOperand& o) {
   const int es = dtype_size(o.dtype);
   const int w = 128 / es;
   for (int i = 0; i < 2; ++i) {
-    const void* p = o.p[i] != nullptr ? o.p[i] : o.p[0];
+    const void* p = o.p[i];
+    if (p == nullptr) {  // no low half: never read
+      map[i] = map[0];
+      continue;
+    }
     // K-major: 128 bytes of K x 128 rows; MN-major: 128 bytes of MN x a stage's 2 w rows of K.
     const int r = o.kmajor ? encode(&map[i], p, o.dtype, o.rows, o.cols, o.ld, w, 128, false)
                            : encode(&map[i], p, o.dtype, o.rows, o.cols, o.ld, w, 2 * w, true);

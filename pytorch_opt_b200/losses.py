@@ -24,6 +24,8 @@ CPU path.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -33,18 +35,16 @@ _REDUCTIONS = ("mean", "sum", "none")
 MAX_TOP = 1024
 
 
-def _check_tensors(name: str, *tensors) -> torch.device:
-    dev = None
-    for t in tensors:
+def _check_tensors(name: str, first, *others) -> None:
+    for t in (first, *others):
         if not isinstance(t, torch.Tensor):
             raise RuntimeError(f"{name}: expected a tensor, got {type(t).__name__}")
         if not t.is_cuda:
             raise RuntimeError("pytorch_opt_b200 runs on CUDA tensors only (there is no CPU path)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+    at = first.device
+    for t in others:
+        if t.device != at:
             raise RuntimeError("all tensors must be on the same CUDA device")
-    return dev
 
 
 def _check_reduction(name: str, reduction: str) -> None:
@@ -54,9 +54,12 @@ def _check_reduction(name: str, reduction: str) -> None:
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """The tensor as rows of its last axis, each contiguous (a copy only if they are not)."""
-    x = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
-    if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
-        x = x.contiguous()
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    if not x.is_contiguous():
+        rows, cols = x.shape
+        if cols > 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < cols:
+            x = x.contiguous()
     return x
 
 
@@ -65,62 +68,83 @@ def _pitch(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
+@functools.lru_cache(maxsize=512)
+def _workspace_bytes(aligned: bool, *args) -> int:
+    # Of the weight's address the workspace depends only on whether TMA takes it.
+    return _lib.load().po_linear_loss_workspace_bytes(16 if aligned else 2, *args)
+
+
 def _linear_loss(hidden, weight, index, teacher, ignore_index, smoothing, z_loss, temperature, mean, scalar, row_grad,
                  want_dh, want_dw, chunk_rows):
     """One call of po_linear_loss: (per-row losses, scalar loss, dhidden, dweight)."""
     tokens, dim = hidden.shape
     vocab, top = weight.shape[0], index.shape[1]
-    dev = hidden.device
-    code = _lib.DTYPE_CODE[hidden.dtype]
-    with torch.cuda.device(dev):
-        lib = _lib.load()
+    dev, dtype = hidden.device, hidden.dtype
+    code, w_ptr, w_ld = _lib.DTYPE_CODE[dtype], weight.data_ptr(), _pitch(weight)
+    with _lib.on_device(dev):
         losses = torch.empty(tokens, dtype=torch.float32, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev) if scalar else None
-        dh = torch.empty(tokens, dim, dtype=hidden.dtype, device=dev) if want_dh else None
-        dw = torch.empty(vocab, dim, dtype=weight.dtype, device=dev) if want_dw else None
-        nbytes = lib.po_linear_loss_workspace_bytes(weight.data_ptr(), _pitch(weight), code, tokens, dim, vocab, top,
-                                                    int(want_dh), int(want_dw), chunk_rows)
+        dh = torch.empty((tokens, dim), dtype=dtype, device=dev) if want_dh else None
+        dw = torch.empty((vocab, dim), dtype=dtype, device=dev) if want_dw else None
+        nbytes = _workspace_bytes(w_ptr % 16 == 0, w_ld, code, tokens, dim, vocab, top, want_dh, want_dw, chunk_rows)
         ws = _lib.workspace(nbytes, dev)
-        _lib.check(lib.po_linear_loss(
-            hidden.data_ptr(), _pitch(hidden), weight.data_ptr(), _pitch(weight), code, tokens, dim, vocab,
-            index.data_ptr(), _pitch(index), teacher.data_ptr() if teacher is not None else None,
-            _pitch(teacher) if teacher is not None else 0,
-            _lib.DTYPE_CODE[teacher.dtype] if teacher is not None else 0, top, ignore_index, smoothing, z_loss,
-            temperature, int(mean), row_grad.data_ptr() if row_grad is not None else None, losses.data_ptr(),
-            loss.data_ptr() if scalar else None, dh.data_ptr() if want_dh else None, dim,
-            dw.data_ptr() if want_dw else None, dim, chunk_rows, ws.data_ptr(), nbytes, _lib.stream_ptr(dev)),
-            "po_linear_loss")
+        if teacher is None:
+            t_ptr, t_ld, t_code = None, 0, 0
+        else:
+            t_ptr, t_ld, t_code = teacher.data_ptr(), _pitch(teacher), _lib.DTYPE_CODE[teacher.dtype]
+        status = _lib.load().po_linear_loss(
+            hidden.data_ptr(), _pitch(hidden), w_ptr, w_ld, code, tokens, dim, vocab, index.data_ptr(), _pitch(index),
+            t_ptr, t_ld, t_code, top, ignore_index, smoothing, z_loss, temperature, mean,
+            None if row_grad is None else row_grad.data_ptr(), losses.data_ptr(), loss.data_ptr() if scalar else None,
+            dh.data_ptr() if want_dh else None, dim, dw.data_ptr() if want_dw else None, dim, chunk_rows,
+            ws.data_ptr(), nbytes, _lib.stream_ptr(dev))
+        if status:
+            _lib.check(status, "po_linear_loss")
     return losses, loss, dh, dw
 
 
 def _distill_logits(logits, index, teacher, temperature, mean, scalar, row_grad, want_grad):
     """One call of po_distill_logits: (per-row losses, scalar loss, dlogits)."""
     tokens, vocab = logits.shape
-    dev = logits.device
-    with torch.cuda.device(dev):
+    dev, dtype = logits.device, logits.dtype
+    with _lib.on_device(dev):
         lib = _lib.load()
         losses = torch.empty(tokens, dtype=torch.float32, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev) if scalar else None
-        dz = torch.empty(tokens, vocab, dtype=logits.dtype, device=dev) if want_grad else None
-        nbytes = lib.po_distill_logits_workspace_bytes(tokens)
-        ws = _lib.workspace(nbytes, dev) if scalar else None
-        _lib.check(lib.po_distill_logits(
-            logits.data_ptr(), _pitch(logits), _lib.DTYPE_CODE[logits.dtype], tokens, vocab, index.data_ptr(),
-            _pitch(index), teacher.data_ptr(), _pitch(teacher), _lib.DTYPE_CODE[teacher.dtype], index.shape[1],
-            temperature, int(mean), row_grad.data_ptr() if row_grad is not None else None, losses.data_ptr(),
-            loss.data_ptr() if scalar else None, dz.data_ptr() if want_grad else None, vocab,
-            ws.data_ptr() if scalar else None, nbytes if scalar else 0, _lib.stream_ptr(dev)), "po_distill_logits")
+        dz = torch.empty((tokens, vocab), dtype=dtype, device=dev) if want_grad else None
+        loss = ws = None
+        nbytes = 0
+        if scalar:
+            loss = torch.empty((), dtype=torch.float32, device=dev)
+            nbytes = lib.po_distill_logits_workspace_bytes(tokens)
+            ws = _lib.workspace(nbytes, dev)
+        status = lib.po_distill_logits(
+            logits.data_ptr(), _pitch(logits), _lib.DTYPE_CODE[dtype], tokens, vocab, index.data_ptr(), _pitch(index),
+            teacher.data_ptr(), _pitch(teacher), _lib.DTYPE_CODE[teacher.dtype], index.shape[1], temperature, mean,
+            None if row_grad is None else row_grad.data_ptr(), losses.data_ptr(), loss.data_ptr() if scalar else None,
+            dz.data_ptr() if want_grad else None, vocab, ws.data_ptr() if scalar else None, nbytes,
+            _lib.stream_ptr(dev))
+        if status:
+            _lib.check(status, "po_distill_logits")
     return losses, loss, dz
 
 
-def _scaled(grad: torch.Tensor | None, factor: torch.Tensor) -> torch.Tensor | None:
-    """``grad`` times a device scalar, in place; a factor of 1 (``loss.backward()``) moves no data."""
-    if grad is not None:
-        with torch.cuda.device(grad.device):
-            _lib.check(_lib.load().po_scale_inplace(grad.data_ptr(), _lib.DTYPE_CODE[grad.dtype], grad.numel(),
-                                                    factor.data_ptr(), _lib.stream_ptr(grad.device)),
-                       "po_scale_inplace")
-    return grad
+def _upstream(up: torch.Tensor) -> torch.Tensor:
+    return up if up.dtype == torch.float32 and up.is_contiguous() else up.float().contiguous()
+
+
+def _scale(factor: torch.Tensor, *grads) -> None:
+    """Gradients times a device scalar, in place; a factor of 1 (``loss.backward()``) moves no data."""
+    dev = factor.device
+    with _lib.on_device(dev):
+        for g in grads:
+            if g is not None:
+                _lib.check(_lib.load().po_scale_inplace(g.data_ptr(), _lib.DTYPE_CODE[g.dtype], g.numel(),
+                                                        factor.data_ptr(), _lib.stream_ptr(dev)), "po_scale_inplace")
+
+
+def _records(*tensors) -> bool:
+    """Whether autograd would record a function of these."""
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
 class _LinearLoss(torch.autograd.Function):
@@ -142,12 +166,13 @@ class _LinearLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, up):
         reduction, chunk_rows, *terms = ctx.opts
-        up = up.float().contiguous()
+        up = _upstream(up)
         if reduction != "none":
             if ctx.grads is None:
                 raise RuntimeError("the gradients of this loss were handed out already: one backward pass per loss")
             (dh, dw), ctx.grads = ctx.grads, None
-            return _scaled(dh, up), _scaled(dw, up), None, None, None
+            _scale(up, dh, dw)
+            return dh, dw, None, None, None
         hidden, weight, index, teacher = ctx.saved_tensors
         _, _, dh, dw = _linear_loss(hidden, weight, index, teacher, *terms, False, False, up, *ctx.needs_input_grad[:2],
                                     chunk_rows)
@@ -170,14 +195,27 @@ class _Distillation(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, up):
-        up = up.float().contiguous()
+        up = _upstream(up)
         if ctx.scalar:
             if ctx.grad is None:
                 raise RuntimeError("the gradient of this loss was handed out already: one backward pass per loss")
             dz, ctx.grad = ctx.grad, None
-            return _scaled(dz, up), None, None, None, None
+            _scale(up, dz)
+            return dz, None, None, None, None
         logits, index, teacher = ctx.saved_tensors
         return _distill_logits(logits, index, teacher, ctx.temperature, False, False, up, True)[2], None, None, None, None
+
+
+def _head_loss(hidden, weight, index, teacher, reduction, chunk_rows, *terms):
+    lead = hidden.shape[:-1]
+    rows, head = _rows(hidden), _rows(weight)
+    if _records(hidden, weight):
+        out = _LinearLoss.apply(rows, head, index, teacher, (reduction, chunk_rows, *terms))
+    else:
+        each, scalar, _, _ = _linear_loss(rows, head, index, teacher, *terms, reduction == "mean", reduction != "none",
+                                          None, False, False, chunk_rows)
+        out = each if scalar is None else scalar
+    return out.reshape(lead) if reduction == "none" and len(lead) != 1 else out
 
 
 def _check_head(name: str, hidden: torch.Tensor, weight: torch.Tensor) -> None:
@@ -190,7 +228,7 @@ def _check_head(name: str, hidden: torch.Tensor, weight: torch.Tensor) -> None:
 
 
 def _check_teacher(name: str, lead, index: torch.Tensor, teacher: torch.Tensor, temperature: float):
-    if index.dtype not in (torch.int64, torch.int32):
+    if index.dtype != torch.int64 and index.dtype != torch.int32:
         raise RuntimeError(f"{name}: teacher_index must be int64 or int32, got {index.dtype}")
     if teacher.dtype not in _DTYPES:
         raise RuntimeError(f"{name}: teacher_logits must be fp32, bf16 or fp16, got {teacher.dtype}")
@@ -201,7 +239,7 @@ def _check_teacher(name: str, lead, index: torch.Tensor, teacher: torch.Tensor, 
         raise RuntimeError(f"{name}: 1 to {MAX_TOP} entries a token, got {index.shape[-1]}")
     if not (temperature > 0 and temperature < float("inf")):
         raise RuntimeError(f"{name}: temperature must be positive, got {temperature}")
-    return _rows(index.long()), _rows(teacher.detach())
+    return _rows(index.long()), _rows(teacher.detach() if teacher.requires_grad else teacher)
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100,
@@ -228,10 +266,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
         raise RuntimeError(f"{name}: label_smoothing must be in [0, 1] and z_loss finite")
     if chunk_rows < 0:
         raise RuntimeError(f"{name}: chunk_rows must not be negative")
-    lead = hidden.shape[:-1]
-    out = _LinearLoss.apply(_rows(hidden), _rows(weight), target.long().reshape(-1, 1), None,
-                            (reduction, int(chunk_rows), int(ignore_index), float(label_smoothing), float(z_loss), 1.0))
-    return out.reshape(lead) if reduction == "none" else out
+    return _head_loss(hidden, weight, target.long().reshape(-1, 1), None, reduction, int(chunk_rows),
+                      int(ignore_index), float(label_smoothing), float(z_loss), 1.0)
 
 
 def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_index: torch.Tensor,
@@ -255,9 +291,7 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_inde
         raise RuntimeError(f"{name}: chunk_rows must not be negative")
     lead = hidden.shape[:-1]
     index, teacher = _check_teacher(name, lead, teacher_index, teacher_logits, temperature)
-    out = _LinearLoss.apply(_rows(hidden), _rows(weight), index, teacher,
-                            (reduction, int(chunk_rows), 0, 0.0, 0.0, float(temperature)))
-    return out.reshape(lead) if reduction == "none" else out
+    return _head_loss(hidden, weight, index, teacher, reduction, int(chunk_rows), 0, 0.0, 0.0, float(temperature))
 
 
 def distillation(logits: torch.Tensor, teacher_index: torch.Tensor, teacher_logits: torch.Tensor, *,
@@ -271,5 +305,11 @@ def distillation(logits: torch.Tensor, teacher_index: torch.Tensor, teacher_logi
                            f"{tuple(logits.shape)}")
     lead = logits.shape[:-1]
     index, teacher = _check_teacher(name, lead, teacher_index, teacher_logits, temperature)
-    out = _Distillation.apply(_rows(logits), index, teacher, reduction, float(temperature))
-    return out.reshape(lead) if reduction == "none" else out
+    rows = _rows(logits)
+    if _records(logits):
+        out = _Distillation.apply(rows, index, teacher, reduction, float(temperature))
+    else:
+        each, mean, _ = _distill_logits(rows, index, teacher, float(temperature), reduction == "mean",
+                                        reduction != "none", None, False)
+        out = each if mean is None else mean
+    return out.reshape(lead) if reduction == "none" and len(lead) != 1 else out
