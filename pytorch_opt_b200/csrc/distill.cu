@@ -13,8 +13,8 @@
 #include <climits>
 #include <cmath>
 
-#include "head_gemm.cuh"
 #include "losses.cuh"
+#include "ptx.cuh"
 
 namespace po {
 namespace {
@@ -58,6 +58,7 @@ __device__ __forceinline__ int entry_status(const DistillArgs& a, long long t, i
 
 // Rows that the mean divides by (counted ones and those with a bad index).
 __global__ void __launch_bounds__(256) count_rows_kernel(DistillArgs a) {
+  grid_launch_next();
   const int lane = threadIdx.x & 31;
   const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);
   int n = 0;
@@ -243,6 +244,7 @@ __global__ void __launch_bounds__((GRAD ? kGradThreads : kEvalThreads) + 32, GRA
   const int s1 = min(static_cast<long long>(s0) + a.seg, static_cast<long long>(a.V));
   const Segment<T> g(z, s0, s1);
   const uint4* src = reinterpret_cast<const uint4*>(g.z0);
+  grid_wait();  // (behind the counting kernel, where there is one)
   if (cs > 1) cluster_arrive_relaxed();  // this CTA runs: its shared memory may be written
 
   float m = -INFINITY, s = 0.0f;
@@ -421,7 +423,9 @@ __global__ void __launch_bounds__((GRAD ? kGradThreads : kEvalThreads) + 32, GRA
 template <int DT, bool GRAD>
 int launch_distill(const DistillArgs& a, int cs, int threads, cudaStream_t s) {
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see launch_next
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cs;
   attr[0].val.clusterDim.y = 1;
@@ -431,7 +435,7 @@ int launch_distill(const DistillArgs& a, int cs, int threads, cudaStream_t s) {
   cfg.dynamicSmemBytes = static_cast<size_t>(a.top) * 12;
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = cs > 1 ? 1 : 0;
+  cfg.numAttrs = a.mean ? 2 : 1;
   return check_cuda(cudaLaunchKernelEx(&cfg, distill_kernel<DT, GRAD>, a), "distill launch");
 }
 

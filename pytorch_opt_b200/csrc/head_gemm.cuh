@@ -26,6 +26,7 @@
 
 #include "common.cuh"
 #include "gemm_pair.cuh"
+#include "losses.cuh"
 
 namespace po {
 
@@ -78,12 +79,6 @@ __device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr) {
 }
 __device__ __forceinline__ void head_sched_release(uint64_t* sempty, int j) {
   mbar_arrive_pair(mapa_shared(smem_u32(sempty + j % kSchedSlots), 0));
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 __device__ __forceinline__ void st_global_32B(void* p, const uint32_t (&v)[8]) {
@@ -412,6 +407,8 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
   cluster_sync();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_holder;
+  grid_launch_next();
+  grid_wait();  // operands and the count come from the kernel before
   const HeadExtent X = head_extent<C>(P);
 
   if (warp == 0) {
@@ -661,7 +658,9 @@ int launch_head(const HeadParams& P, int max_tiles, cudaStream_t stream) {
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return set_error(PO_ERR_CUDA, "device ordinal out of range");
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see launch_next
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
@@ -684,6 +683,7 @@ int launch_head(const HeadParams& P, int max_tiles, cudaStream_t stream) {
     max_pairs[dev] = n;
   }
   const int pairs = max_tiles < max_pairs[dev] ? max_tiles : max_pairs[dev];
+  cfg.numAttrs = 2;
   cfg.gridDim = dim3(2 * pairs, 1, 1);
   return check_cuda(cudaLaunchKernelEx(&cfg, kern, P), "loss head launch");
 }

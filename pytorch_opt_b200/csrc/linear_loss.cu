@@ -71,6 +71,8 @@ struct Targets {
 // = the next power of two; empty entries sort last as INT_MAX, q = 0).
 __global__ void teacher_targets_kernel(Targets tg, long long V, float inv_temp, int width, int* __restrict__ status,
                                        int* __restrict__ ent, float* __restrict__ q, float* __restrict__ qlogq) {
+  grid_launch_next();
+  grid_wait();
   extern __shared__ float sm[];
   int* si = reinterpret_cast<int*>(sm);
   float* sl = sm + width;
@@ -145,6 +147,8 @@ __global__ void teacher_targets_kernel(Targets tg, long long V, float inv_temp, 
 
 // max |row_grad| into state->grad_max (1 when there is nothing to scale by).
 __global__ void grad_max_kernel(const float* __restrict__ g, long long T, CallState* st) {
+  grid_launch_next();
+  grid_wait();
   __shared__ float buf[32];
   float m = 0.0f;
   for (long long t = threadIdx.x; t < T; t += blockDim.x) m = fmaxf(m, fabsf(g[t]));
@@ -211,6 +215,8 @@ constexpr int kPackWarps = 8;
 // launch; the host keeps blocks x T / 2 reads small.
 template <int DT>
 __global__ void __launch_bounds__(32 * kPackWarps) pack_kernel(PackArgs a, int groups) {
+  grid_launch_next();
+  grid_wait();
   using T = typename ElemOf<DT>::T;
   __shared__ int buf[32];
   const long long first = static_cast<long long>(blockIdx.x) * groups * kPackWarps;
@@ -296,6 +302,8 @@ __global__ void __launch_bounds__(32 * kPackWarps) pack_kernel(PackArgs a, int g
 template <int DT>
 __global__ void __launch_bounds__(256) stage_weight_kernel(const void* w, long long w_ld, long long V, int D, int ldp,
                                                            void* out, float* lo, int vec) {
+  grid_launch_next();
+  grid_wait();
   using T = typename ElemOf<DT>::T;
   if (DT == PO_F32 && vec) {
     // A thread splits 4 values; two loads in flight.
@@ -340,7 +348,7 @@ struct FinishArgs {
   const float2* part;
   const float* zsum;
   int nparts;
-  int row0;
+  int row0, rows;
   const int* rowmap;
   const float* zpick;
   const int* ent;
@@ -359,42 +367,48 @@ struct FinishArgs {
   int row_words;
 };
 
-// One block a packed row: lse = log2 sum 2^z2 from the row's partial
+// One warp a packed row: lse = log2 sum 2^z2 from the row's partial
 // statistics, and the loss; the last block to finish sums the losses of all
 // rows in a fixed order (fp64). Rows past the counted ones are zeroed up to a
 // K block of dW, where they meet the zeros of dZ.
-__global__ void __launch_bounds__(128) finish_kernel(FinishArgs a) {
-  __shared__ float buf[32];
+constexpr int kFinishWarps = 8;
+
+__global__ void __launch_bounds__(32 * kFinishWarps) finish_kernel(FinishArgs a) {
+  grid_launch_next();
+  grid_wait();
   __shared__ double dbuf[32];
   __shared__ int s_last;
-  const int row = blockIdx.x;
-  if (a.row0 + row < a.st->count) {
+  const int lane = threadIdx.x & 31;
+  const int row = blockIdx.x * kFinishWarps + (threadIdx.x >> 5);
+  const int left = a.st->count - a.row0;
+  if (row < left && row < a.rows) {
     const float2* p = a.part + static_cast<long long>(row) * a.nparts;
     float m = -INFINITY, s = 0.0f;
-    for (int i0 = threadIdx.x; i0 < a.nparts; i0 += 4 * blockDim.x) {
-      float2 v[4];
+    for (int i0 = lane; i0 < a.nparts; i0 += 8 * 32) {  // eight loads in flight
+      float2 v[8];
+      float c = m;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = i0 + u * blockDim.x;
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * 32;
         v[u] = i < a.nparts ? p[i] : make_float2(-INFINITY, 0.0f);
+        c = fmaxf(c, v[u].x);
       }
-      const float c = fmaxf(fmaxf(v[0].x, v[1].x), fmaxf(v[2].x, v[3].x));
       if (c > m) {
         s *= ex2(m - c);
         m = c;
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < 8; ++u)
         s += v[u].x == -INFINITY ? v[u].y : v[u].y * ex2(v[u].x - m);  // an empty part holds 0, or a NaN to keep
     }
-    const float mm = block_max(m, buf);
-    s = block_sum(m == -INFINITY ? s : s * ex2(m - mm), buf);
+    const float mm = warp_max(m);
+    s = warp_sum(m == -INFINITY ? s : s * ex2(m - mm));
     const float log2s = log2f(s), lse2 = mm + log2s;
     const long long t = a.rowmap[a.row0 + row];
     float zs = 0.0f;
     if (a.zsum != nullptr) {
-      for (int i = threadIdx.x; i < a.nparts; i += blockDim.x) zs += a.zsum[static_cast<long long>(row) * a.nparts + i];
-      zs = block_sum(zs, buf);
+      for (int i = lane; i < a.nparts; i += 32) zs += a.zsum[static_cast<long long>(row) * a.nparts + i];
+      zs = warp_sum(zs);
     }
     float loss;
     if (a.q == nullptr) {
@@ -403,25 +417,23 @@ __global__ void __launch_bounds__(128) finish_kernel(FinishArgs a) {
       if (a.smoothing != 0.0f) loss += a.smoothing * (kLn2 * a.zpick[t] - zs * a.inv_vocab);
     } else {
       float c = 0.0f;
-      for (int k = threadIdx.x; k < a.top; k += blockDim.x) {
+      for (int k = lane; k < a.top; k += 32) {
         const float q = a.q[t * a.top + k];
         if (q != 0.0f) c += q * ((mm - a.zpick[t * a.top + k]) + log2s);
       }
-      c = block_sum(c, buf);
+      c = warp_sum(c);
       loss = a.temperature * a.temperature * (a.qlogq[t] + kLn2 * c);
     }
-    if (threadIdx.x == 0) {
+    if (lane == 0) {
       a.stat[row] = make_float4(mm, 1.0f / s, lse2, 0.0f);
       a.loss_rows[t] = loss;
     }
-  } else if (a.packed != nullptr) {
-    const int left = a.st->count - a.row0;
-    if (left > 0 && row < (left + kRowPad - 1) / kRowPad * kRowPad) {
-      const uint4 none = make_uint4(0, 0, 0, 0);
-      for (int i = threadIdx.x; i < a.row_words; i += blockDim.x) {
-        a.packed[static_cast<long long>(row) * a.row_words + i] = none;
-        if (a.packed_lo != nullptr) a.packed_lo[static_cast<long long>(row) * a.row_words + i] = none;
-      }
+  } else if (a.packed != nullptr && left > 0 && row < (left + kRowPad - 1) / kRowPad * kRowPad &&
+             row < (a.rows + kRowPad - 1) / kRowPad * kRowPad) {
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    for (int i = lane; i < a.row_words; i += 32) {
+      a.packed[static_cast<long long>(row) * a.row_words + i] = none;
+      if (a.packed_lo != nullptr) a.packed_lo[static_cast<long long>(row) * a.row_words + i] = none;
     }
   }
   if (a.loss == nullptr || !a.final_launch) return;
@@ -432,7 +444,13 @@ __global__ void __launch_bounds__(128) finish_kernel(FinishArgs a) {
   if (!s_last) return;
   __threadfence();
   double sum = 0.0;
-  for (long long t = threadIdx.x; t < a.T; t += blockDim.x) sum += static_cast<double>(__ldcg(a.loss_rows + t));
+  for (long long t0 = threadIdx.x; t0 < a.T; t0 += 8 * blockDim.x) {  // eight loads in flight
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = t0 + u * blockDim.x < a.T ? __ldcg(a.loss_rows + t0 + u * blockDim.x) : 0.0f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) sum += static_cast<double>(v[u]);
+  }
   sum = block_sum(sum, dbuf);
   if (threadIdx.x == 0) {
     if (a.mean) sum /= static_cast<double>(a.st->counted_mean > 0 ? a.st->counted_mean : 1);
@@ -481,6 +499,8 @@ __device__ __forceinline__ void put_dz(const RescaleArgs& a, long long off, floa
 // case. Bound by memory: 4 bytes a logit in 16-bit types.
 template <int DT>
 __global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
+  grid_launch_next();
+  grid_wait();
   const int row = blockIdx.x / nseg;
   const int seg = blockIdx.x - row * nseg;
   const int left = a.st->count - a.row0;
@@ -564,6 +584,8 @@ template <int DT>
 __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ partial, int splits, int M, long long pld,
                                                    int N, const float* alpha, const int* count, int row0, int limit_rows,
                                                    const int* rows, void* out, long long ld) {
+  grid_launch_next();
+  grid_wait();
   const int r = blockIdx.x;
   if (limit_rows && row0 + r >= *count) return;
   const float al = *alpha;
@@ -785,13 +807,9 @@ int make_plan(Plan& p, const void* weight, long long w_ld, int dtype, long long 
 int join(int dtype, const float* partial, int splits, int M, long long pld, int N, const Plan& p, int row0,
          bool limit_rows, const int* rows, void* out, long long ld, cudaStream_t s) {
   const dim3 grid(M, N > 4096 ? 4 : 1);
-  if (dtype == PO_F32)
-    join_kernel<PO_F32><<<grid, 256, 0, s>>>(partial, splits, M, pld, N, &p.st->alpha, &p.st->count, row0, limit_rows, rows, out, ld);
-  else if (dtype == PO_BF16)
-    join_kernel<PO_BF16><<<grid, 256, 0, s>>>(partial, splits, M, pld, N, &p.st->alpha, &p.st->count, row0, limit_rows, rows, out, ld);
-  else
-    join_kernel<PO_F16><<<grid, 256, 0, s>>>(partial, splits, M, pld, N, &p.st->alpha, &p.st->count, row0, limit_rows, rows, out, ld);
-  return check_cuda(cudaGetLastError(), "linear_loss join");
+  const auto kern = dtype == PO_F32 ? join_kernel<PO_F32> : dtype == PO_BF16 ? join_kernel<PO_BF16> : join_kernel<PO_F16>;
+  return launch_next(false, kern, grid, 256, 0, s, "linear_loss join", partial, splits, M, pld, N, &p.st->alpha, &p.st->count,
+                     row0, limit_rows, rows, out, ld);
 }
 
 int run_head(const Plan& p, int product, HeadParams& P, const HeadOperand& A, const HeadOperand& B, int splits,
@@ -894,16 +912,19 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
   const int T = static_cast<int>(tokens), D = static_cast<int>(dim), V = static_cast<int>(vocab);
   const Targets tg{index, index_ld, teacher, teacher_ld, teacher_dtype, static_cast<int>(top), ignore_index};
 
+  bool first = true;
   if (soft) {
     int width = 2;
     while (width < top) width <<= 1;
     const int threads = width < 64 ? 32 : (width > 256 ? 128 : width / 2);
-    teacher_targets_kernel<<<T, threads, width * 8, s>>>(tg, vocab, 1.0f / temperature, width, p.status, p.ent, p.q, p.qlogq);
-    if ((r = check_cuda(cudaGetLastError(), "linear_loss targets"))) return r;
+    if ((r = launch_next(first, teacher_targets_kernel, T, threads, width * 8, s, "linear_loss targets", tg, vocab,
+                         1.0f / temperature, width, p.status, p.ent, p.q, p.qlogq)))
+      return r;
+    first = false;
   }
   if (row_grad != nullptr) {
-    grad_max_kernel<<<1, 1024, 0, s>>>(row_grad, tokens, p.st);
-    if ((r = check_cuda(cudaGetLastError(), "linear_loss grad_max"))) return r;
+    if ((r = launch_next(first, grad_max_kernel, 1, 1024, 0, s, "linear_loss grad_max", row_grad, tokens, p.st))) return r;
+    first = false;
   }
   const float gscale = dtype == PO_F16 ? kF16Scale : 1.0f;
   PackArgs pa{};
@@ -914,17 +935,16 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
   pa.dhidden = dhidden, pa.dh_ld = dh_ld, pa.loss_rows = loss_rows, pa.st = p.st, pa.sched = p.sched;
   pa.alpha = temperature / gscale, pa.mean = mean, pa.has_row_grad = row_grad != nullptr;
   const int groups = cdiv(T, 2048 * kPackWarps), pblocks = cdiv(T, groups * kPackWarps);
-  if (dtype == PO_F32) pack_kernel<PO_F32><<<pblocks, 32 * kPackWarps, 0, s>>>(pa, groups);
-  else if (dtype == PO_BF16) pack_kernel<PO_BF16><<<pblocks, 32 * kPackWarps, 0, s>>>(pa, groups);
-  else pack_kernel<PO_F16><<<pblocks, 32 * kPackWarps, 0, s>>>(pa, groups);
-  if ((r = check_cuda(cudaGetLastError(), "linear_loss pack"))) return r;
+  const auto pack = dtype == PO_F32 ? pack_kernel<PO_F32> : dtype == PO_BF16 ? pack_kernel<PO_BF16> : pack_kernel<PO_F16>;
+  if ((r = launch_next(first, pack, pblocks, 32 * kPackWarps, 0, s, "linear_loss pack", pa, groups))) return r;
 
   const void* w = weight;
   long long wld = w_ld;
   if (p.stage_w) {
-    if (p.f32) stage_weight_kernel<PO_F32><<<8 * sms, 256, 0, s>>>(weight, w_ld, vocab, D, static_cast<int>(p.ldp), p.w, p.w_lo, dim % 4 == 0 && w_ld % 4 == 0 && reinterpret_cast<uintptr_t>(weight) % 16 == 0);
-    else stage_weight_kernel<PO_BF16><<<8 * sms, 256, 0, s>>>(weight, w_ld, vocab, D, static_cast<int>(p.ldp), p.w, nullptr, 0);
-    if ((r = check_cuda(cudaGetLastError(), "linear_loss stage"))) return r;
+    const int vec = p.f32 && dim % 4 == 0 && w_ld % 4 == 0 && reinterpret_cast<uintptr_t>(weight) % 16 == 0;
+    if ((r = launch_next(false, p.f32 ? stage_weight_kernel<PO_F32> : stage_weight_kernel<PO_BF16>, 8 * sms, 256, 0, s,
+                         "linear_loss stage", weight, w_ld, vocab, D, static_cast<int>(p.ldp), p.w, p.w_lo, vec)))
+      return r;
     w = p.w;
     wld = p.ldp;
   }
@@ -965,8 +985,10 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
       fa.packed_lo = p.f32 ? reinterpret_cast<uint4*>(p.packed_lo + hoff) : nullptr;
       fa.row_words = static_cast<int>(p.ldp * p.es / 16);
     }
-    finish_kernel<<<static_cast<int>(p.want_dw ? krows : rows), 128, 0, s>>>(fa);
-    if ((r = check_cuda(cudaGetLastError(), "linear_loss finish"))) return r;
+    fa.rows = rows;
+    if ((r = launch_next(false, finish_kernel, cdiv(p.want_dw ? krows : rows, kFinishWarps), 32 * kFinishWarps, 0, s,
+                         "linear_loss finish", fa)))
+      return r;
     if (!p.grads) continue;
 
     RescaleArgs ra{};
@@ -977,10 +999,9 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
     const int nseg = cdiv(p.e_ld, kSegment);
     const long long rblocks = krows * nseg;
     if (rblocks > INT_MAX) return set_error(PO_ERR_ARG, "linear_loss: chunk too large");
-    if (dtype == PO_F32) rescale_kernel<PO_F32><<<static_cast<int>(rblocks), 256, 0, s>>>(ra, nseg);
-    else if (dtype == PO_BF16) rescale_kernel<PO_BF16><<<static_cast<int>(rblocks), 256, 0, s>>>(ra, nseg);
-    else rescale_kernel<PO_F16><<<static_cast<int>(rblocks), 256, 0, s>>>(ra, nseg);
-    if ((r = check_cuda(cudaGetLastError(), "linear_loss rescale"))) return r;
+    const auto rescale =
+        dtype == PO_F32 ? rescale_kernel<PO_F32> : dtype == PO_BF16 ? rescale_kernel<PO_BF16> : rescale_kernel<PO_F16>;
+    if ((r = launch_next(false, rescale, static_cast<int>(rblocks), 256, 0, s, "linear_loss rescale", ra, nseg))) return r;
 
     const long long pld = round_up(dim, 256);
     if (p.want_dh) {

@@ -76,6 +76,12 @@ __device__ __forceinline__ float load_as_f32(const void* p, int dtype, long long
   return __half2float(static_cast<const __half*>(p)[i]);
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -107,6 +113,32 @@ __device__ __forceinline__ T block_sum(T v, T* buf) {
   v = warp_sum(static_cast<int>(threadIdx.x & 31) < nw ? buf[threadIdx.x & 31] : T(0));
   __syncthreads();
   return v;
+}
+
+// Launches of one call follow one another closely: each may start (blocks
+// scheduled, barriers and tensor memory set up) while the one before it drains.
+// So every kernel of a call begins with grid_wait(), which returns when all
+// earlier work is done and visible, and lets its successor start with
+// grid_launch_next().
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Launch behind the previous kernel of the same call (`first`: behind whatever
+// is on the stream, in the ordinary way).
+template <class... Params, class... Args>
+int launch_next(bool first, void (*kern)(Params...), dim3 grid, int block, size_t smem, cudaStream_t s, const char* what,
+                Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = first ? 0 : 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...), what);
 }
 
 // What a row is to the loss.
