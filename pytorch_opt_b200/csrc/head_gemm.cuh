@@ -696,6 +696,31 @@ int dispatch_head(int product, const HeadParams& P, int max_tiles, cudaStream_t 
   if (product == HEAD_DHIDDEN) return launch_head<KIND, false, true, HEAD_STORE>(P, max_tiles, s);
   return launch_head<KIND, true, true, HEAD_STORE>(P, max_tiles, s);
 }
+
+// The logits product for up to kFewRows rows (head_few.cu): the same outputs
+// from the call's own hidden rows and weights, statistics per kFewPartCols columns.
+constexpr int kFewRows = 8;
+constexpr int kFewPartCols = 64, kPartCols = 256;
+struct FewParams {
+  const void* h;  // [row of the call][h_ld]; rows of both on 16-byte boundaries
+  long long h_ld;
+  const void* w;
+  long long w_ld;
+  int D, V;
+  const int* count;
+  const int* rowmap;
+  float scale2;
+  float2* part;
+  int nparts;
+  float* zsum;
+  void* e;
+  long long e_ld;
+  const int* ent;
+  int top;
+  float* zpick;
+};
+int launch_few_rows(const FewParams& P, int dtype, int rows, cudaStream_t s);
+
 extern template int dispatch_head<KIND_BF16>(int, const HeadParams&, int, cudaStream_t);
 extern template int dispatch_head<KIND_TF32>(int, const HeadParams&, int, cudaStream_t);
 

@@ -465,7 +465,7 @@ struct RescaleArgs {
   long long e_ld;
   long long V;
   const float2* part;
-  int nparts;
+  int nparts, part_cols;  // (64 or 256)
   const float4* stat;
   int row0, rows;
   const int* rowmap;
@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
   if (DT == PO_F32) {
 #pragma unroll 2
     for (int c = c0 + threadIdx.x * 4; c < c1; c += 256 * 4) {
-      const float m = part[c >> 8].x;
+      const float m = part[c / a.part_cols].x;
       const float f = m == -INFINITY ? (pcoef == pcoef ? 0.0f : pcoef) : pcoef * ex2(m - mm);
       const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(a.e) + base + c);
       const float x[4] = {fmaf(v.x, f, -flat), fmaf(v.y, f, -flat), fmaf(v.z, f, -flat), fmaf(v.w, f, -flat)};
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
       const int c = c0 + (i * 256 + static_cast<int>(threadIdx.x)) * 8;
       if (c < c1) {
         raw[i] = *reinterpret_cast<const uint4*>(static_cast<const __half*>(a.e) + base + c);
-        ms[i] = part[c >> 8].x;
+        ms[i] = part[c / a.part_cols].x;
       }
     }
 #pragma unroll
@@ -684,7 +684,7 @@ int choose_splits(long long tiles, int nkb, long long M, long long N) {
   const long long pairs = sm_count() / 2;
   int best = 1;
   double best_cost = 1e300;
-  for (int s = 1; s <= 32 && s <= (nkb + 3) / 4; ++s) {
+  for (int s = 1; s <= pairs && s <= (nkb + 3) / 4; ++s) {
     const double waves = static_cast<double>((tiles * s + pairs - 1) / pairs);
     double cost = waves * (static_cast<double>((nkb + s - 1) / s) + 3.0);
     if (s > 1) cost += 5.0 + static_cast<double>(s) * static_cast<double>(M) * static_cast<double>(N) * 8.0 / 3.0e6;
@@ -701,6 +701,8 @@ struct Plan {
   long long T, D, V, top;
   int dtype, es;
   bool f32, soft, grads, want_dh, want_dw;
+  bool few;           // up to kFewRows rows: logits on the CUDA cores
+  int part_cols;      // columns a partial statistic covers
   long long chunk;    // rows a pass of the products takes
   int nchunks;
   long long rows_alloc;
@@ -734,21 +736,33 @@ struct Plan {
   size_t bytes;
 };
 
+// Rows up to which the CUDA cores make the logits. A whole call without
+// gradients, CUDA cores against tensor cores, us: bf16, 50257 x 768, 1 row 25 /
+// 37, 4 rows 33 / 33, fp16 8 rows 53 / 34; bf16, 128256 x 4096, 2 rows 205 /
+// 257, 4 rows 258 / 260, 8 rows 485 / 283; fp32 (where the tensor cores need W
+// split into pairs first), 50257 x 768, 8 rows 58 / 203.
+int few_rows(int dtype) { return dtype == PO_F32 ? kFewRows : 2; }
+
 // Rows a pass keeps in the workspace by default: as many as leave 2 GiB of
 // exponentials (8191 rows of 128 thousand columns in 16 bits).
 constexpr long long kDefaultChunkBytes = 2LL << 30;
 
 int make_plan(Plan& p, const void* weight, long long w_ld, int dtype, long long T, long long D, long long V,
-              long long top, bool soft, bool want_dh, bool want_dw, long long chunk_rows, void* ws, size_t ws_bytes) {
+              long long top, bool soft, bool few, bool want_dh, bool want_dw, long long chunk_rows, void* ws,
+              size_t ws_bytes) {
   memset(&p, 0, sizeof(p));
   p.T = T, p.D = D, p.V = V, p.top = top, p.dtype = dtype, p.es = dtype_size(dtype);
   p.f32 = dtype == PO_F32;
   p.soft = soft;
   p.want_dh = want_dh, p.want_dw = want_dw, p.grads = want_dh || want_dw;
   p.ldp = round_up(D, 64);
-  p.stage_w = p.f32 || reinterpret_cast<uintptr_t>(weight) % 16 != 0 || (w_ld * p.es) % 16 != 0;
-  p.nparts = cdiv(V, 256);
+  p.few = few;
+  // The few-rows kernel takes W as it is; the tensor cores need pitches that
+  // TMA takes, and fp32 as tf32 pairs.
+  p.stage_w = (!p.few || want_dh) && (p.f32 || reinterpret_cast<uintptr_t>(weight) % 16 != 0 || (w_ld * p.es) % 16 != 0);
+  p.part_cols = p.few ? kFewPartCols : kPartCols;
   p.e_ld = round_up(V, 256);
+  p.nparts = static_cast<int>(p.e_ld / p.part_cols);
   p.bk = p.f32 ? 64 : 128;
   long long most = chunk_rows;
   if (most <= 0) {
@@ -837,8 +851,9 @@ int run_head(const Plan& p, int product, HeadParams& P, const HeadOperand& A, co
 // 2.3e-7 / 1.6e-7, 4.1e-7 / 3.1e-7, 6.9e-7 / 6.7e-7; time of the 4096 x 128256
 // x 4096 logits 4.33, 3.59, 3.38 ms before the epilogue's other steps, 3.40
 // and 3.39 ms (4, 8 blocks) after them. fp32 gradients: 5.3e-7, 6.7e-7 and
-// 1.1e-6 with 2, 4, 8 blocks (64 of K each); 16-bit ones round to 2^-9.
-constexpr int kChunkStats16 = 4, kChunkStats32 = 4, kChunkGrad16 = 16, kChunkGrad32 = 4;
+// 1.1e-6 with 2, 4, 8 blocks (64 of K each) and 2 in the logits, 9.2e-7 with 4
+// there too; 16-bit ones round to 2^-9.
+constexpr int kChunkStats16 = 4, kChunkStats32 = 2, kChunkGrad16 = 16, kChunkGrad32 = 4;
 
 bool vec32(const void* p, long long ld, int es) {
   return reinterpret_cast<uintptr_t>(p) % 32 == 0 && (ld * es) % 32 == 0;
@@ -854,13 +869,14 @@ extern "C" size_t po_linear_loss_workspace_bytes(const void* weight, long long w
                                                  int want_dweight, long long chunk_rows) {
   if (tokens <= 0 || dim <= 0 || vocab <= 0 || top <= 0 || dtype_size(dtype) == 0) return 0;
   Plan p;
-  // A teacher's rows need the larger workspace of the two kinds of targets but for zsum: size for both.
+  // Enough for both kinds of targets, and for hidden rows on any boundary.
   size_t best = 0;
-  for (int soft = 0; soft < 2; ++soft) {
-    make_plan(p, weight, w_ld, dtype, tokens, dim, vocab, top, soft != 0, want_dhidden != 0, want_dweight != 0,
-              chunk_rows, nullptr, 0);
-    if (p.bytes > best) best = p.bytes;
-  }
+  for (int soft = 0; soft < 2; ++soft)
+    for (int few = 0; few < (tokens <= few_rows(dtype) ? 2 : 1); ++few) {
+      make_plan(p, weight, w_ld, dtype, tokens, dim, vocab, top, soft != 0, few != 0, want_dhidden != 0,
+                want_dweight != 0, chunk_rows, nullptr, 0);
+      if (p.bytes > best) best = p.bytes;
+    }
   return best + 256;
 }
 
@@ -906,7 +922,11 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
   }
   if (workspace == nullptr) return set_error(PO_ERR_WORKSPACE, "linear_loss: workspace too small");
   Plan p;
-  int r = make_plan(p, weight, w_ld, dtype, tokens, dim, vocab, top, soft, dhidden != nullptr, dweight != nullptr,
+  const auto aligned = [&](const void* x, long long ld) {
+    return reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld * dtype_size(dtype) % 16 == 0;
+  };
+  const bool few = tokens <= few_rows(dtype) && aligned(hidden, h_ld) && aligned(weight, w_ld);
+  int r = make_plan(p, weight, w_ld, dtype, tokens, dim, vocab, top, soft, few, dhidden != nullptr, dweight != nullptr,
                     chunk_rows, workspace, workspace_bytes);
   if (r) return r;
   const int T = static_cast<int>(tokens), D = static_cast<int>(dim), V = static_cast<int>(vocab);
@@ -958,7 +978,14 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
     const long long krows = round_up(rows, kRowPad);
     const HeadOperand Hk{{hp, hlo}, dtype, rows, dim, p.ldp, true};
     const HeadOperand Wk{{w, p.w_lo}, dtype, vocab, dim, wld, true};
-    {
+    if (p.few) {
+      FewParams P{};
+      P.h = hidden, P.h_ld = h_ld, P.w = weight, P.w_ld = w_ld, P.D = D, P.V = V;
+      P.count = &p.st->count, P.rowmap = p.rowmap, P.scale2 = kLog2e / temperature, P.part = p.part, P.nparts = p.nparts;
+      P.zsum = smoothing != 0.0f ? p.zsum : nullptr, P.e = p.e, P.e_ld = p.e_ld, P.ent = p.ent;
+      P.top = static_cast<int>(top), P.zpick = p.zpick;
+      if ((r = launch_few_rows(P, dtype, T, s))) return r;
+    } else {
       HeadParams P;
       memset(&P, 0, sizeof(P));
       P.M = rows, P.N = V, P.K = D, P.limit = LIMIT_M, P.row0 = static_cast<int>(row0);
@@ -992,7 +1019,7 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
     if (!p.grads) continue;
 
     RescaleArgs ra{};
-    ra.e = p.e, ra.lo = p.e_lo, ra.e_ld = p.e_ld, ra.V = vocab, ra.part = p.part, ra.nparts = p.nparts, ra.stat = p.stat;
+    ra.e = p.e, ra.lo = p.e_lo, ra.e_ld = p.e_ld, ra.V = vocab, ra.part = p.part, ra.nparts = p.nparts, ra.part_cols = p.part_cols, ra.stat = p.stat;
     ra.row0 = static_cast<int>(row0), ra.rows = rows, ra.rowmap = p.rowmap, ra.ent = p.ent, ra.q = soft ? p.q : nullptr;
     ra.zpick = p.zpick, ra.top = static_cast<int>(top), ra.row_grad = row_grad, ra.smoothing = smoothing;
     ra.z_loss = z_loss, ra.inv_vocab = 1.0f / static_cast<float>(vocab), ra.scale = gscale, ra.st = p.st;
