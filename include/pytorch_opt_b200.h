@@ -312,8 +312,8 @@ int po_matmul(const void* A, long long lda, long long sa, int trans_a, const voi
  * dweight (pitch dw_ld), nullable, receive the gradients of that loss in
  * `dtype`; with row_grad (fp32 [tokens], nullable) the gradients of
  * sum_t row_grad[t] l_t instead (`mean` must be 0).
- * The logits are never stored: without gradients each tile of them leaves two
- * numbers a row; with gradients at most chunk_rows rows at a time (0: a
+ * The logits are never stored: without gradients each tile of them (256
+ * columns, 64 for a few rows) leaves two numbers a row; with gradients at most chunk_rows rows at a time (0: a
  * default by the workspace it takes) leave their scaled exponentials in the
  * workspace, in 16 bits (32 for fp32).
  * ---------------------------------------------------------------------- */
@@ -339,10 +339,11 @@ int po_distill_logits(const void* logits, long long ld, int dtype, long long tok
                       float* loss_rows, float* loss, void* dlogits, long long dl_ld, void* workspace,
                       size_t workspace_bytes, void* stream);
 
-/* x[i] <- x[i] * *factor over n elements of `dtype` (PO_F32 / PO_BF16 /
- * PO_F16), factor a device scalar; a factor of exactly 1 moves no data. The
- * chain rule of a loss whose gradients were made with it. */
-int po_scale_inplace(void* x, int dtype, long long n, const float* factor, void* stream);
+/* x[i] <- x[i] * *factor over n elements, and y (nullable) over ny, both of
+ * `dtype` (PO_F32 / PO_BF16 / PO_F16), in one launch; factor a device scalar.
+ * A factor of exactly 1 moves no data. The chain rule of a loss whose
+ * gradients were made with it. */
+int po_scale_inplace(void* x, long long n, void* y, long long ny, int dtype, const float* factor, void* stream);
 
 #ifdef __cplusplus
 }

@@ -63,7 +63,7 @@ SIGNATURES = {
     "po_distill_logits_workspace_bytes": (_sz, [_ll]),
     "po_distill_logits": (_i, [_vp, _ll, _i, _ll, _ll, _vp, _ll, _vp, _ll, _i, _ll, _f, _i, _vp, _vp, _vp, _vp, _ll,
                                _vp, _sz, _vp]),
-    "po_scale_inplace": (_i, [_vp, _i, _ll, _vp, _vp]),
+    "po_scale_inplace": (_i, [_vp, _ll, _vp, _ll, _i, _vp, _vp]),
 }
 
 _lock = threading.Lock()

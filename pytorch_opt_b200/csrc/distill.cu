@@ -413,23 +413,29 @@ int launch_distill(const DistillArgs& a, int cs, int threads, cudaStream_t s) {
 }
 
 template <int DT>
-__global__ void __launch_bounds__(256) scale_kernel(void* x, long long n, const float* factor) {
+__device__ __forceinline__ void scale_range(void* x, long long n, float f, long long first, long long step) {
   using T = typename ElemOf<DT>::T;
+  constexpr int N = DT == PO_F32 ? 4 : 8;
+  T* p = static_cast<T*>(x);
+  const long long nv = reinterpret_cast<uintptr_t>(x) % 16 == 0 ? n / N : 0;
+  for (long long i = first; i < nv; i += step) {
+    float v[N];
+    unpack16<DT>(reinterpret_cast<const uint4*>(x)[i], v);
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] *= f;
+    reinterpret_cast<uint4*>(x)[i] = pack16<DT>(v);
+  }
+  for (long long i = nv * N + first; i < n; i += step) from_f32(to_f32(p[i]) * f, p[i]);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256) scale_kernel(void* x, long long n, void* y, long long ny, const float* factor) {
   const float f = *factor;
   if (f == 1.0f) return;
-  T* p = static_cast<T*>(x);
-  constexpr int VEC = 16 / sizeof(T);
   const long long first = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
   const long long step = static_cast<long long>(gridDim.x) * blockDim.x;
-  const long long nv = reinterpret_cast<uintptr_t>(x) % 16 == 0 ? n / VEC : 0;
-  for (long long i = first; i < nv; i += step) {
-    uint4 raw = reinterpret_cast<uint4*>(x)[i];
-    T* o = reinterpret_cast<T*>(&raw);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) from_f32(to_f32(o[k]) * f, o[k]);
-    reinterpret_cast<uint4*>(x)[i] = raw;
-  }
-  for (long long i = nv * VEC + first; i < n; i += step) from_f32(to_f32(p[i]) * f, p[i]);
+  scale_range<DT>(x, n, f, first, step);
+  scale_range<DT>(y, ny, f, first, step);
 }
 
 }  // namespace
@@ -495,17 +501,18 @@ extern "C" int po_distill_logits(const void* logits, long long ld, int dtype, lo
   return g ? launch_distill<PO_F16, true>(a, cs, threads, s) : launch_distill<PO_F16, false>(a, cs, threads, s);
 }
 
-extern "C" int po_scale_inplace(void* x, int dtype, long long n, const float* factor, void* stream) {
+extern "C" int po_scale_inplace(void* x, long long n, void* y, long long ny, int dtype, const float* factor,
+                                void* stream) {
   if (dtype != PO_F32 && dtype != PO_BF16 && dtype != PO_F16)
     return set_error(PO_ERR_ARG, "scale_inplace: dtype must be fp32, bf16 or fp16");
-  if (n < 0) return set_error(PO_ERR_ARG, "scale_inplace: negative size");
-  if (n == 0) return PO_OK;
-  if (x == nullptr || factor == nullptr) return set_error(PO_ERR_ARG, "scale_inplace: null operand");
+  if (y == nullptr) ny = 0;
+  if (n < 0 || ny < 0) return set_error(PO_ERR_ARG, "scale_inplace: negative size");
+  if (n + ny == 0) return PO_OK;
+  if ((n > 0 && x == nullptr) || factor == nullptr) return set_error(PO_ERR_ARG, "scale_inplace: null operand");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const long long want = (n + 2047) / 2048;
+  const long long want = (n + ny + 2047) / 2048;
   const int blocks = static_cast<int>(want < 8LL * sm_count() ? want : 8LL * sm_count());
-  if (dtype == PO_F32) scale_kernel<PO_F32><<<blocks, 256, 0, s>>>(x, n, factor);
-  else if (dtype == PO_BF16) scale_kernel<PO_BF16><<<blocks, 256, 0, s>>>(x, n, factor);
-  else scale_kernel<PO_F16><<<blocks, 256, 0, s>>>(x, n, factor);
+  const auto kern = dtype == PO_F32 ? scale_kernel<PO_F32> : dtype == PO_BF16 ? scale_kernel<PO_BF16> : scale_kernel<PO_F16>;
+  kern<<<blocks, 256, 0, s>>>(x, n, y, ny, factor);
   return check_cuda(cudaGetLastError(), "scale_inplace");
 }

@@ -101,6 +101,22 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
 // 128 columns a thread) did not.
 constexpr int kHeadEpiWarps = 16;
 constexpr int HC = 64;  // columns of a tile one epilogue thread holds
+// The bounded waits of ptx.cuh read the clock on the first miss; most waits
+// here end within a try_wait or two (which suspend the thread by themselves).
+__device__ __forceinline__ bool head_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_bounded(bar, parity, abort_flag, err, code);
+}
+__device__ __forceinline__ bool head_wait_sleep(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
+                                                int code) {
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_bounded_sleep(bar, parity, abort_flag, err, code);
+}
+
 constexpr int kShareFloats = 3 * 128;  // a lane quarter's maxima, sums and logit sums
 constexpr int kHeadSmemExtra = 4 * kShareFloats * 4;
 constexpr int kHeadThreads = 64 + 32 * kHeadEpiWarps;
@@ -133,16 +149,20 @@ __device__ __forceinline__ HeadExtent head_extent(const HeadParams& P) {
 __device__ __forceinline__ HeadTile head_tile(const HeadParams& P, const HeadExtent& x, int t) {
   HeadTile h;
   const int per = x.tiles_m * P.tiles_n;
-  h.split = t / per;
+  h.split = P.splits > 1 ? t / per : 0;
   const int r = t - h.split * per;
-  const int b = r / (P.band * P.tiles_n);
+  const int b = x.tiles_m <= P.band ? 0 : r / (P.band * P.tiles_n);
   const int first = b * P.band;
   const int rows = min(x.tiles_m - first, P.band);
   const int in_band = r - b * P.band * P.tiles_n;
   h.mt = first + in_band % rows;
   h.nt = in_band / rows;
-  h.kb0 = static_cast<int>(static_cast<long long>(x.nkb) * h.split / P.splits);
-  h.kb1 = static_cast<int>(static_cast<long long>(x.nkb) * (h.split + 1) / P.splits);
+  h.kb0 = 0;
+  h.kb1 = x.nkb;
+  if (P.splits > 1) {
+    h.kb0 = static_cast<int>(static_cast<long long>(x.nkb) * h.split / P.splits);
+    h.kb1 = static_cast<int>(static_cast<long long>(x.nkb) * (h.split + 1) / P.splits);
+  }
   return h;
 }
 
@@ -236,19 +256,17 @@ __device__ __forceinline__ void stats_epilogue(const HeadParams& P, float (&x)[H
   bar_sync(1 + q, 128);
   const float m = fmaxf(fmaxf(share[lane], share[32 + lane]), fmaxf(share[64 + lane], share[96 + lane])) * P.scale2;
   const float off = m == -INFINITY ? 0.0f : -m;
-  float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
+  uint64_t sum2[2] = {0, 0};
+  const uint64_t scale2 = pack2(P.scale2, P.scale2), off2 = pack2(off, off);
 #pragma unroll
-  for (int j = 0; j < HC; j += 4) {
-    x[j] = ex2(fmaf(x[j], P.scale2, off));
-    x[j + 1] = ex2(fmaf(x[j + 1], P.scale2, off));
-    x[j + 2] = ex2(fmaf(x[j + 2], P.scale2, off));
-    x[j + 3] = ex2(fmaf(x[j + 3], P.scale2, off));
-    s0 += x[j];
-    s1 += x[j + 1];
-    s2 += x[j + 2];
-    s3 += x[j + 3];
+  for (int j = 0; j < HC; j += 2) {
+    const float2 a = unpack2(fma2(pack2(x[j], x[j + 1]), scale2, off2));
+    x[j] = ex2(a.x);
+    x[j + 1] = ex2(a.y);
+    sum2[(j / 2) & 1] = add2(sum2[(j / 2) & 1], pack2(x[j], x[j + 1]));
   }
-  share[128 + group * 32 + lane] = (s0 + s1) + (s2 + s3);
+  const float2 sums = unpack2(add2(sum2[0], sum2[1]));
+  share[128 + group * 32 + lane] = sums.x + sums.y;
   share[256 + group * 32 + lane] = zs;
   bar_sync(1 + q, 128);
   if (group == 0 && live) {
@@ -290,8 +308,13 @@ __device__ __forceinline__ void store_epilogue(const HeadParams& P, float (&x)[H
   }
   const bool live = row < m_rows;
   const float alpha = __ldg(P.alpha);
+  const uint64_t alpha2 = pack2(alpha, alpha);
 #pragma unroll
-  for (int j = 0; j < HC; ++j) x[j] *= alpha;
+  for (int j = 0; j < HC; j += 2) {
+    const float2 f = unpack2(mul2(pack2(x[j], x[j + 1]), alpha2));
+    x[j] = f.x;
+    x[j + 1] = f.y;
+  }
   if (P.cin != nullptr && live) {
     const float* ci = P.cin + static_cast<long long>(row) * P.cin_ld + n0;
     if (P.vec && ncols == HC) {
@@ -443,7 +466,7 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
         for (int v = 0; v < nv; ++v) {
           const int pass = v / nk;
           const int k0 = (h.kb0 + v - pass * nk) * C::BK;
-          if (!mbar_wait_bounded(empty + stage, phase ^ 1u, abort_flag, P.err, kErrTimeoutProducer)) {
+          if (!head_wait(empty + stage, phase ^ 1u, abort_flag, P.err, kErrTimeoutProducer)) {
             ok = false;
             break;
           }
@@ -529,7 +552,7 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
           const uint32_t dtmem = tmem_base + static_cast<uint32_t>(acc * BN);
           const int v1 = min(nv, v0 + P.chunk);
           for (int v = v0; v < v1; ++v) {
-            if (!mbar_wait_bounded(full + stage, phase, abort_flag, P.err, kErrTimeoutMma)) {
+            if (!head_wait(full + stage, phase, abort_flag, P.err, kErrTimeoutMma)) {
               ok = false;
               break;
             }
@@ -597,13 +620,13 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
         }
         if (lo < P.top) c = __ldg(P.ent + tk + lo) - n0;
       }
-      float x[HC];
+      uint64_t acc2[HC / 2];  // two columns a register pair
 #pragma unroll
-      for (int i = 0; i < HC; ++i) x[i] = 0.0f;
+      for (int i = 0; i < HC / 2; ++i) acc2[i] = 0;
       for (int v0 = 0; v0 < nv; v0 += P.chunk, ++ucount) {
         const int acc = ucount & 1;
         const bool ready =
-            mbar_wait_bounded_sleep(tfull + acc, (ucount >> 1) & 1u, abort_flag, P.err, kErrTimeoutEpilogue);
+            head_wait_sleep(tfull + acc, (ucount >> 1) & 1u, abort_flag, P.err, kErrTimeoutEpilogue);
         if (!__all_sync(0xffffffffu, ready)) {
           ok = false;
           break;
@@ -615,13 +638,21 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
           tmem_ld_32x16(tcol + static_cast<uint32_t>(acc * BN + i * 16), r);
           tmem_ld_wait();
 #pragma unroll
-          for (int k = 0; k < 16; ++k) x[16 * i + k] += __uint_as_float(r[k]);
+          for (int k = 0; k < 8; ++k)
+            acc2[8 * i + k] = add2(acc2[8 * i + k], pack2(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1])));
         }
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive_pair(mapa_shared(smem_u32(tempty + acc), 0));
       }
       if (!ok) break;
+      float x[HC];
+#pragma unroll
+      for (int i = 0; i < HC / 2; ++i) {
+        const float2 f = unpack2(acc2[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
       if (EPI == HEAD_STATS) {
         stats_epilogue<KIND == KIND_TF32>(P, x, live, row, n0, h.nt, tk, lo, c, share, group, q, lane, X.m);
         __syncwarp();

@@ -71,23 +71,27 @@ def _pitch(x: torch.Tensor) -> int:
 @functools.lru_cache(maxsize=512)
 def _workspace_bytes(aligned: bool, *args) -> int:
     # Of the weight's address the workspace depends only on whether TMA takes it.
-    return _lib.load().po_linear_loss_workspace_bytes(16 if aligned else 2, *args)
+    return (_lib.load().po_linear_loss_workspace_bytes(16 if aligned else 2, *args) + 15) // 16 * 16
 
 
 def _linear_loss(hidden, weight, index, teacher, ignore_index, smoothing, z_loss, temperature, mean, scalar, row_grad,
                  want_dh, want_dw, chunk_rows):
-    """One call of po_linear_loss: (per-row losses, scalar loss, dhidden, dweight)."""
+    """One call of po_linear_loss: (per-row losses or None, scalar loss or None, dhidden, dweight)."""
     tokens, dim = hidden.shape
     vocab, top = weight.shape[0], index.shape[1]
     dev, dtype = hidden.device, hidden.dtype
     code, w_ptr, w_ld = _lib.DTYPE_CODE[dtype], weight.data_ptr(), _pitch(weight)
     with _lib.on_device(dev):
-        losses = torch.empty(tokens, dtype=torch.float32, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev) if scalar else None
-        dh = torch.empty((tokens, dim), dtype=dtype, device=dev) if want_dh else None
-        dw = torch.empty((vocab, dim), dtype=dtype, device=dev) if want_dw else None
         nbytes = _workspace_bytes(w_ptr % 16 == 0, w_ld, code, tokens, dim, vocab, top, want_dh, want_dw, chunk_rows)
-        ws = _lib.workspace(nbytes, dev)
+        if scalar:  # the per-row losses are the call's own: 4 bytes a row at the end of its workspace
+            loss = torch.empty((), dtype=torch.float32, device=dev)
+            ws = _lib.workspace(nbytes + 4 * tokens, dev)
+            losses, rows_ptr = None, ws.data_ptr() + nbytes
+        else:
+            loss, losses = None, torch.empty(tokens, dtype=torch.float32, device=dev)
+            ws, rows_ptr = _lib.workspace(nbytes, dev), losses.data_ptr()
+        dh = hidden.new_empty((tokens, dim)) if want_dh else None
+        dw = weight.new_empty((vocab, dim)) if want_dw else None
         if teacher is None:
             t_ptr, t_ld, t_code = None, 0, 0
         else:
@@ -95,7 +99,7 @@ def _linear_loss(hidden, weight, index, teacher, ignore_index, smoothing, z_loss
         status = _lib.load().po_linear_loss(
             hidden.data_ptr(), _pitch(hidden), w_ptr, w_ld, code, tokens, dim, vocab, index.data_ptr(), _pitch(index),
             t_ptr, t_ld, t_code, top, ignore_index, smoothing, z_loss, temperature, mean,
-            None if row_grad is None else row_grad.data_ptr(), losses.data_ptr(), loss.data_ptr() if scalar else None,
+            None if row_grad is None else row_grad.data_ptr(), rows_ptr, loss.data_ptr() if scalar else None,
             dh.data_ptr() if want_dh else None, dim, dw.data_ptr() if want_dw else None, dim, chunk_rows,
             ws.data_ptr(), nbytes, _lib.stream_ptr(dev))
         if status:
@@ -104,23 +108,25 @@ def _linear_loss(hidden, weight, index, teacher, ignore_index, smoothing, z_loss
 
 
 def _distill_logits(logits, index, teacher, temperature, mean, scalar, row_grad, want_grad):
-    """One call of po_distill_logits: (per-row losses, scalar loss, dlogits)."""
+    """One call of po_distill_logits: (per-row losses or None, scalar loss or None, dlogits)."""
     tokens, vocab = logits.shape
     dev, dtype = logits.device, logits.dtype
     with _lib.on_device(dev):
         lib = _lib.load()
-        losses = torch.empty(tokens, dtype=torch.float32, device=dev)
-        dz = torch.empty((tokens, vocab), dtype=dtype, device=dev) if want_grad else None
-        loss = ws = None
-        nbytes = 0
+        dz = logits.new_empty((tokens, vocab)) if want_grad else None
         if scalar:
-            loss = torch.empty((), dtype=torch.float32, device=dev)
-            nbytes = lib.po_distill_logits_workspace_bytes(tokens)
-            ws = _lib.workspace(nbytes, dev)
+            nbytes = (lib.po_distill_logits_workspace_bytes(tokens) + 15) // 16 * 16
+            loss, losses = torch.empty((), dtype=torch.float32, device=dev), None
+            ws = _lib.workspace(nbytes + 4 * tokens, dev)
+            rows_ptr = ws.data_ptr() + nbytes
+        else:
+            nbytes, ws, loss = 0, None, None
+            losses = torch.empty(tokens, dtype=torch.float32, device=dev)
+            rows_ptr = losses.data_ptr()
         status = lib.po_distill_logits(
             logits.data_ptr(), _pitch(logits), _lib.DTYPE_CODE[dtype], tokens, vocab, index.data_ptr(), _pitch(index),
             teacher.data_ptr(), _pitch(teacher), _lib.DTYPE_CODE[teacher.dtype], index.shape[1], temperature, mean,
-            None if row_grad is None else row_grad.data_ptr(), losses.data_ptr(), loss.data_ptr() if scalar else None,
+            None if row_grad is None else row_grad.data_ptr(), rows_ptr, loss.data_ptr() if scalar else None,
             dz.data_ptr() if want_grad else None, vocab, ws.data_ptr() if scalar else None, nbytes,
             _lib.stream_ptr(dev))
         if status:
@@ -134,12 +140,15 @@ def _upstream(up: torch.Tensor) -> torch.Tensor:
 
 def _scale(factor: torch.Tensor, *grads) -> None:
     """Gradients times a device scalar, in place; a factor of 1 (``loss.backward()``) moves no data."""
+    have = [g for g in grads if g is not None]
+    if not have:
+        return
+    x, y = have[0], have[1] if len(have) > 1 else None
     dev = factor.device
     with _lib.on_device(dev):
-        for g in grads:
-            if g is not None:
-                _lib.check(_lib.load().po_scale_inplace(g.data_ptr(), _lib.DTYPE_CODE[g.dtype], g.numel(),
-                                                        factor.data_ptr(), _lib.stream_ptr(dev)), "po_scale_inplace")
+        _lib.check(_lib.load().po_scale_inplace(x.data_ptr(), x.numel(), None if y is None else y.data_ptr(),
+                                                0 if y is None else y.numel(), _lib.DTYPE_CODE[x.dtype],
+                                                factor.data_ptr(), _lib.stream_ptr(dev)), "po_scale_inplace")
 
 
 def _records(*tensors) -> bool:
@@ -163,8 +172,11 @@ class _LinearLoss(torch.autograd.Function):
         return losses
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, up):
+        return _LinearLoss._once(ctx, up) if torch.is_grad_enabled() else _LinearLoss._backward(ctx, up)
+
+    @staticmethod
+    def _backward(ctx, up):
         reduction, chunk_rows, *terms = ctx.opts
         up = _upstream(up)
         if reduction != "none":
@@ -177,6 +189,8 @@ class _LinearLoss(torch.autograd.Function):
         _, _, dh, dw = _linear_loss(hidden, weight, index, teacher, *terms, False, False, up, *ctx.needs_input_grad[:2],
                                     chunk_rows)
         return dh, dw, None, None, None
+
+    _once = staticmethod(torch.autograd.function.once_differentiable(_backward))  # under create_graph
 
 
 class _Distillation(torch.autograd.Function):
@@ -193,8 +207,11 @@ class _Distillation(torch.autograd.Function):
         return losses
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, up):
+        return _Distillation._once(ctx, up) if torch.is_grad_enabled() else _Distillation._backward(ctx, up)
+
+    @staticmethod
+    def _backward(ctx, up):
         up = _upstream(up)
         if ctx.scalar:
             if ctx.grad is None:
@@ -204,6 +221,8 @@ class _Distillation(torch.autograd.Function):
             return dz, None, None, None, None
         logits, index, teacher = ctx.saved_tensors
         return _distill_logits(logits, index, teacher, ctx.temperature, False, False, up, True)[2], None, None, None, None
+
+    _once = staticmethod(torch.autograd.function.once_differentiable(_backward))  # under create_graph
 
 
 def _head_loss(hidden, weight, index, teacher, reduction, chunk_rows, *terms):

@@ -301,6 +301,22 @@ def test_linear_cross_entropy_backward_runs_once_per_loss():
         loss.backward()
 
 
+def test_losses_differentiate_once():
+    """A graph of the gradient may be asked for; going through it a second time is refused."""
+    h, w, y = _head(20, 64, 300, torch.float32, seed=14)
+    index, teacher = y[:, None], torch.zeros(20, 1, device="cuda")
+    for reduction in ("mean", "none"):
+        for call in (lambda a: losses.linear_cross_entropy(a, w, y, reduction=reduction),
+                     lambda a: losses.distillation(a, index, teacher, reduction=reduction)):
+            a = h.clone().requires_grad_()
+            loss = call(a).sum()
+            g, = torch.autograd.grad(loss, a, create_graph=True)
+            b = h.clone().requires_grad_()
+            assert torch.equal(g.detach(), torch.autograd.grad(call(b).sum(), b)[0])
+            with pytest.raises(RuntimeError):
+                g.sum().backward()
+
+
 @pytest.mark.parametrize("fn", ["ce", "distil"])
 def test_gradient_agrees_with_differences(fn):
     """(l(h + e d) - l(h - e d)) / 2e along random directions, fp32: e = 2^-6 leaves a term of e^2 |d|^3 of third
@@ -616,19 +632,19 @@ def test_distillation_empty():
 
 def test_scale_of_gradients_is_skipped_for_one():
     x = torch.randn(1001, device="cuda")
+    lib = _lib.load()
     for dt in DTYPES.values():
-        for off in (0, 1):
-            v = x.to(dt)[off:].clone() if off == 0 else x.to(dt)[off:]
-            want = (v.float() * 0.3).to(dt)
-            lib = _lib.load()
-            f = torch.tensor(0.3, device="cuda")
-            _lib.check(lib.po_scale_inplace(v.data_ptr(), _lib.DTYPE_CODE[dt], v.numel(), f.data_ptr(),
-                                            _lib.stream_ptr(v.device)), "scale")
-            assert torch.equal(v, want)
-            f.fill_(1.0)
-            _lib.check(lib.po_scale_inplace(v.data_ptr(), _lib.DTYPE_CODE[dt], v.numel(), f.data_ptr(),
-                                            _lib.stream_ptr(v.device)), "scale")
-            assert torch.equal(v, want)
+        for off in (0, 1):  # on a 16-byte boundary, and not
+            v, u = x.to(dt).clone()[off:], x.to(dt).clone()[off:off + 77]
+            for a, b in ((v, u), (u, None)):
+                for f in (0.3, 1.0):
+                    factor = torch.tensor(f, device="cuda")
+                    want = [(t.float() * f).to(dt) for t in (a, b) if t is not None]
+                    _lib.check(lib.po_scale_inplace(a.data_ptr(), a.numel(), None if b is None else b.data_ptr(),
+                                                    0 if b is None else b.numel(), _lib.DTYPE_CODE[dt],
+                                                    factor.data_ptr(), _lib.stream_ptr(a.device)), "scale")
+                    assert torch.equal(a, want[0])
+                    assert b is None or torch.equal(b, want[1])
 
 
 def test_example_trains_and_distills():

@@ -77,10 +77,12 @@ def test_distill_abi_refuses(bad, word):
 
 def test_scale_abi_refuses():
     lib = _lib.load()
-    assert lib.po_scale_inplace(P, F64, 4, P, None) == 1
-    assert lib.po_scale_inplace(P, F32, -4, P, None) == 1
-    assert lib.po_scale_inplace(None, F32, 4, P, None) == 1
-    assert lib.po_scale_inplace(None, F32, 0, None, None) == 0
+    assert lib.po_scale_inplace(P, 4, None, 0, F64, P, None) == 1
+    assert lib.po_scale_inplace(P, -4, None, 0, F32, P, None) == 1
+    assert lib.po_scale_inplace(P, 4, P, -4, F32, P, None) == 1
+    assert lib.po_scale_inplace(None, 4, None, 0, F32, P, None) == 1
+    assert lib.po_scale_inplace(P, 4, None, 0, F32, None, None) == 1
+    assert lib.po_scale_inplace(None, 0, None, 0, F32, None, None) == 0
 
 
 def test_workspace_follows_what_is_asked():
