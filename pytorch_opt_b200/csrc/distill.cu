@@ -120,16 +120,16 @@ __device__ __forceinline__ void online_add(const uint4& raw, float scale2, float
     s *= ex2((m - c) * scale2);
     m = c;
   }
-  // The scaled maximum is rounded once and every exponential sees the same
-  // rounding: at most 2^-24 of m scale2, the size of the logits' own.
-  const float off = m == -INFINITY ? 0.0f : -m * scale2;
+  // The maximum is subtracted before the scaling: exact where it matters, and a
+  // row of the type's lowest value does not overflow.
+  const float off = m == -INFINITY ? 0.0f : -m;
   const uint64_t off2 = pack2(off, off), sc2 = pack2(scale2, scale2);
   float x[N];
   unpack16<DT>(raw, x);
   uint64_t add = 0;
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
-    const float2 e = unpack2(fma2(pack2(x[i], x[i + 1]), sc2, off2));
+    const float2 e = unpack2(mul2(add2(pack2(x[i], x[i + 1]), off2), sc2));
     add = add2(add, pack2(ex2(e.x), ex2(e.y)));
   }
   const float2 a = unpack2(add);
@@ -328,14 +328,14 @@ __global__ void __launch_bounds__((GRAD ? kGradThreads : kEvalThreads) + 32, GRA
       if (a.mean) w /= static_cast<float>(a.st->count);
       if (a.row_grad != nullptr) w *= a.row_grad[t];
     }
-    const float ws = w / s, off = -m * scale2;
+    const float ws = w / s;
     const auto grad = [&](const uint4& raw) {
-      const uint64_t off2 = pack2(off, off), sc2 = pack2(scale2, scale2), w2 = pack2(ws, ws);
+      const uint64_t off2 = pack2(-m, -m), sc2 = pack2(scale2, scale2), w2 = pack2(ws, ws);
       float x[VEC];
       unpack16<DT>(raw, x);
 #pragma unroll
       for (int i = 0; i < VEC; i += 2) {
-        const float2 e = unpack2(fma2(pack2(x[i], x[i + 1]), sc2, off2));
+        const float2 e = unpack2(mul2(add2(pack2(x[i], x[i + 1]), off2), sc2));
         const float2 p = unpack2(mul2(pack2(ex2(e.x), ex2(e.y)), w2));
         x[i] = p.x;
         x[i + 1] = p.y;
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__((GRAD ? kGradThreads : kEvalThreads) + 32, GRA
           first = first && j >= k;
           goal += sq[j];
         }
-        if (first) from_f32(ws * ex2(fmaf(sz[k], scale2, off)) - w * goal, out[c]);
+        if (first) from_f32(ws * ex2((sz[k] - m) * scale2) - w * goal, out[c]);
       }
     }
   }

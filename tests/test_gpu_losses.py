@@ -86,6 +86,8 @@ def ref_distill(z, index, teacher, a, up=None):
     logq = t - torch.logsumexp(t, 1, keepdim=True)
     q = torch.where(counts[:, None], logq.exp(), 0.0)
     z = torch.where(counts[:, None], z.double(), 0.0)
+    top = z.amax(1, keepdim=True)
+    z = torch.where(top > -math.inf, z - top, z)  # as above: a row of the lowest value, 64 bits or not
     logp = (z / a) - torch.logsumexp(z / a, 1, keepdim=True)
     at = index.clamp(min=0)
     each = torch.where(q > 0, q * (logq - logp.gather(1, at)), 0.0)
@@ -552,6 +554,28 @@ def test_distillation_masked_vocabulary():
     assert _rel(grad, dz) <= 2.0**-16
     x = torch.full((1, V), -math.inf, device="cuda")  # nothing to put mass on
     assert math.isnan(float(losses.distillation(x, index[:1], teacher[:1], reduction="none")))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("temperature", [1.0, 0.5, 4.0])
+def test_distillation_masked_by_the_lowest_value(dtype, temperature):
+    """Logits masked by the type's lowest finite value: probability 0 beside others, equal shares alone."""
+    dt = DTYPES[dtype]
+    T, V = 4, 300
+    z = torch.randn(T, V, generator=_gen(31), device="cuda").to(dt)
+    low = torch.finfo(dt).min
+    z[0, 5:] = low
+    z[1] = low
+    z[2, ::2] = low
+    index = torch.tensor([[0, 3], [7, 299], [1, 3], [0, 1]], device="cuda")
+    teacher = torch.tensor([[0.0, 1.0]] * T, device="cuda")
+    want, dz, _ = ref_distill(z, index, teacher, temperature)
+    x = z.clone().requires_grad_()
+    rows = losses.distillation(x, index, teacher, temperature=temperature, reduction="none")
+    assert ((rows - want).abs() <= max(1.0, temperature**2) * 2.0**-17).all()
+    grad, = _grads(rows, x, up=torch.ones_like(rows))
+    assert torch.isfinite(grad).all()
+    assert _rel(grad, dz) <= {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-10, torch.float32: 2.0**-17}[dt]
 
 
 def test_distillation_bad_index_is_loud_and_contained():
