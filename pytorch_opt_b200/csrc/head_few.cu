@@ -6,7 +6,9 @@
 // the multiplications, and its ring and accumulators take longer to fill than
 // the tile to compute. Sums are plain fp32 FMA chains over D / 16 terms and
 // three shuffles, so a single token's loss carries no accumulator truncation.
-// Bound by memory: 50257 x 768 bf16 for one row 15.2 us, 5.1 TB/s.
+// Bound by memory: 50257 x 768 bf16 for one row 15.2 us, 5.1 TB/s. (Eight fp32
+// rows are bound by their loads of H and the FMAs: 32000 x 4096 in 170 us, 3.1
+// TB/s, with registers held to 128 for four blocks on an SM; 410 us without.)
 //
 // A block takes 64 rows of W: a warp 16, in four groups of 8 lanes; a lane
 // holds 4 of its group's rows in registers while it walks T rows of H (in L1),
@@ -38,10 +40,13 @@ __device__ __forceinline__ void load_pairs(const typename ElemOf<DT>::T* p, int 
 }
 
 template <int DT, int TT>
-__global__ void __launch_bounds__(kFewThreads) few_rows_kernel(FewParams P) {
+__global__ void __launch_bounds__(kFewThreads, TT == 8 ? 4 : 0) few_rows_kernel(FewParams P) {
   using T = typename ElemOf<DT>::T;
   constexpr int VEC = DT == PO_F32 ? 4 : 8;
   __shared__ float s_z[TT][kFewCols];
+  __shared__ double dbuf[32];
+  __shared__ int s_last;
+  const FinishArgs& F = P.finish;
   grid_launch_next();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane & 7;
@@ -51,12 +56,11 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(FewParams P) {
 #pragma unroll
   for (int i = 0; i < R; ++i)
     w[i] = static_cast<const T*>(P.w) + static_cast<long long>(min(r0 + i, P.V - 1)) * P.w_ld;  // (repeats the last row)
-  grid_wait();
-  const int count = min(TT, __ldg(P.count));
+  // The products need the call's own inputs alone, so they run beside the
+  // launches before; which rows count is asked for afterwards.
   const T* h[TT];
 #pragma unroll
-  for (int t = 0; t < TT; ++t)
-    h[t] = static_cast<const T*>(P.h) + (t < count ? static_cast<long long>(__ldg(P.rowmap + t)) * P.h_ld : 0);
+  for (int t = 0; t < TT; ++t) h[t] = static_cast<const T*>(P.h) + (t < F.T ? t * P.h_ld : 0);
   // Even and odd terms of each sum in the halves of a register pair.
   uint64_t acc[R][TT];
 #pragma unroll
@@ -77,12 +81,10 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(FewParams P) {
         for (int e = 0; e < VEC / 2; ++e) acc[i][t] = fma2(x[i][e], y[e], acc[i][t]);
     }
   };
-  if (count > 0) {
-    int d = sub * VEC;
-#pragma unroll 2
-    for (; d + VEC <= P.D; d += 8 * VEC) step(d, VEC);
-    if (d < P.D) step(d, P.D - d);
-  }
+  int d = sub * VEC;
+#pragma unroll (TT == 8 ? 1 : 2)
+  for (; d + VEC <= P.D; d += 8 * VEC) step(d, VEC);
+  if (d < P.D) step(d, P.D - d);
 #pragma unroll
   for (int i = 0; i < R; ++i)
 #pragma unroll
@@ -94,32 +96,49 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(FewParams P) {
       v += __shfl_xor_sync(0xffffffffu, v, 1);
       if (sub == 0) s_z[t][warp * 16 + (lane >> 3) * R + i] = v;
     }
+  grid_wait();
   __syncthreads();
-  // A warp a row, two columns a lane.
-  for (int t = warp; t < count; t += kFewThreads / 32) {
-    const int c = 2 * lane;
+  const int count = F.st->count;
+  // A warp a counted row, two columns a lane.
+  for (int r = warp; r < count; r += kFewThreads / 32) {
+    const int c = 2 * lane, t = F.rowmap[r];
     const float z0 = n0 + c < P.V ? s_z[t][c] : -INFINITY, z1 = n0 + c + 1 < P.V ? s_z[t][c + 1] : -INFINITY;
     const float m = warp_max(fmaxf(z0, z1)) * P.scale2;
     const float off = m == -INFINITY ? 0.0f : -m;
     const float e0 = ex2(fmaf(z0, P.scale2, off)), e1 = ex2(fmaf(z1, P.scale2, off));
     const float s = warp_sum(e0 + e1);
-    const long long at = static_cast<long long>(t) * P.nparts + blockIdx.x;
+    const long long at = static_cast<long long>(r) * F.nparts + blockIdx.x;
     if (lane == 0) P.part[at] = make_float2(m, s);
     if (P.zsum != nullptr) {
       const float zs = warp_sum((n0 + c < P.V ? z0 : 0.0f) + (n0 + c + 1 < P.V ? z1 : 0.0f));
       if (lane == 0) P.zsum[at] = zs;
     }
     if (P.e != nullptr) {
-      const long long to = static_cast<long long>(t) * P.e_ld + n0 + c;  // e_ld: a multiple of 256
+      const long long to = static_cast<long long>(r) * P.e_ld + n0 + c;  // e_ld: a multiple of 256
       if (DT == PO_F32) *reinterpret_cast<float2*>(static_cast<float*>(P.e) + to) = make_float2(e0, e1);
       else *reinterpret_cast<uint32_t*>(static_cast<__half*>(P.e) + to) = pack_f16x2(e0, e1);
     }
-    const long long tk = static_cast<long long>(__ldg(P.rowmap + t)) * P.top;
-    for (int k = lane; k < P.top; k += 32) {
-      const int col = __ldg(P.ent + tk + k) - n0;
+    const long long tk = static_cast<long long>(t) * F.top;
+    for (int k = lane; k < F.top; k += 32) {
+      const int col = F.ent[tk + k] - n0;
       if (col >= 0 && col < kFewCols) P.zpick[tk + k] = s_z[t][col] * P.scale2;
     }
   }
+  if (count > 0)  // the rows that complete dW's K block
+    for (int r = count + blockIdx.x * (kFewThreads / 32) + warp; r < kRowPad; r += gridDim.x * (kFewThreads / 32))
+      zero_row(F, r, lane);
+  // The last block joins the statistics of all and writes the losses.
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = atomicAdd(&F.st->done, 1) == static_cast<int>(gridDim.x) - 1;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  for (int r = warp; r < count; r += kFewThreads / 32) finish_row(F, r, lane);
+  if (F.loss == nullptr) return;
+  __threadfence();
+  __syncthreads();
+  finish_total(F, dbuf);
 }
 
 template <int DT>
@@ -127,7 +146,7 @@ int launch_few_typed(const FewParams& P, int rows, cudaStream_t s) {
   auto kern = rows == 1 ? few_rows_kernel<DT, 1> : few_rows_kernel<DT, 2>;
   if constexpr (DT == PO_F32)
     if (rows > 2) kern = rows <= 4 ? few_rows_kernel<DT, 4> : few_rows_kernel<DT, 8>;
-  return launch_next(false, kern, P.nparts, kFewThreads, 0, s, "linear_loss few rows", P);
+  return launch_next(false, kern, P.finish.nparts, kFewThreads, 0, s, "linear_loss few rows", P);
 }
 
 }  // namespace

@@ -1,0 +1,123 @@
+// From the partial statistics of the logits to losses: shared by the kernel
+// that does this for many rows and the few-rows kernel's last block.
+#pragma once
+
+#include "losses.cuh"
+
+namespace po {
+
+// Rows of packed operands are zero up to a multiple of this (a K block of the
+// 16-bit products), so that dW's last K block adds nothing.
+constexpr int kRowPad = 128;
+
+// Device-side state of a call.
+struct CallState {
+  int count;         // counted rows
+  int counted_mean;  // rows that the mean divides by
+  int done;          // blocks of the finishing launch that are through
+  float alpha;       // factor of the gradient products
+  float grad_max;    // max |row_grad|
+};
+
+struct FinishArgs {
+  const float2* part;
+  const float* zsum;
+  int nparts;
+  int row0, rows;
+  const int* rowmap;
+  const float* zpick;
+  const int* ent;
+  const float* q;      // nullable: hard targets
+  const float* qlogq;
+  int top;
+  float smoothing, z_loss, temperature, inv_vocab;
+  float4* stat;        // [row of this launch] max, 1 / sum, log2 sum 2^z2
+  float* loss_rows;
+  float* loss;         // nullable; written by the last block of the last launch
+  long long T;
+  int mean, final_launch;
+  CallState* st;
+  uint4* packed;       // 16-byte words of H's packed rows of this launch (and of their low halves, nullable)
+  uint4* packed_lo;
+  int row_words;
+};
+
+// One warp: log2 sum 2^z2 of a packed row from its partial statistics, and its
+// loss. (Loads bypass L1: other SMs wrote, perhaps in this launch.)
+__device__ __forceinline__ void finish_row(const FinishArgs& a, int row, int lane) {
+  const float2* p = a.part + static_cast<long long>(row) * a.nparts;
+  float m = -INFINITY, s = 0.0f;
+  for (int i0 = lane; i0 < a.nparts; i0 += 8 * 32) {  // eight loads in flight
+    float2 v[8];
+    float c = m;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + u * 32;
+      v[u] = i < a.nparts ? __ldcg(p + i) : make_float2(-INFINITY, 0.0f);
+      c = fmaxf(c, v[u].x);
+    }
+    if (c > m) {
+      s *= ex2(m - c);
+      m = c;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      s += v[u].x == -INFINITY ? v[u].y : v[u].y * ex2(v[u].x - m);  // an empty part holds 0, or a NaN to keep
+  }
+  const float mm = warp_max(m);
+  s = warp_sum(m == -INFINITY ? s : s * ex2(m - mm));
+  const float log2s = log2f(s), lse2 = mm + log2s;
+  const long long t = a.rowmap[a.row0 + row];
+  float zs = 0.0f;
+  if (a.zsum != nullptr) {
+    for (int i = lane; i < a.nparts; i += 32) zs += __ldcg(a.zsum + static_cast<long long>(row) * a.nparts + i);
+    zs = warp_sum(zs);
+  }
+  float loss;
+  if (a.q == nullptr) {
+    const float lse = lse2 * kLn2, zy = __ldcg(a.zpick + t);
+    loss = kLn2 * ((mm - zy) + log2s) + a.z_loss * lse * lse;
+    if (a.smoothing != 0.0f) loss += a.smoothing * (kLn2 * zy - zs * a.inv_vocab);
+  } else {
+    float c = 0.0f;
+    for (int k = lane; k < a.top; k += 32) {
+      const float q = a.q[t * a.top + k];
+      if (q != 0.0f) c += q * ((mm - __ldcg(a.zpick + t * a.top + k)) + log2s);
+    }
+    c = warp_sum(c);
+    loss = a.temperature * a.temperature * (a.qlogq[t] + kLn2 * c);
+  }
+  if (lane == 0) {
+    a.stat[row] = make_float4(mm, 1.0f / s, lse2, 0.0f);
+    a.loss_rows[t] = loss;
+  }
+}
+
+// One warp: a packed row of zeros.
+__device__ __forceinline__ void zero_row(const FinishArgs& a, int row, int lane) {
+  if (a.packed == nullptr) return;
+  const uint4 none = make_uint4(0, 0, 0, 0);
+  for (int i = lane; i < a.row_words; i += 32) {
+    a.packed[static_cast<long long>(row) * a.row_words + i] = none;
+    if (a.packed_lo != nullptr) a.packed_lo[static_cast<long long>(row) * a.row_words + i] = none;
+  }
+}
+
+// The whole block: the sum of all rows' losses in a fixed order (fp64).
+__device__ __forceinline__ void finish_total(const FinishArgs& a, double* dbuf) {
+  double sum = 0.0;
+  for (long long t0 = threadIdx.x; t0 < a.T; t0 += 8 * blockDim.x) {  // eight loads in flight
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = t0 + u * blockDim.x < a.T ? __ldcg(a.loss_rows + t0 + u * blockDim.x) : 0.0f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) sum += static_cast<double>(v[u]);
+  }
+  sum = block_sum(sum, dbuf);
+  if (threadIdx.x == 0) {
+    if (a.mean) sum /= static_cast<double>(a.st->counted_mean > 0 ? a.st->counted_mean : 1);
+    *a.loss = static_cast<float>(sum);
+  }
+}
+
+}  // namespace po

@@ -3,12 +3,13 @@
 // dW = dZ^T H.
 //
 // Mainloop as in gemm_pair.cuh (cluster of two CTAs, 256 x 256 tile, 64 KB
-// stages of two 128-byte K atoms, dynamic tile queue), with three differences:
+// stages, dynamic tile queue), with four differences:
 //  * The extent that counts rows of H is read on the device (rows that count
 //    for nothing are packed away before, and their number never reaches the
 //    host), so tiles beyond it are not computed.
 //  * K may be split over tiles (few rows of H, a long vocabulary): each split
 //    stores its fp32 partial tile, a later kernel joins them in order.
+//  * fp32 operands are read once for their three products (HeadCfg).
 //  * The accumulator is drained into registers every `chunk` K blocks and
 //    summed there (fp32, round to nearest): the tensor core's own accumulator
 //    truncates, by -1.1e-5 of the sum at K = 4096, which the loss (a difference
@@ -26,9 +27,35 @@
 
 #include "common.cuh"
 #include "gemm_pair.cuh"
+#include "head_finish.cuh"
 #include "losses.cuh"
 
 namespace po {
+
+// A stage of the ring (64 KB a CTA, three of them): 16-bit operands, two
+// 128-byte atoms of K of A and of B; fp32 operands, one atom of each one's high
+// and low halves, from which the three products hi*hi, hi*lo and lo*hi are
+// issued: operands are read from L2 once, where a pass over K for each product
+// would read the high halves twice (L2 at about 10 TB/s is what bounds these
+// tiles: 500 x 50257 x 768 175 us a product in three passes).
+template <int KIND>
+struct HeadCfg {
+  static constexpr int TM = 256;  // rows of a pair's tile
+  static constexpr int BN = 256;  // columns
+  static constexpr int ES = KIND == KIND_BF16 ? 2 : 4;
+  static constexpr int HALVES = KIND == KIND_BF16 ? 1 : 2;
+  static constexpr int ATOMS = KIND == KIND_BF16 ? 2 : 1;
+  static constexpr int AK = 128 / ES;       // K elements an atom
+  static constexpr int BK = ATOMS * AK;     // a stage
+  static constexpr int PART = 128 * 128 * ATOMS;  // bytes: 128 rows of one half of one operand
+  static constexpr int A_BYTES = HALVES * PART;
+  static constexpr int STAGE_BYTES = 2 * A_BYTES;
+  static constexpr int STAGES = 3;
+  static constexpr int MMA_K = KIND == KIND_BF16 ? 16 : 8;
+  static constexpr int KSTEPS = BK / MMA_K;
+  static constexpr uint32_t TMEM_COLS = 2 * BN;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 512;
+};
 
 enum HeadEpi : int { HEAD_STATS = 0, HEAD_STORE = 1 };
 enum HeadLimit : int { LIMIT_M = 0, LIMIT_K = 1 };  // which extent `count` bounds
@@ -41,7 +68,6 @@ struct alignas(64) HeadParams {
   const int* count;  // device: counted rows of the whole call
   int row0;          // first packed row of this launch
   int tiles_n, splits, band;
-  int npass;         // 1, or 3: hi*hi, hi*lo, lo*hi
   int chunk;         // K blocks summed inside the accumulator
   uint32_t fmt;      // operand format of the instruction descriptor
   unsigned int* sched;
@@ -378,7 +404,7 @@ __device__ __forceinline__ void store_epilogue(const HeadParams& P, float (&x)[H
 // ---------------------------------------------------------------- kernel
 template <int KIND, bool A_MN, bool B_MN, int EPI>
 __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid_constant__ HeadParams P) {
-  using C = PairCfg<KIND, 2>;
+  using C = HeadCfg<KIND>;
   constexpr int BN = C::BN;
 
   extern __shared__ uint8_t smem_raw[];
@@ -459,13 +485,10 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
         }
         if (t >= X.total) break;
         const HeadTile h = head_tile(P, X, t);
-        const int nk = h.kb1 - h.kb0;
-        const int nv = P.npass * nk;
         const int arow = h.mt * C::TM + static_cast<int>(rank) * 128;
         const int brow = h.nt * BN + static_cast<int>(rank) * (BN / 2);
-        for (int v = 0; v < nv; ++v) {
-          const int pass = v / nk;
-          const int k0 = (h.kb0 + v - pass * nk) * C::BK;
+        for (int v = h.kb0; v < h.kb1; ++v) {
+          const int k0 = v * C::BK;
           if (!head_wait(empty + stage, phase ^ 1u, abort_flag, P.err, kErrTimeoutProducer)) {
             ok = false;
             break;
@@ -475,26 +498,30 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
             armed = (armed & ~(0x101u << stage)) | (1u << stage) | (phase << (8 + stage));
           }
           const uint32_t bar = mapa_shared(smem_u32(full + stage), 0);
-          const CUtensorMap* ma = &P.mapA[pass == 2 ? 1 : 0];
-          const CUtensorMap* mb = &P.mapB[pass == 1 ? 1 : 0];
-          uint8_t* sa = tiles + stage * C::STAGE_BYTES;
-          uint8_t* sb = sa + C::A_BYTES;
-          if (!A_MN) {
 #pragma unroll
-            for (int a = 0; a < C::ATOMS; ++a) tma_load_3d_pair(sa + a * 128 * 128, ma, bar, k0 + a * C::AK, arow, 0);
-          } else {
+          for (int half = 0; half < C::HALVES; ++half) {
+            const CUtensorMap* ma = &P.mapA[half];
+            const CUtensorMap* mb = &P.mapB[half];
+            uint8_t* sa = tiles + stage * C::STAGE_BYTES + half * C::PART;
+            uint8_t* sb = sa + C::A_BYTES;
+            if (!A_MN) {
 #pragma unroll
-            for (int i = 0; i < 128 * C::ES / 128; ++i)
-              tma_load_3d_pair(sa + i * C::BK * 128, ma, bar, arow + i * (128 / C::ES), k0, 0);
-          }
-          if (!B_MN) {
+              for (int a = 0; a < C::ATOMS; ++a)
+                tma_load_3d_pair(sa + a * 128 * 128, ma, bar, k0 + a * C::AK, arow, 0);
+            } else {
 #pragma unroll
-            for (int a = 0; a < C::ATOMS; ++a)
-              tma_load_3d_pair(sb + a * (BN / 2) * 128, mb, bar, k0 + a * C::AK, brow, 0);
-          } else {
+              for (int i = 0; i < C::ES; ++i)
+                tma_load_3d_pair(sa + i * C::BK * 128, ma, bar, arow + i * (128 / C::ES), k0, 0);
+            }
+            if (!B_MN) {
 #pragma unroll
-            for (int i = 0; i < (BN / 2) * C::ES / 128; ++i)
-              tma_load_3d_pair(sb + i * C::BK * 128, mb, bar, brow + i * (128 / C::ES), k0, 0);
+              for (int a = 0; a < C::ATOMS; ++a)
+                tma_load_3d_pair(sb + a * 128 * 128, mb, bar, k0 + a * C::AK, brow, 0);
+            } else {
+#pragma unroll
+              for (int i = 0; i < C::ES; ++i)
+                tma_load_3d_pair(sb + i * C::BK * 128, mb, bar, brow + i * (128 / C::ES), k0, 0);
+            }
           }
           if (++stage == C::STAGES) {
             stage = 0;
@@ -540,7 +567,7 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
         head_sched_release(sempty, j);
         if (t >= X.total) break;
         const HeadTile h = head_tile(P, X, t);
-        const int nv = P.npass * (h.kb1 - h.kb0);
+        const int nv = h.kb1 - h.kb0;
         for (int v0 = 0; v0 < nv && ok; v0 += P.chunk, ++ucount) {
           const int acc = ucount & 1;
           if (!mbar_wait_bounded_cluster(tempty + acc, ((ucount >> 1) & 1u) ^ 1u, abort_flag, P.err,
@@ -559,15 +586,20 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
             const uint32_t sa = smem_u32(tiles + stage * C::STAGE_BYTES);
             const uint32_t sb = sa + C::A_BYTES;
 #pragma unroll
-            for (int ks = 0; ks < C::KSTEPS; ++ks) {
-              constexpr int PER = C::KSTEPS / C::ATOMS;
-              const uint32_t aoff = A_MN ? ks * A_STEP : (ks / PER) * (128 * 128) + (ks % PER) * 32;
-              const uint32_t boff = B_MN ? ks * B_STEP : (ks / PER) * ((BN / 2) * 128) + (ks % PER) * 32;
-              const uint64_t ad = make_sw128_desc(sa + aoff, A_LBO, A_SBO, A_LAY);
-              const uint64_t bd = make_sw128_desc(sb + boff, B_LBO, B_SBO, B_LAY);
-              const uint32_t accumulate = (v > v0 || ks > 0) ? 1u : 0u;
-              if (KIND == KIND_BF16) mma_f16_pair(dtmem, ad, bd, idesc, accumulate);
-              else mma_tf32_pair(dtmem, ad, bd, idesc, accumulate);
+            for (int pass = 0; pass < (C::HALVES == 2 ? 3 : 1); ++pass) {  // hi*hi, hi*lo, lo*hi
+#pragma unroll
+              for (int ks = 0; ks < C::KSTEPS; ++ks) {
+                constexpr int PER = C::KSTEPS / C::ATOMS;
+                const uint32_t aoff = (pass == 2 ? C::PART : 0) +
+                                      (A_MN ? ks * A_STEP : (ks / PER) * (128 * 128) + (ks % PER) * 32);
+                const uint32_t boff = (pass == 1 ? C::PART : 0) +
+                                      (B_MN ? ks * B_STEP : (ks / PER) * (128 * 128) + (ks % PER) * 32);
+                const uint64_t ad = make_sw128_desc(sa + aoff, A_LBO, A_SBO, A_LAY);
+                const uint64_t bd = make_sw128_desc(sb + boff, B_LBO, B_SBO, B_LAY);
+                const uint32_t accumulate = (v > v0 || pass > 0 || ks > 0) ? 1u : 0u;
+                if (KIND == KIND_BF16) mma_f16_pair(dtmem, ad, bd, idesc, accumulate);
+                else mma_tf32_pair(dtmem, ad, bd, idesc, accumulate);
+              }
             }
             mma_commit_pair_mc(empty + stage, 0x3);
             if (++stage == C::STAGES) {
@@ -603,7 +635,7 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
       if (lane == 0) head_sched_release(sempty, j);
       if (t >= X.total) break;
       const HeadTile h = head_tile(P, X, t);
-      const int nv = P.npass * (h.kb1 - h.kb0);
+      const int nv = h.kb1 - h.kb0;
       const int row = h.mt * C::TM + static_cast<int>(rank) * 128 + q * 32 + lane;
       const int n0 = h.nt * BN + group * HC;
       const bool live = row < X.m;
@@ -682,7 +714,7 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
 // The tile counts here are upper bounds: the kernel reads the real extent.
 template <int KIND, bool A_MN, bool B_MN, int EPI>
 int launch_head(const HeadParams& P, int max_tiles, cudaStream_t stream) {
-  using C = PairCfg<KIND, 2>;
+  using C = HeadCfg<KIND>;
   auto kern = head_gemm_kernel<KIND, A_MN, B_MN, EPI>;
   static int max_pairs[64] = {};
   int dev = 0;
@@ -738,17 +770,13 @@ struct FewParams {
   const void* w;
   long long w_ld;
   int D, V;
-  const int* count;
-  const int* rowmap;
   float scale2;
   float2* part;
-  int nparts;
   float* zsum;
   void* e;
   long long e_ld;
-  const int* ent;
-  int top;
   float* zpick;
+  FinishArgs finish;  // the last block finishes the rows
 };
 int launch_few_rows(const FewParams& P, int dtype, int rows, cudaStream_t s);
 

@@ -32,28 +32,17 @@
 #include <cstring>
 #include <mutex>
 
+#include "head_finish.cuh"
 #include "head_gemm.cuh"
 #include "losses.cuh"
 
 namespace po {
 namespace {
 
-// Rows of packed operands are zero up to a multiple of this (a K block of the
-// 16-bit products), so that dW's last K block adds nothing.
-constexpr int kRowPad = 128;
 // Values of the fp16 gradient operand are 2^10 of dZ / upstream: |dZ| is at
 // most 1 + 2 z_loss lse, and softmax values down to 6e-8 stay normal. bf16
 // and tf32 have fp32's range and need no factor.
 constexpr float kF16Scale = 1024.0f;
-
-// Device-side state of a call.
-struct CallState {
-  int count;         // counted rows
-  int counted_mean;  // rows that the mean divides by
-  int done;          // blocks of the finishing kernel that are through
-  float alpha;       // factor of the gradient products
-  float grad_max;    // max |row_grad|
-};
 
 struct Targets {
   const long long* index;
@@ -344,33 +333,8 @@ __global__ void __launch_bounds__(256) stage_weight_kernel(const void* w, long l
 }
 
 // ----------------------------------------------------------------- finish
-struct FinishArgs {
-  const float2* part;
-  const float* zsum;
-  int nparts;
-  int row0, rows;
-  const int* rowmap;
-  const float* zpick;
-  const int* ent;
-  const float* q;      // nullable: hard targets
-  const float* qlogq;
-  int top;
-  float smoothing, z_loss, temperature, inv_vocab;
-  float4* stat;        // [row of this launch] max, 1 / sum, log2 sum 2^z2
-  float* loss_rows;
-  float* loss;         // nullable; written by the last block of the last launch
-  long long T;
-  int mean, final_launch;
-  CallState* st;
-  uint4* packed;       // 16-byte words of H's packed rows of this launch (and of their low halves, nullable)
-  uint4* packed_lo;
-  int row_words;
-};
-
-// One warp a packed row: lse = log2 sum 2^z2 from the row's partial
-// statistics, and the loss; the last block to finish sums the losses of all
-// rows in a fixed order (fp64). Rows past the counted ones are zeroed up to a
-// K block of dW, where they meet the zeros of dZ.
+// The last block to finish sums the losses of all rows. Rows past the counted
+// ones are zeroed up to a K block of dW, where they meet the zeros of dZ.
 constexpr int kFinishWarps = 8;
 
 __global__ void __launch_bounds__(32 * kFinishWarps) finish_kernel(FinishArgs a) {
@@ -381,61 +345,9 @@ __global__ void __launch_bounds__(32 * kFinishWarps) finish_kernel(FinishArgs a)
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.x * kFinishWarps + (threadIdx.x >> 5);
   const int left = a.st->count - a.row0;
-  if (row < left && row < a.rows) {
-    const float2* p = a.part + static_cast<long long>(row) * a.nparts;
-    float m = -INFINITY, s = 0.0f;
-    for (int i0 = lane; i0 < a.nparts; i0 += 8 * 32) {  // eight loads in flight
-      float2 v[8];
-      float c = m;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int i = i0 + u * 32;
-        v[u] = i < a.nparts ? p[i] : make_float2(-INFINITY, 0.0f);
-        c = fmaxf(c, v[u].x);
-      }
-      if (c > m) {
-        s *= ex2(m - c);
-        m = c;
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        s += v[u].x == -INFINITY ? v[u].y : v[u].y * ex2(v[u].x - m);  // an empty part holds 0, or a NaN to keep
-    }
-    const float mm = warp_max(m);
-    s = warp_sum(m == -INFINITY ? s : s * ex2(m - mm));
-    const float log2s = log2f(s), lse2 = mm + log2s;
-    const long long t = a.rowmap[a.row0 + row];
-    float zs = 0.0f;
-    if (a.zsum != nullptr) {
-      for (int i = lane; i < a.nparts; i += 32) zs += a.zsum[static_cast<long long>(row) * a.nparts + i];
-      zs = warp_sum(zs);
-    }
-    float loss;
-    if (a.q == nullptr) {
-      const float lse = lse2 * kLn2;
-      loss = kLn2 * ((mm - a.zpick[t]) + log2s) + a.z_loss * lse * lse;
-      if (a.smoothing != 0.0f) loss += a.smoothing * (kLn2 * a.zpick[t] - zs * a.inv_vocab);
-    } else {
-      float c = 0.0f;
-      for (int k = lane; k < a.top; k += 32) {
-        const float q = a.q[t * a.top + k];
-        if (q != 0.0f) c += q * ((mm - a.zpick[t * a.top + k]) + log2s);
-      }
-      c = warp_sum(c);
-      loss = a.temperature * a.temperature * (a.qlogq[t] + kLn2 * c);
-    }
-    if (lane == 0) {
-      a.stat[row] = make_float4(mm, 1.0f / s, lse2, 0.0f);
-      a.loss_rows[t] = loss;
-    }
-  } else if (a.packed != nullptr && left > 0 && row < (left + kRowPad - 1) / kRowPad * kRowPad &&
-             row < (a.rows + kRowPad - 1) / kRowPad * kRowPad) {
-    const uint4 none = make_uint4(0, 0, 0, 0);
-    for (int i = lane; i < a.row_words; i += 32) {
-      a.packed[static_cast<long long>(row) * a.row_words + i] = none;
-      if (a.packed_lo != nullptr) a.packed_lo[static_cast<long long>(row) * a.row_words + i] = none;
-    }
-  }
+  if (row < left && row < a.rows) finish_row(a, row, lane);
+  else if (left > 0 && row < (left + kRowPad - 1) / kRowPad * kRowPad && row < (a.rows + kRowPad - 1) / kRowPad * kRowPad)
+    zero_row(a, row, lane);
   if (a.loss == nullptr || !a.final_launch) return;
   __threadfence();
   __syncthreads();
@@ -443,19 +355,7 @@ __global__ void __launch_bounds__(32 * kFinishWarps) finish_kernel(FinishArgs a)
   __syncthreads();
   if (!s_last) return;
   __threadfence();
-  double sum = 0.0;
-  for (long long t0 = threadIdx.x; t0 < a.T; t0 += 8 * blockDim.x) {  // eight loads in flight
-    float v[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = t0 + u * blockDim.x < a.T ? __ldcg(a.loss_rows + t0 + u * blockDim.x) : 0.0f;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) sum += static_cast<double>(v[u]);
-  }
-  sum = block_sum(sum, dbuf);
-  if (threadIdx.x == 0) {
-    if (a.mean) sum /= static_cast<double>(a.st->counted_mean > 0 ? a.st->counted_mean : 1);
-    *a.loss = static_cast<float>(sum);
-  }
+  finish_total(a, dbuf);
 }
 
 // ---------------------------------------------------------------- rescale
@@ -669,9 +569,9 @@ int encode_operand(CUtensorMap map[2], const HeadOperand& o) {
       map[i] = map[0];
       continue;
     }
-    // K-major: 128 bytes of K x 128 rows; MN-major: 128 bytes of MN x a stage's 2 w rows of K.
+    // K-major: 128 bytes of K x 128 rows; MN-major: 128 bytes of MN x a stage's rows of K.
     const int r = o.kmajor ? encode(&map[i], p, o.dtype, o.rows, o.cols, o.ld, w, 128, false)
-                           : encode(&map[i], p, o.dtype, o.rows, o.cols, o.ld, w, 2 * w, true);
+                           : encode(&map[i], p, o.dtype, o.rows, o.cols, o.ld, w, es == 4 ? w : 2 * w, true);
     if (r) return r;
   }
   return PO_OK;
@@ -740,7 +640,7 @@ struct Plan {
 // gradients, CUDA cores against tensor cores, us: bf16, 50257 x 768, 1 row 25 /
 // 37, 4 rows 33 / 33, fp16 8 rows 53 / 34; bf16, 128256 x 4096, 2 rows 205 /
 // 257, 4 rows 258 / 260, 8 rows 485 / 283; fp32 (where the tensor cores need W
-// split into pairs first), 50257 x 768, 8 rows 58 / 203.
+// split into pairs first), 50257 x 768, 8 rows 68 / 203.
 int few_rows(int dtype) { return dtype == PO_F32 ? kFewRows : 2; }
 
 // Rows a pass keeps in the workspace by default: as many as leave 2 GiB of
@@ -763,7 +663,7 @@ int make_plan(Plan& p, const void* weight, long long w_ld, int dtype, long long 
   p.part_cols = p.few ? kFewPartCols : kPartCols;
   p.e_ld = round_up(V, 256);
   p.nparts = static_cast<int>(p.e_ld / p.part_cols);
-  p.bk = p.f32 ? 64 : 128;
+  p.bk = p.f32 ? 32 : 128;
   long long most = chunk_rows;
   if (most <= 0) {
     // Without gradients a row leaves 8 bytes per 256 columns.
@@ -776,10 +676,11 @@ int make_plan(Plan& p, const void* weight, long long w_ld, int dtype, long long 
   p.chunk = p.nchunks == 1 ? T : round_up((T + p.nchunks - 1) / p.nchunks, 256);
   p.rows_alloc = round_up(T, kRowPad);
   const long long mt = (p.chunk + 255) / 256, nd = (D + 255) / 256, nv = (V + 255) / 256;
-  const int npass = p.f32 ? 3 : 1;
-  p.splits_dh = want_dh ? choose_splits(mt * nd, npass * cdiv(V, p.bk), p.chunk, D) : 1;
+  // K blocks in units of a 16-bit one's time (an fp32 block issues 1.5 times as much).
+  const auto blocks = [&](long long k) { return p.f32 ? cdiv(3LL * cdiv(k, p.bk), 2) : cdiv(k, p.bk); };
+  p.splits_dh = want_dh ? choose_splits(mt * nd, blocks(V), p.chunk, D) : 1;
   p.dw_acc = want_dw && p.nchunks > 1;
-  p.splits_dw = want_dw && !p.dw_acc ? choose_splits(nv * nd, npass * cdiv(p.chunk, p.bk), V, D) : 1;
+  p.splits_dw = want_dw && !p.dw_acc ? choose_splits(nv * nd, blocks(p.chunk), V, D) : 1;
 
   Arena ar(ws, ws_bytes);
   auto i32 = [&](long long n) { return static_cast<int*>(ar.take(static_cast<size_t>(n) * 4)); };
@@ -836,7 +737,6 @@ int run_head(const Plan& p, int product, HeadParams& P, const HeadOperand& A, co
   P.err = device_error_word();
   if (P.err == nullptr) return set_error(PO_ERR_CUDA, "device error word unavailable");
   P.fmt = p.f32 ? 2u : (p.dtype == PO_BF16 ? 1u : 0u);
-  P.npass = p.f32 ? 3 : 1;
   P.splits = splits;
   P.tiles_n = cdiv(P.N, 256);
   const int tiles_m = cdiv(P.M, 256);
@@ -850,9 +750,10 @@ int run_head(const Plan& p, int product, HeadParams& P, const HeadOperand& A, co
 // mean loss at D = 768 / 4096 with 2, 4, 8 blocks (256, 512, 1024 of K):
 // 2.3e-7 / 1.6e-7, 4.1e-7 / 3.1e-7, 6.9e-7 / 6.7e-7; time of the 4096 x 128256
 // x 4096 logits 4.33, 3.59, 3.38 ms before the epilogue's other steps, 3.40
-// and 3.39 ms (4, 8 blocks) after them. fp32 gradients: 5.3e-7, 6.7e-7 and
-// 1.1e-6 with 2, 4, 8 blocks (64 of K each) and 2 in the logits, 9.2e-7 with 4
-// there too; 16-bit ones round to 2^-9.
+// and 3.39 ms (4, 8 blocks) after them. 16-bit gradients round to 2^-9: 2048 of
+// K. fp32 (blocks of 32 of K), 500 x 50257 x 768: gradients off by 7e-7 with 2
+// and 4 blocks in logits and gradients, 1.3e-6 with 4 and 4; 2 blocks for 4 in
+// the logits cost 10 of 180 us.
 constexpr int kChunkStats16 = 4, kChunkStats32 = 2, kChunkGrad16 = 16, kChunkGrad32 = 4;
 
 bool vec32(const void* p, long long ld, int es) {
@@ -978,12 +879,24 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
     const long long krows = round_up(rows, kRowPad);
     const HeadOperand Hk{{hp, hlo}, dtype, rows, dim, p.ldp, true};
     const HeadOperand Wk{{w, p.w_lo}, dtype, vocab, dim, wld, true};
+    FinishArgs fa{};
+    fa.part = p.part, fa.zsum = smoothing != 0.0f ? p.zsum : nullptr, fa.nparts = p.nparts, fa.row0 = static_cast<int>(row0);
+    fa.rowmap = p.rowmap, fa.zpick = p.zpick, fa.ent = p.ent, fa.q = soft ? p.q : nullptr, fa.qlogq = p.qlogq;
+    fa.top = static_cast<int>(top), fa.smoothing = smoothing, fa.z_loss = z_loss, fa.temperature = temperature;
+    fa.inv_vocab = 1.0f / static_cast<float>(vocab), fa.stat = p.stat, fa.loss_rows = loss_rows, fa.loss = loss;
+    fa.T = tokens, fa.mean = mean, fa.final_launch = c == p.nchunks - 1, fa.st = p.st;
+    if (p.want_dw) {
+      fa.packed = static_cast<uint4*>(p.packed) + hoff * p.es / 16;
+      fa.packed_lo = p.f32 ? reinterpret_cast<uint4*>(p.packed_lo + hoff) : nullptr;
+      fa.row_words = static_cast<int>(p.ldp * p.es / 16);
+    }
+    fa.rows = rows;
     if (p.few) {
       FewParams P{};
       P.h = hidden, P.h_ld = h_ld, P.w = weight, P.w_ld = w_ld, P.D = D, P.V = V;
-      P.count = &p.st->count, P.rowmap = p.rowmap, P.scale2 = kLog2e / temperature, P.part = p.part, P.nparts = p.nparts;
-      P.zsum = smoothing != 0.0f ? p.zsum : nullptr, P.e = p.e, P.e_ld = p.e_ld, P.ent = p.ent;
-      P.top = static_cast<int>(top), P.zpick = p.zpick;
+      P.scale2 = kLog2e / temperature, P.part = p.part, P.zsum = smoothing != 0.0f ? p.zsum : nullptr;
+      P.e = p.e, P.e_ld = p.e_ld, P.zpick = p.zpick;
+      P.finish = fa;
       if ((r = launch_few_rows(P, dtype, T, s))) return r;
     } else {
       HeadParams P;
@@ -1001,20 +914,8 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
       P.e = p.e, P.e_ld = p.e_ld, P.rowmap = p.rowmap, P.ent = p.ent, P.top = static_cast<int>(top), P.zpick = p.zpick;
       if ((r = run_head(p, HEAD_LOGITS, P, Hk, Wk, 1, s))) return r;
     }
-    FinishArgs fa{};
-    fa.part = p.part, fa.zsum = smoothing != 0.0f ? p.zsum : nullptr, fa.nparts = p.nparts, fa.row0 = static_cast<int>(row0);
-    fa.rowmap = p.rowmap, fa.zpick = p.zpick, fa.ent = p.ent, fa.q = soft ? p.q : nullptr, fa.qlogq = p.qlogq;
-    fa.top = static_cast<int>(top), fa.smoothing = smoothing, fa.z_loss = z_loss, fa.temperature = temperature;
-    fa.inv_vocab = 1.0f / static_cast<float>(vocab), fa.stat = p.stat, fa.loss_rows = loss_rows, fa.loss = loss;
-    fa.T = tokens, fa.mean = mean, fa.final_launch = c == p.nchunks - 1, fa.st = p.st;
-    if (p.want_dw) {
-      fa.packed = static_cast<uint4*>(p.packed) + hoff * p.es / 16;
-      fa.packed_lo = p.f32 ? reinterpret_cast<uint4*>(p.packed_lo + hoff) : nullptr;
-      fa.row_words = static_cast<int>(p.ldp * p.es / 16);
-    }
-    fa.rows = rows;
-    if ((r = launch_next(false, finish_kernel, cdiv(p.want_dw ? krows : rows, kFinishWarps), 32 * kFinishWarps, 0, s,
-                         "linear_loss finish", fa)))
+    if (!p.few && (r = launch_next(false, finish_kernel, cdiv(p.want_dw ? krows : rows, kFinishWarps), 32 * kFinishWarps,
+                                   0, s, "linear_loss finish", fa)))
       return r;
     if (!p.grads) continue;
 

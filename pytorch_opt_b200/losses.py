@@ -36,15 +36,16 @@ MAX_TOP = 1024
 
 
 def _check_tensors(name: str, first, *others) -> None:
-    for t in (first, *others):
+    if not isinstance(first, torch.Tensor):
+        raise RuntimeError(f"{name}: expected a tensor, got {type(first).__name__}")
+    at = first.device
+    if at.type != "cuda":
+        raise RuntimeError("pytorch_opt_b200 runs on CUDA tensors only (there is no CPU path)")
+    for t in others:
         if not isinstance(t, torch.Tensor):
             raise RuntimeError(f"{name}: expected a tensor, got {type(t).__name__}")
-        if not t.is_cuda:
-            raise RuntimeError("pytorch_opt_b200 runs on CUDA tensors only (there is no CPU path)")
-    at = first.device
-    for t in others:
         if t.device != at:
-            raise RuntimeError("all tensors must be on the same CUDA device")
+            raise RuntimeError("pytorch_opt_b200 runs on CUDA tensors only, all on the same device")
 
 
 def _check_reduction(name: str, reduction: str) -> None:
@@ -153,7 +154,11 @@ def _scale(factor: torch.Tensor, *grads) -> None:
 
 def _records(*tensors) -> bool:
     """Whether autograd would record a function of these."""
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                return True
+    return False
 
 
 class _LinearLoss(torch.autograd.Function):
