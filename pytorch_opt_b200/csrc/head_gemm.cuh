@@ -143,7 +143,7 @@ __device__ __forceinline__ bool head_wait_sleep(uint64_t* bar, uint32_t parity, 
   return mbar_wait_bounded_sleep(bar, parity, abort_flag, err, code);
 }
 
-constexpr int kShareFloats = 3 * 128;  // a lane quarter's maxima, sums and logit sums
+constexpr int kShareFloats = 3 * 128 + 4;  // a lane quarter's maxima, sums, logit sums and flags
 constexpr int kHeadSmemExtra = 4 * kShareFloats * 4;
 constexpr int kHeadThreads = 64 + 32 * kHeadEpiWarps;
 // Readers of a slot of the tile queue: leader MMA issuer and epilogue warps, peer producer and epilogue warps.
@@ -161,7 +161,7 @@ struct HeadExtent {
 template <class C>
 __device__ __forceinline__ HeadExtent head_extent(const HeadParams& P) {
   HeadExtent x;
-  const int left = max(0, __ldg(P.count) - P.row0);
+  const int left = max(0, *P.count - P.row0);
   x.m = P.limit == LIMIT_M ? min(P.M, left) : P.M;
   const int k = P.limit == LIMIT_K ? min(P.K, left) : P.K;
   x.tiles_m = (x.m + C::TM - 1) / C::TM;
@@ -228,6 +228,16 @@ __device__ __forceinline__ void store_lines(uint32_t (&v)[32], int lane, RowPtr 
   }
 }
 
+// Whether all four warps of a lane quarter may go on: a wait that gave up in one
+// of them must not leave the others at a barrier. (The flags are read before
+// the next barrier and written after the one that follows it.)
+__device__ __forceinline__ bool quarter_agrees(int* flags, int group, int q, int lane, bool go) {
+  if (lane == 0) flags[group] = go ? 1 : 0;
+  bar_sync(1 + q, 128);
+  const volatile int* f = flags;
+  return (f[0] & f[1] & f[2] & f[3]) != 0;
+}
+
 // ------------------------------------------------------------- epilogues
 // x: accumulators of columns n0 .. n0 + HC - 1 of packed row `row` (of this launch).
 // `share`: this lane quarter's rows of shared memory, [column group][row].
@@ -248,7 +258,7 @@ __device__ __forceinline__ void stats_epilogue(const HeadParams& P, float (&x)[H
           if (c == 16 * g + j) v = x[16 * g + j];
         P.zpick[tk + lo] = v * P.scale2;
         ++lo;
-        c = lo < P.top ? __ldg(P.ent + tk + lo) - n0 : 0x7fffffff;
+        c = lo < P.top ? P.ent[tk + lo] - n0 : 0x7fffffff;
       }
     }
   }
@@ -333,7 +343,7 @@ __device__ __forceinline__ void store_epilogue(const HeadParams& P, float (&x)[H
     return;
   }
   const bool live = row < m_rows;
-  const float alpha = __ldg(P.alpha);
+  const float alpha = *P.alpha;
   const uint64_t alpha2 = pack2(alpha, alpha);
 #pragma unroll
   for (int j = 0; j < HC; j += 2) {
@@ -364,7 +374,7 @@ __device__ __forceinline__ void store_epilogue(const HeadParams& P, float (&x)[H
     char* base = static_cast<char*>(P.out) + static_cast<long long>(n0) * es;
     const auto row_ptr = [&](int r) -> char* {
       if (row_w + r >= m_rows) return nullptr;
-      const long long o = P.out_rows != nullptr ? __ldg(P.out_rows + P.row0 + row_w + r) : row_w + r;
+      const long long o = P.out_rows != nullptr ? P.out_rows[P.row0 + row_w + r] : row_w + r;
       return base + o * P.out_ld * es;
     };
     uint32_t v[32];
@@ -383,7 +393,7 @@ __device__ __forceinline__ void store_epilogue(const HeadParams& P, float (&x)[H
     return;
   }
   if (!live) return;
-  const long long orow = P.out_rows != nullptr ? __ldg(P.out_rows + P.row0 + row) : row;
+  const long long orow = P.out_rows != nullptr ? P.out_rows[P.row0 + row] : row;
   const long long base = orow * P.out_ld + n0;
   if (P.out_dtype == PO_F32) {
     float* o = static_cast<float*>(P.out) + base;
@@ -626,31 +636,31 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
     float* share = shares + q * kShareFloats;
     const uint32_t tcol = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(group * HC);
     int ucount = 0;
-    bool ok = true;
-    for (int j = 0; ok; ++j) {
-      int t;
-      const bool got = sched_read(sfull, stile, j, abort_flag, P.err, kErrTimeoutEpilogue, t);
-      if (!__all_sync(0xffffffffu, got)) break;
+    for (int j = 0;; ++j) {
+      int t = 0;
+      bool go = sched_read(sfull, stile, j, abort_flag, P.err, kErrTimeoutEpilogue, t);
+      go = __all_sync(0xffffffffu, go);
       __syncwarp();
-      if (lane == 0) head_sched_release(sempty, j);
-      if (t >= X.total) break;
-      const HeadTile h = head_tile(P, X, t);
+      if (go && lane == 0) head_sched_release(sempty, j);
+      go = go && t < X.total;
+      HeadTile h{0, 0, 0, 0, 0};
+      if (go) h = head_tile(P, X, t);
       const int nv = h.kb1 - h.kb0;
       const int row = h.mt * C::TM + static_cast<int>(rank) * 128 + q * 32 + lane;
       const int n0 = h.nt * BN + group * HC;
-      const bool live = row < X.m;
+      const bool live = go && row < X.m;
       long long tk = 0;
       int lo = 0, c = 0x7fffffff;
       if (EPI == HEAD_STATS && live) {
         // First target of this row at or after column n0.
-        tk = static_cast<long long>(__ldg(P.rowmap + P.row0 + row)) * P.top;
+        tk = static_cast<long long>(P.rowmap[P.row0 + row]) * P.top;
         int hi = P.top;
         while (lo < hi) {
           const int mid = (lo + hi) >> 1;
-          if (__ldg(P.ent + tk + mid) < n0) lo = mid + 1;
+          if (P.ent[tk + mid] < n0) lo = mid + 1;
           else hi = mid;
         }
-        if (lo < P.top) c = __ldg(P.ent + tk + lo) - n0;
+        if (lo < P.top) c = P.ent[tk + lo] - n0;
       }
       uint64_t acc2[HC / 2];  // two columns a register pair
 #pragma unroll
@@ -660,7 +670,7 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
         const bool ready =
             head_wait_sleep(tfull + acc, (ucount >> 1) & 1u, abort_flag, P.err, kErrTimeoutEpilogue);
         if (!__all_sync(0xffffffffu, ready)) {
-          ok = false;
+          go = false;
           break;
         }
         tc_fence_after_sync();
@@ -677,7 +687,9 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
         __syncwarp();
         if (lane == 0) mbar_arrive_pair(mapa_shared(smem_u32(tempty + acc), 0));
       }
-      if (!ok) break;
+      // The warps that exchange statistics go on or leave together.
+      if (EPI == HEAD_STATS) go = quarter_agrees(reinterpret_cast<int*>(share + 3 * 128), group, q, lane, go);
+      if (!go) break;
       float x[HC];
 #pragma unroll
       for (int i = 0; i < HC / 2; ++i) {

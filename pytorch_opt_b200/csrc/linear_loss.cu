@@ -58,8 +58,8 @@ struct Targets {
 // One block a row: q = softmax(teacher / a) over the entries with index >= 0,
 // sum q log q, and (index, q) sorted by index (a bitonic network over `width`
 // = the next power of two; empty entries sort last as INT_MAX, q = 0).
-__global__ void teacher_targets_kernel(Targets tg, long long V, float inv_temp, int width, int* __restrict__ status,
-                                       int* __restrict__ ent, float* __restrict__ q, float* __restrict__ qlogq) {
+__global__ void teacher_targets_kernel(Targets tg, long long V, float inv_temp, int width, int* status,
+                                       int* ent, float* q, float* qlogq) {
   grid_launch_next();
   grid_wait();
   extern __shared__ float sm[];
@@ -135,7 +135,7 @@ __global__ void teacher_targets_kernel(Targets tg, long long V, float inv_temp, 
 }
 
 // max |row_grad| into state->grad_max (1 when there is nothing to scale by).
-__global__ void grad_max_kernel(const float* __restrict__ g, long long T, CallState* st) {
+__global__ void grad_max_kernel(const float* g, long long T, CallState* st) {
   grid_launch_next();
   grid_wait();
   __shared__ float buf[32];
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
 // ------------------------------------------------------------------- join
 // out[rows[row0 + r] or r][c] = alpha sum_s partial[s][r][c], in order of s.
 template <int DT>
-__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ partial, int splits, int M, long long pld,
+__global__ void __launch_bounds__(256) join_kernel(const float* partial, int splits, int M, long long pld,
                                                    int N, const float* alpha, const int* count, int row0, int limit_rows,
                                                    const int* rows, void* out, long long ld) {
   grid_launch_next();

@@ -146,7 +146,9 @@ __device__ __forceinline__ T block_sum(T v, T* buf) {
 // scheduled, barriers and tensor memory set up) while the one before it drains.
 // So every kernel of a call begins with grid_wait(), which returns when all
 // earlier work is done and visible, and lets its successor start with
-// grid_launch_next().
+// grid_launch_next(). What an earlier launch of the call wrote is read with ordinary
+// loads: the read-only path wants data that no kernel writes while this one is
+// resident.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
