@@ -144,7 +144,9 @@ __device__ __forceinline__ bool head_wait_sleep(uint64_t* bar, uint32_t parity, 
 }
 
 constexpr int kShareFloats = 3 * 128 + 4;  // a lane quarter's maxima, sums, logit sums and flags
-constexpr int kHeadSmemExtra = 4 * kShareFloats * 4;
+constexpr int kStageWords = 256;              // a warp's eight rows on their way to unaligned ones
+constexpr int kHeadSmemExtra = kHeadEpiWarps * kStageWords * 4;  // (products that store exchange no statistics)
+static_assert(4 * kShareFloats * 4 <= kHeadSmemExtra, "shared memory");
 constexpr int kHeadThreads = 64 + 32 * kHeadEpiWarps;
 // Readers of a slot of the tile queue: leader MMA issuer and epilogue warps, peer producer and epilogue warps.
 constexpr int kHeadReaders = 2 + 2 * kHeadEpiWarps;
@@ -196,13 +198,10 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-// Stores 128 bytes of each of the warp's 32 rows. v: this thread's row, as four
-// blocks of 32 bytes. Four lanes first exchange blocks (two butterfly rounds),
-// so that each store instruction writes whole 128-byte lines of eight rows
-// instead of 32-byte pieces of 32 rows. row_ptr(r): where row r of the warp
-// goes, null where it does not.
-template <class RowPtr>
-__device__ __forceinline__ void store_lines(uint32_t (&v)[32], int lane, RowPtr row_ptr) {
+// v: 128 bytes of this thread's row, as four blocks of 32 bytes. Four lanes
+// exchange blocks (two butterfly rounds): afterwards block i is block lane % 4
+// of row 4 (lane / 4) + i of the warp.
+__device__ __forceinline__ void quad_exchange(uint32_t (&v)[32], int lane) {
 #pragma unroll
   for (int round = 0; round < 2; ++round) {
     const int x = 1 << round;
@@ -218,6 +217,14 @@ __device__ __forceinline__ void store_lines(uint32_t (&v)[32], int lane, RowPtr 
       }
     }
   }
+}
+
+// Stores 128 bytes of each of the warp's 32 rows, whole 128-byte lines of eight
+// rows an instruction instead of 32-byte pieces of 32 rows. row_ptr(r): where
+// row r of the warp goes (on a 32-byte boundary), null where it does not.
+template <class RowPtr>
+__device__ __forceinline__ void store_lines(uint32_t (&v)[32], int lane, RowPtr row_ptr) {
+  quad_exchange(v, lane);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t w[8];
@@ -225,6 +232,42 @@ __device__ __forceinline__ void store_lines(uint32_t (&v)[32], int lane, RowPtr 
     for (int k = 0; k < 8; ++k) w[k] = v[8 * i + k];
     char* at = row_ptr((lane & ~3) + i);
     if (at != nullptr) st_global_32B(at + (lane & 3) * 32, w);
+  }
+}
+
+// The same for rows on any boundary of ES bytes, of which `n` elements exist:
+// eight rows at a time through 1 KB of the warp's shared memory, then a row an
+// instruction, by words where they are aligned. (Element stores straight from
+// the registers touch a sector each: dW of 1024 x 50257 x 1001 took 460 us, and
+// takes 119 this way; 90 with 1024 features.)
+template <int ES, class RowPtr>
+__device__ __forceinline__ void store_any(uint32_t (&v)[32], int lane, uint32_t* stage, int n, bool words,
+                                          RowPtr row_ptr) {
+  quad_exchange(v, lane);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    __syncwarp();
+    uint4* to = reinterpret_cast<uint4*>(stage + (lane >> 2) * 32 + (lane & 3) * 8);
+    to[0] = make_uint4(v[8 * i], v[8 * i + 1], v[8 * i + 2], v[8 * i + 3]);
+    to[1] = make_uint4(v[8 * i + 4], v[8 * i + 5], v[8 * i + 6], v[8 * i + 7]);
+    __syncwarp();
+#pragma unroll 1
+    for (int r = 0; r < 8; ++r) {
+      char* at = row_ptr(4 * r + i);
+      if (at == nullptr) continue;
+      const uint32_t* from = stage + r * 32;
+      if (ES == 4) {
+        if (lane < n) reinterpret_cast<uint32_t*>(at)[lane] = from[lane];
+      } else if (words && 2 * lane + 1 < n) {
+        reinterpret_cast<uint32_t*>(at)[lane] = from[lane];
+      } else if (words) {
+        if (2 * lane < n) reinterpret_cast<uint16_t*>(at)[2 * lane] = static_cast<uint16_t>(from[lane]);
+      } else {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(from);
+        if (lane < n) reinterpret_cast<uint16_t*>(at)[lane] = h[lane];
+        if (lane + 32 < n) reinterpret_cast<uint16_t*>(at)[lane + 32] = h[lane + 32];
+      }
+    }
   }
 }
 
@@ -326,7 +369,7 @@ __device__ __forceinline__ void stats_epilogue(const HeadParams& P, float (&x)[H
 }
 
 __device__ __forceinline__ void store_epilogue(const HeadParams& P, float (&x)[HC], int row, int n0, int split,
-                                               int lane, int m_rows) {
+                                               int lane, int m_rows, uint32_t* stage) {
   const int ncols = min(HC, P.N - n0);
   const int row_w = row - lane;
   if (P.splits > 1) {
@@ -369,45 +412,29 @@ __device__ __forceinline__ void store_epilogue(const HeadParams& P, float (&x)[H
     }
   }
   const bool bf = P.out_dtype == PO_BF16;
-  if (P.vec && ncols == HC) {
-    const int es = P.out_dtype == PO_F32 ? 4 : 2;
-    char* base = static_cast<char*>(P.out) + static_cast<long long>(n0) * es;
-    const auto row_ptr = [&](int r) -> char* {
-      if (row_w + r >= m_rows) return nullptr;
-      const long long o = P.out_rows != nullptr ? P.out_rows[P.row0 + row_w + r] : row_w + r;
-      return base + o * P.out_ld * es;
-    };
-    uint32_t v[32];
-    if (P.out_dtype == PO_F32) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(x[i]);
-      store_lines(v, lane, row_ptr);
-      base += 128;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(x[32 + i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = bf ? pack_bf16x2(x[2 * i], x[2 * i + 1]) : pack_f16x2(x[2 * i], x[2 * i + 1]);
-    }
-    store_lines(v, lane, row_ptr);
-    return;
-  }
-  if (!live) return;
-  const long long orow = P.out_rows != nullptr ? P.out_rows[P.row0 + row] : row;
-  const long long base = orow * P.out_ld + n0;
+  const int es = P.out_dtype == PO_F32 ? 4 : 2;
+  char* base = static_cast<char*>(P.out) + static_cast<long long>(n0) * es;
+  const auto row_ptr = [&](int r) -> char* {
+    if (row_w + r >= m_rows) return nullptr;
+    const long long o = P.out_rows != nullptr ? P.out_rows[P.row0 + row_w + r] : row_w + r;
+    return base + o * P.out_ld * es;
+  };
+  const bool lines = P.vec && ncols == HC;
+  uint32_t v[32];
   if (P.out_dtype == PO_F32) {
-    float* o = static_cast<float*>(P.out) + base;
 #pragma unroll
-    for (int j = 0; j < HC; ++j)
-      if (j < ncols) o[j] = x[j];
-  } else {
-    uint16_t* o = static_cast<uint16_t*>(P.out) + base;
+    for (int part = 0; part < 2; ++part) {
 #pragma unroll
-    for (int j = 0; j < HC; j += 2) {
-      const uint32_t v = bf ? pack_bf16x2(x[j], x[j + 1]) : pack_f16x2(x[j], x[j + 1]);
-      if (j < ncols) o[j] = static_cast<uint16_t>(v);
-      if (j + 1 < ncols) o[j + 1] = static_cast<uint16_t>(v >> 16);
+      for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(x[32 * part + i]);
+      if (lines) store_lines(v, lane, row_ptr);
+      else store_any<4>(v, lane, stage, ncols - 32 * part, true, row_ptr);
+      base += 128;
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = bf ? pack_bf16x2(x[2 * i], x[2 * i + 1]) : pack_f16x2(x[2 * i], x[2 * i + 1]);
+    if (lines) store_lines(v, lane, row_ptr);
+    else store_any<2>(v, lane, stage, ncols, (reinterpret_cast<uintptr_t>(P.out) | static_cast<uintptr_t>(2 * P.out_ld)) % 4 == 0, row_ptr);
   }
 }
 
@@ -701,7 +728,8 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
         stats_epilogue<KIND == KIND_TF32>(P, x, live, row, n0, h.nt, tk, lo, c, share, group, q, lane, X.m);
         __syncwarp();
       } else if (n0 < P.N) {
-        store_epilogue(P, x, row, n0, h.split, lane, X.m);
+        store_epilogue(P, x, row, n0, h.split, lane, X.m,
+                       reinterpret_cast<uint32_t*>(shares) + (warp - 2) * kStageWords);
       }
     }
   }

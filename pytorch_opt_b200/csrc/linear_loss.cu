@@ -196,6 +196,32 @@ __device__ __forceinline__ void split_vec(const uint4& v, float4* hi, float4* lo
 }
 
 
+// One warp: a row of D 16-bit elements on any boundary to one on a 16-byte
+// boundary, 8 elements a lane: the words around them, shifted by half a word
+// where the row starts in the middle of one. Words that reach out of the row
+// are not read: its first and last elements are copied one by one.
+template <class T>
+__device__ __forceinline__ void copy_row16(const T* src, T* dst, int D, int lane) {
+  const bool odd = reinterpret_cast<uintptr_t>(src) % 4 != 0;
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(src) & ~uintptr_t(3));
+  const int first = odd ? 1 : 0, whole = (D - 1) / 8;  // vectors with an element of the row before and after them
+#pragma unroll 4
+  for (int i = first + lane; i < whole; i += 32) {
+    uint32_t x[5];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = words[4 * i + k];
+    x[4] = odd ? words[4 * i + 4] : 0u;
+    uint4 o;
+    o.x = odd ? __funnelshift_r(x[0], x[1], 16) : x[0];
+    o.y = odd ? __funnelshift_r(x[1], x[2], 16) : x[1];
+    o.z = odd ? __funnelshift_r(x[2], x[3], 16) : x[2];
+    o.w = odd ? __funnelshift_r(x[3], x[4], 16) : x[3];
+    reinterpret_cast<uint4*>(dst)[i] = o;
+  }
+  if (odd && lane < 8 && lane < D) dst[lane] = src[lane];
+  for (int i = 8 * whole + lane; i < D; i += 32) dst[i] = src[i];
+}
+
 constexpr int kPackWarps = 8;
 
 // A warp copies a row; a block takes `groups` times 8 consecutive rows. Their
@@ -263,16 +289,15 @@ __global__ void __launch_bounds__(32 * kPackWarps) pack_kernel(PackArgs a, int g
           else reinterpret_cast<uint4*>(dst)[i0 + 32 * u] = v[u];
         }
       }
-    } else {
+    } else if (DT == PO_F32) {
+#pragma unroll 4
       for (int i = lane; i < a.D; i += 32) {
-        if (DT == PO_F32) {
-          const float v = to_f32(src[i]), h = tf32_rna(v);
-          from_f32(h, dst[i]);
-          lo[i] = tf32_rna(v - h);
-        } else {
-          dst[i] = src[i];
-        }
+        const float v = to_f32(src[i]), h = tf32_rna(v);
+        from_f32(h, dst[i]);
+        lo[i] = tf32_rna(v - h);
       }
+    } else {
+      copy_row16(src, dst, a.D, lane);
     }
   }
   if (last && threadIdx.x == 0) {
@@ -293,7 +318,7 @@ __global__ void __launch_bounds__(256) stage_weight_kernel(const void* w, long l
                                                            void* out, float* lo, int vec) {
   grid_launch_next();
   grid_wait();
-  using T = typename ElemOf<DT>::T;
+  using T = typename ElemOf<DT>::T;  // (of 16-bit types only the size matters)
   if (DT == PO_F32 && vec) {
     // A thread splits 4 values; two loads in flight.
     const int n = D / 4;
@@ -317,17 +342,18 @@ __global__ void __launch_bounds__(256) stage_weight_kernel(const void* w, long l
     }
     return;
   }
+  if (DT != PO_F32) {  // a warp a row
+    const int warps = gridDim.x * (blockDim.x >> 5);
+    for (long long v = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); v < V; v += warps)
+      copy_row16(static_cast<const T*>(w) + v * w_ld, static_cast<T*>(out) + v * ldp, D, threadIdx.x & 31);
+    return;
+  }
   for (long long v = blockIdx.x; v < V; v += gridDim.x) {
-    const T* src = static_cast<const T*>(w) + v * w_ld;
-    T* dst = static_cast<T*>(out) + v * ldp;
+    const float* src = static_cast<const float*>(w) + v * w_ld;
     for (int i = threadIdx.x; i < D; i += blockDim.x) {
-      if (DT == PO_F32) {
-        const float x = to_f32(src[i]), h = tf32_rna(x);
-        from_f32(h, dst[i]);
-        lo[v * ldp + i] = tf32_rna(x - h);
-      } else {
-        dst[i] = src[i];
-      }
+      const float x = src[i], h = tf32_rna(x);
+      static_cast<float*>(out)[v * ldp + i] = h;
+      lo[v * ldp + i] = tf32_rna(x - h);
     }
   }
 }
