@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kFewThreads, TT == 8 ? 4 : 0) few_rows_kernel(
     const long long tk = static_cast<long long>(t) * F.top;
     for (int k = lane; k < F.top; k += 32) {
       const int col = F.ent[tk + k] - n0;
-      if (col >= 0 && col < kFewCols) P.zpick[tk + k] = s_z[t][col] * P.scale2;
+      if (col >= 0 && col < kFewCols) P.zpick[tk + k] = s_z[t][col];
     }
   }
   if (count > 0)  // the rows that complete dW's K block

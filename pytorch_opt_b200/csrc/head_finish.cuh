@@ -30,7 +30,7 @@ struct FinishArgs {
   const float* q;      // nullable: hard targets
   const float* qlogq;
   int top;
-  float smoothing, z_loss, temperature, inv_vocab;
+  float smoothing, z_loss, temperature, inv_vocab, scale2;
   float4* stat;        // [row of this launch] max, 1 / sum, log2 sum 2^z2
   float* loss_rows;
   float* loss;         // nullable; written by the last block of the last launch
@@ -76,13 +76,13 @@ __device__ __forceinline__ void finish_row(const FinishArgs& a, int row, int lan
   float loss;
   if (a.q == nullptr) {
     const float lse = lse2 * kLn2, zy = __ldcg(a.zpick + t);
-    loss = kLn2 * ((mm - zy) + log2s) + a.z_loss * lse * lse;
-    if (a.smoothing != 0.0f) loss += a.smoothing * (kLn2 * zy - zs * a.inv_vocab);
+    loss = kLn2 * (log2s - fmaf(zy, a.scale2, -mm)) + a.z_loss * lse * lse;
+    if (a.smoothing != 0.0f) loss += a.smoothing * (zy - zs * a.inv_vocab);
   } else {
     float c = 0.0f;
     for (int k = lane; k < a.top; k += 32) {
       const float q = a.q[t * a.top + k];
-      if (q != 0.0f) c += q * ((mm - __ldcg(a.zpick + t * a.top + k)) + log2s);
+      if (q != 0.0f) c += q * (log2s - fmaf(__ldcg(a.zpick + t * a.top + k), a.scale2, -mm));
     }
     c = warp_sum(c);
     loss = a.temperature * a.temperature * (a.qlogq[t] + kLn2 * c);

@@ -400,7 +400,7 @@ struct RescaleArgs {
   const float* zpick;
   int top;
   const float* row_grad;  // nullable
-  float smoothing, z_loss, inv_vocab, scale;
+  float smoothing, z_loss, inv_vocab, scale, scale2;
   const CallState* st;
 };
 
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
     if (a.q == nullptr) goal = 1.0f - a.smoothing;
     else
       for (int j = k; j < a.top && ent[j] == c; ++j) goal += a.q[t * a.top + j];
-    put_dz<DT>(a, base + c, pcoef * ex2(a.zpick[t * a.top + k] - mm) - flat - w * goal);
+    put_dz<DT>(a, base + c, pcoef * ex2(fmaf(a.zpick[t * a.top + k], a.scale2, -mm)) - flat - w * goal);
   }
 }
 
@@ -772,15 +772,15 @@ int run_head(const Plan& p, int product, HeadParams& P, const HeadOperand& A, co
                : dispatch_head<KIND_BF16>(product, P, static_cast<int>(tiles), s);
 }
 
-// K blocks summed inside the tensor core's accumulator. Relative error of a
-// mean loss at D = 768 / 4096 with 2, 4, 8 blocks (256, 512, 1024 of K):
-// 2.3e-7 / 1.6e-7, 4.1e-7 / 3.1e-7, 6.9e-7 / 6.7e-7; time of the 4096 x 128256
-// x 4096 logits 4.33, 3.59, 3.38 ms before the epilogue's other steps, 3.40
-// and 3.39 ms (4, 8 blocks) after them. 16-bit gradients round to 2^-9: 2048 of
-// K. fp32 (blocks of 32 of K), 500 x 50257 x 768: gradients off by 7e-7 with 2
-// and 4 blocks in logits and gradients, 1.3e-6 with 4 and 4; 2 blocks for 4 in
-// the logits cost 10 of 180 us.
-constexpr int kChunkStats16 = 4, kChunkStats32 = 2, kChunkGrad16 = 16, kChunkGrad32 = 4;
+// K blocks summed inside the tensor core's accumulator, which truncates. 16-bit
+// operands (blocks of 128 of K): a mean loss is off by 2e-7 with 2 and 4e-7 with
+// 4 blocks; 2047 x 128256 x 4096 takes 1.56 and 1.45 ms, 8191 x 32000 x 2048
+// with gradients 753 and 708 us, 8 blocks save nothing more. 16-bit gradients
+// round to 2^-9: 2048 of K. fp32 (blocks of 32 of K), 500 x 50257 x 768: with 1
+// and 2 blocks in the logits the loss is off by 1.1e-7 and 2.9e-7 and the
+// gradients by 4e-7 and 5e-7, and the logits take 214 and 196 us of 700 and 680;
+// few confident rows, whose gradients are small differences, need the former.
+constexpr int kChunkStats16 = 4, kChunkStats32 = 1, kChunkGrad16 = 16, kChunkGrad32 = 4;
 
 bool vec32(const void* p, long long ld, int es) {
   return reinterpret_cast<uintptr_t>(p) % 32 == 0 && (ld * es) % 32 == 0;
@@ -908,7 +908,8 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
     FinishArgs fa{};
     fa.part = p.part, fa.zsum = smoothing != 0.0f ? p.zsum : nullptr, fa.nparts = p.nparts, fa.row0 = static_cast<int>(row0);
     fa.rowmap = p.rowmap, fa.zpick = p.zpick, fa.ent = p.ent, fa.q = soft ? p.q : nullptr, fa.qlogq = p.qlogq;
-    fa.top = static_cast<int>(top), fa.smoothing = smoothing, fa.z_loss = z_loss, fa.temperature = temperature;
+    fa.top = static_cast<int>(top), fa.smoothing = smoothing, fa.z_loss = z_loss;
+    fa.temperature = temperature, fa.scale2 = kLog2e / temperature;
     fa.inv_vocab = 1.0f / static_cast<float>(vocab), fa.stat = p.stat, fa.loss_rows = loss_rows, fa.loss = loss;
     fa.T = tokens, fa.mean = mean, fa.final_launch = c == p.nchunks - 1, fa.st = p.st;
     if (p.want_dw) {
@@ -948,7 +949,7 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
     RescaleArgs ra{};
     ra.e = p.e, ra.lo = p.e_lo, ra.e_ld = p.e_ld, ra.V = vocab, ra.part = p.part, ra.nparts = p.nparts, ra.part_cols = p.part_cols, ra.stat = p.stat;
     ra.row0 = static_cast<int>(row0), ra.rows = rows, ra.rowmap = p.rowmap, ra.ent = p.ent, ra.q = soft ? p.q : nullptr;
-    ra.zpick = p.zpick, ra.top = static_cast<int>(top), ra.row_grad = row_grad, ra.smoothing = smoothing;
+    ra.scale2 = kLog2e / temperature, ra.zpick = p.zpick, ra.top = static_cast<int>(top), ra.row_grad = row_grad, ra.smoothing = smoothing;
     ra.z_loss = z_loss, ra.inv_vocab = 1.0f / static_cast<float>(vocab), ra.scale = gscale, ra.st = p.st;
     const int nseg = cdiv(p.e_ld, kSegment);
     const long long rblocks = krows * nseg;
