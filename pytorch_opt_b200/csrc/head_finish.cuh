@@ -17,9 +17,31 @@ struct CallState {
   int done;          // blocks of the finishing launch that are through
   float alpha;       // factor of the gradient products
   float grad_max;    // max |row_grad|
+  int splits;        // of K in the next dH product
+};
+
+// Cost of `s` splits of K for a product's tiles, in 16-bit K blocks (~0.6 us):
+// the tiles' waves over the pairs of SMs, each tile paying its blocks and about
+// 3 more to fill and drain, plus the join's traffic (8 bytes a value and split
+// at ~5 TB/s).
+__host__ __device__ inline float split_cost(int s, int tiles, int nkb, float values, int pairs) {
+  const int waves = (tiles * s + pairs - 1) / pairs;
+  const float cost = static_cast<float>(waves) * (static_cast<float>((nkb + s - 1) / s) + 3.0f);
+  return s > 1 ? cost + 5.0f + static_cast<float>(s) * values * (8.0f / 3.0e6f) : cost;
+}
+
+// The split of dH's K is chosen again from the counted rows, which fill fewer
+// tiles than the rows the host knows of. A pass of 50257 x 768, the host's
+// choice against this one: bf16, 410 of 2048 rows 233 / 183 us, 410 of 1024 183
+// / 171, fp32, 400 of 1000 740 / 662; all rows counted: the same.
+struct SplitArgs {
+  int nkb;     // K blocks (0: the host's choice stays)
+  int tiles_n, dim, pairs;
+  int units;   // tiles times splits that the workspace holds
 };
 
 struct FinishArgs {
+  SplitArgs split;
   const float2* part;
   const float* zsum;
   int nparts;

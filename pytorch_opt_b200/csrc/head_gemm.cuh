@@ -68,6 +68,7 @@ struct alignas(64) HeadParams {
   const int* count;  // device: counted rows of the whole call
   int row0;          // first packed row of this launch
   int tiles_n, splits, band;
+  const int* splits_at;  // nullable: the number of splits stands there
   int chunk;         // K blocks summed inside the accumulator
   uint32_t fmt;      // operand format of the instruction descriptor
   unsigned int* sched;
@@ -92,7 +93,7 @@ struct alignas(64) HeadParams {
   int out_dtype;       // PO_F32 / PO_BF16 / PO_F16
   int vec;             // 32-byte vector access legal
   const int* out_rows;
-  float* partial;      // splits > 1: [split][M][part_ld] fp32, instead of out
+  float* partial;      // splits > 1: [split][rows][part_ld] fp32, instead of out
   long long part_ld;
 };
 
@@ -157,7 +158,7 @@ struct HeadTile {
 
 // Extents of this launch after the device-side count.
 struct HeadExtent {
-  int m, tiles_m, nkb, total;
+  int m, tiles_m, nkb, splits, total;
 };
 
 template <class C>
@@ -168,7 +169,8 @@ __device__ __forceinline__ HeadExtent head_extent(const HeadParams& P) {
   const int k = P.limit == LIMIT_K ? min(P.K, left) : P.K;
   x.tiles_m = (x.m + C::TM - 1) / C::TM;
   x.nkb = (k + C::BK - 1) / C::BK;
-  x.total = x.tiles_m * P.tiles_n * P.splits;
+  x.splits = P.splits_at != nullptr ? *P.splits_at : P.splits;
+  x.total = x.tiles_m * P.tiles_n * x.splits;
   return x;
 }
 
@@ -177,7 +179,7 @@ __device__ __forceinline__ HeadExtent head_extent(const HeadParams& P) {
 __device__ __forceinline__ HeadTile head_tile(const HeadParams& P, const HeadExtent& x, int t) {
   HeadTile h;
   const int per = x.tiles_m * P.tiles_n;
-  h.split = P.splits > 1 ? t / per : 0;
+  h.split = x.splits > 1 ? t / per : 0;
   const int r = t - h.split * per;
   const int b = x.tiles_m <= P.band ? 0 : r / (P.band * P.tiles_n);
   const int first = b * P.band;
@@ -187,9 +189,9 @@ __device__ __forceinline__ HeadTile head_tile(const HeadParams& P, const HeadExt
   h.nt = in_band / rows;
   h.kb0 = 0;
   h.kb1 = x.nkb;
-  if (P.splits > 1) {
-    h.kb0 = static_cast<int>(static_cast<long long>(x.nkb) * h.split / P.splits);
-    h.kb1 = static_cast<int>(static_cast<long long>(x.nkb) * (h.split + 1) / P.splits);
+  if (x.splits > 1) {
+    h.kb0 = static_cast<int>(static_cast<long long>(x.nkb) * h.split / x.splits);
+    h.kb1 = static_cast<int>(static_cast<long long>(x.nkb) * (h.split + 1) / x.splits);
   }
   return h;
 }
@@ -369,13 +371,13 @@ __device__ __forceinline__ void stats_epilogue(const HeadParams& P, float (&x)[H
 }
 
 __device__ __forceinline__ void store_epilogue(const HeadParams& P, float (&x)[HC], int row, int n0, int split,
-                                               int lane, int m_rows, uint32_t* stage) {
+                                               int splits, int lane, int m_rows, uint32_t* stage) {
   const int ncols = min(HC, P.N - n0);
   const int row_w = row - lane;
-  if (P.splits > 1) {
+  if (splits > 1) {
     // part_ld is a multiple of 256: whole lines, on 128-byte boundaries.
     char* base =
-        reinterpret_cast<char*>(P.partial + (static_cast<long long>(split) * P.M + row_w) * P.part_ld + n0);
+        reinterpret_cast<char*>(P.partial + (static_cast<long long>(split) * m_rows + row_w) * P.part_ld + n0);
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
       uint32_t v[32];
@@ -730,7 +732,7 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
         stats_epilogue<KIND == KIND_TF32>(P, x, live, row, n0, h.nt, tk, lo, c, share, group, q, lane, X.m);
         __syncwarp();
       } else if (n0 < P.N) {
-        store_epilogue(P, x, row, n0, h.split, lane, X.m,
+        store_epilogue(P, x, row, n0, h.split, X.splits, lane, X.m,
                        reinterpret_cast<uint32_t*>(shares) + (warp - 2) * kStageWords);
       }
     }

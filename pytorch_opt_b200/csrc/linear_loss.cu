@@ -363,6 +363,27 @@ __global__ void __launch_bounds__(256) stage_weight_kernel(const void* w, long l
 // ones are zeroed up to a K block of dW, where they meet the zeros of dZ.
 constexpr int kFinishWarps = 8;
 
+// One warp: the cheapest split for this launch's rows (the host's rule).
+__device__ __forceinline__ void choose_splits(const FinishArgs& a, int left, int lane) {
+  const SplitArgs& c = a.split;
+  const int rows = max(1, min(a.rows, left));
+  const int tiles = (rows + 255) / 256 * c.tiles_n;
+  const int most = max(1, min(min(c.pairs, (c.nkb + 3) / 4), c.units / tiles));
+  const float values = static_cast<float>(rows) * static_cast<float>(c.dim);
+  float cost = INFINITY;
+  int best = 1;
+  for (int s = 1 + lane; s <= most; s += 32) {
+    const float x = split_cost(s, tiles, c.nkb, values, c.pairs) * (s == 1 ? 0.98f : 1.0f);
+    if (x < cost) cost = x, best = s;
+  }
+  for (int o = 16; o > 0; o >>= 1) {
+    const float x = __shfl_xor_sync(0xffffffffu, cost, o);
+    const int s = __shfl_xor_sync(0xffffffffu, best, o);
+    if (x < cost || (x == cost && s < best)) cost = x, best = s;
+  }
+  if (lane == 0) a.st->splits = best;
+}
+
 __global__ void __launch_bounds__(32 * kFinishWarps) finish_kernel(FinishArgs a) {
   grid_launch_next();
   grid_wait();
@@ -374,6 +395,7 @@ __global__ void __launch_bounds__(32 * kFinishWarps) finish_kernel(FinishArgs a)
   if (row < left && row < a.rows) finish_row(a, row, lane);
   else if (left > 0 && row < (left + kRowPad - 1) / kRowPad * kRowPad && row < (a.rows + kRowPad - 1) / kRowPad * kRowPad)
     zero_row(a, row, lane);
+  if (a.split.nkb > 0 && blockIdx.x == 0 && threadIdx.x < 32) choose_splits(a, left, lane);
   if (a.loss == nullptr || !a.final_launch) return;
   __threadfence();
   __syncthreads();
@@ -507,13 +529,15 @@ __global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
 // ------------------------------------------------------------------- join
 // out[rows[row0 + r] or r][c] = alpha sum_s partial[s][r][c], in order of s.
 template <int DT>
-__global__ void __launch_bounds__(256) join_kernel(const float* partial, int splits, int M, long long pld,
-                                                   int N, const float* alpha, const int* count, int row0, int limit_rows,
-                                                   const int* rows, void* out, long long ld) {
+__global__ void __launch_bounds__(256) join_kernel(const float* partial, int splits, const int* splits_at, int M,
+                                                   long long pld, int N, const float* alpha, const int* count, int row0,
+                                                   int limit_rows, const int* rows, void* out, long long ld) {
   grid_launch_next();
   grid_wait();
+  if (splits_at != nullptr) splits = *splits_at;
+  if (limit_rows) M = min(M, *count - row0);
   const int r = blockIdx.x;
-  if (limit_rows && row0 + r >= *count) return;
+  if (r >= M || splits == 1) return;  // (one split wrote the output itself)
   const float al = *alpha;
   typename ElemOf<DT>::T* o =
       static_cast<typename ElemOf<DT>::T*>(out) + (rows != nullptr ? rows[row0 + r] : r) * ld;
@@ -603,18 +627,16 @@ int encode_operand(CUtensorMap map[2], const HeadOperand& o) {
   return PO_OK;
 }
 
-// Splits of K for a store product: the tiles' waves over the pairs, each tile
-// paying its K blocks and about 3 more to fill and drain, plus the join's
-// traffic (8 bytes a value and split at ~5 TB/s, in blocks of ~0.6 us).
+// Splits of K for a store product.
 int choose_splits(long long tiles, int nkb, long long M, long long N) {
-  const long long pairs = sm_count() / 2;
+  const int pairs = sm_count() / 2;
+  if (tiles > 16 * pairs) return 1;  // (a last wave weighs little)
+  const float values = static_cast<float>(M) * static_cast<float>(N);
   int best = 1;
-  double best_cost = 1e300;
+  float best_cost = INFINITY;
   for (int s = 1; s <= pairs && s <= (nkb + 3) / 4; ++s) {
-    const double waves = static_cast<double>((tiles * s + pairs - 1) / pairs);
-    double cost = waves * (static_cast<double>((nkb + s - 1) / s) + 3.0);
-    if (s > 1) cost += 5.0 + static_cast<double>(s) * static_cast<double>(M) * static_cast<double>(N) * 8.0 / 3.0e6;
-    if (cost < best_cost * 0.98) {
+    const float cost = split_cost(s, static_cast<int>(tiles), nkb, values, pairs);
+    if (cost < best_cost * 0.98f) {
       best_cost = cost;
       best = s;
     }
@@ -638,6 +660,7 @@ struct Plan {
   long long e_ld;
   int bk;
   int splits_dh, splits_dw;
+  int dh_blocks, split_units;  // dH's splits are chosen on the device (0: they are not)
   bool dw_acc;
   // workspace
   CallState* st;
@@ -705,6 +728,13 @@ int make_plan(Plan& p, const void* weight, long long w_ld, int dtype, long long 
   // K blocks in units of a 16-bit one's time (an fp32 block issues 1.5 times as much).
   const auto blocks = [&](long long k) { return p.f32 ? cdiv(3LL * cdiv(k, p.bk), 2) : cdiv(k, p.bk); };
   p.splits_dh = want_dh ? choose_splits(mt * nd, blocks(V), p.chunk, D) : 1;
+  // Fewer rows may count, and fewer tiles then take more splits: the finishing
+  // kernel chooses, within 256 KB a tile and split and four units a pair of SMs.
+  if (want_dh && mt > 1 && mt * nd <= 16 * (sm_count() / 2)) {
+    p.dh_blocks = blocks(V);
+    const long long units = mt * nd * p.splits_dh;
+    p.split_units = static_cast<int>(units > 4 * (sm_count() / 2) ? units : 4 * (sm_count() / 2));
+  }
   p.dw_acc = want_dw && p.nchunks > 1;
   p.splits_dw = want_dw && !p.dw_acc ? choose_splits(nv * nd, blocks(p.chunk), V, D) : 1;
 
@@ -736,7 +766,8 @@ int make_plan(Plan& p, const void* weight, long long w_ld, int dtype, long long 
     if (p.f32) p.e_lo = f32(rows * p.e_ld);
     const long long pld = round_up(D, 256);
     long long partial = 0;
-    if (p.splits_dh > 1) partial = p.splits_dh * p.chunk * pld;
+    if (p.split_units > 0) partial = static_cast<long long>(p.split_units) * (256 * 256);
+    else if (p.splits_dh > 1) partial = p.splits_dh * p.chunk * pld;
     if (p.splits_dw > 1 && p.splits_dw * V * pld > partial) partial = p.splits_dw * V * pld;
     if (partial > 0) p.partial = f32(partial);
     if (p.dw_acc && !p.f32) p.dw_accum = f32(V * round_up(D, 8));
@@ -745,11 +776,11 @@ int make_plan(Plan& p, const void* weight, long long w_ld, int dtype, long long 
   return ar.overflow() ? set_error(PO_ERR_WORKSPACE, "linear_loss: workspace too small") : PO_OK;
 }
 
-int join(int dtype, const float* partial, int splits, int M, long long pld, int N, const Plan& p, int row0,
+int join(int dtype, const float* partial, int splits, const int* splits_at, int M, long long pld, int N, const Plan& p, int row0,
          bool limit_rows, const int* rows, void* out, long long ld, cudaStream_t s) {
   const dim3 grid(M, N > 4096 ? 4 : 1);
   const auto kern = dtype == PO_F32 ? join_kernel<PO_F32> : dtype == PO_BF16 ? join_kernel<PO_BF16> : join_kernel<PO_F16>;
-  return launch_next(false, kern, grid, 256, 0, s, "linear_loss join", partial, splits, M, pld, N, &p.st->alpha, &p.st->count,
+  return launch_next(false, kern, grid, 256, 0, s, "linear_loss join", partial, splits, splits_at, M, pld, N, &p.st->alpha, &p.st->count,
                      row0, limit_rows, rows, out, ld);
 }
 
@@ -918,6 +949,7 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
       fa.row_words = static_cast<int>(p.ldp * p.es / 16);
     }
     fa.rows = rows;
+    if (p.split_units > 0) fa.split = {p.dh_blocks, cdiv(D, 256), D, sm_count() / 2, p.split_units};
     if (p.few) {
       FewParams P{};
       P.h = hidden, P.h_ld = h_ld, P.w = weight, P.w_ld = w_ld, P.D = D, P.V = V;
@@ -968,9 +1000,10 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
       P.out_rows = p.rowmap, P.partial = p.partial, P.part_ld = pld;
       const HeadOperand A{{p.e, p.e_lo}, dtype, rows, vocab, p.e_ld, true};
       const HeadOperand B{{w, p.w_lo}, dtype, vocab, dim, wld, false};
+      P.splits_at = p.split_units > 0 ? &p.st->splits : nullptr;
       if ((r = run_head(p, HEAD_DHIDDEN, P, A, B, p.splits_dh, s))) return r;
-      if (p.splits_dh > 1 &&
-          (r = join(dtype, p.partial, p.splits_dh, rows, pld, D, p, static_cast<int>(row0), true, p.rowmap, dhidden, dh_ld, s)))
+      if ((p.splits_dh > 1 || P.splits_at != nullptr) &&
+          (r = join(dtype, p.partial, p.splits_dh, P.splits_at, rows, pld, D, p, static_cast<int>(row0), true, p.rowmap, dhidden, dh_ld, s)))
         return r;
     }
     if (p.want_dw) {
@@ -994,7 +1027,7 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
       const HeadOperand A{{p.e, p.e_lo}, dtype, krows, vocab, p.e_ld, false};
       const HeadOperand B{{hp, hlo}, dtype, p.rows_alloc - row0 < krows ? p.rows_alloc - row0 : krows, dim, p.ldp, false};
       if ((r = run_head(p, HEAD_DWEIGHT, P, A, B, p.splits_dw, s))) return r;
-      if (p.splits_dw > 1 && (r = join(dtype, p.partial, p.splits_dw, V, pld, D, p, 0, false, nullptr, dweight, dw_ld, s)))
+      if (p.splits_dw > 1 && (r = join(dtype, p.partial, p.splits_dw, nullptr, V, pld, D, p, 0, false, nullptr, dweight, dw_ld, s)))
         return r;
     }
   }

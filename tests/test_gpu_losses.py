@@ -204,6 +204,23 @@ def test_linear_cross_entropy_nothing_counts(dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("counted", [1, 200, 257, 1100])
+def test_linear_cross_entropy_few_of_many_rows_count(dtype, counted):
+    # How dH's long axis is split goes by the rows that count, on the device.
+    T, D, V = 1100, 264, 6001
+    h, w, y = _head(T, D, V, DTYPES[dtype], seed=counted)
+    drop = torch.randperm(T, generator=_gen(2), device="cuda")[counted:]
+    y[drop] = -100
+    want, dh, dw = ref_ce(h, w, y)
+    h.requires_grad_(), w.requires_grad_()
+    loss = losses.linear_cross_entropy(h, w, y, reduction="sum")
+    assert abs(float(loss.detach() - want.sum())) <= float(_loss_bound(h.detach(), w.detach())[y != -100].sum())
+    gh, gw = _grads(loss, h, w)
+    assert _rel(gh, dh) < GRAD_TOL[DTYPES[dtype]] and _rel(gw, dw) < GRAD_TOL[DTYPES[dtype]]
+    assert (gh[drop] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 def test_linear_cross_entropy_masked_rows_hold_anything(dtype):
     T, D, V = 140, 72, 300
     h, w, y = _head(T, D, V, DTYPES[dtype], seed=5)
