@@ -43,6 +43,7 @@ struct DistillArgs {
   float* loss_rows;
   float* loss;
   DistillState* st;
+  float* unscale;  // nullable: 1 / store_scale
   int seg;  // elements a CTA takes
 };
 
@@ -54,6 +55,14 @@ __device__ __forceinline__ int entry_status(const DistillArgs& a, long long t, i
   if (x < 0) return ROW_IGNORED;
   l = load_as_f32(a.teacher, a.teacher_dtype, t * a.teacher_ld + k);
   return l > -INFINITY || isnan(l) ? ROW_COUNTED : ROW_IGNORED;
+}
+
+// The power of two that fp16 gradients of a mean are stored by, so that the
+// rounding here comes above fp16's smallest values and the caller's loss scale
+// not too late: |dz| <= 2 a / n, times n 2^14 / max(a, 1) at most.
+__device__ __forceinline__ float store_scale(const DistillArgs& a) {
+  if (a.unscale == nullptr) return 1.0f;
+  return exp2f(floorf(log2f(static_cast<float>(a.st->count) / fmaxf(a.temperature, 1.0f))) + 14.0f);
 }
 
 // Rows that the mean divides by (counted ones and those with a bad index).
@@ -311,6 +320,7 @@ __global__ void __launch_bounds__((GRAD ? kGradThreads : kEvalThreads) + 32, GRA
       c = warp_sum(c);
       if (lane == 0) {
         a.loss_rows[t] = live ? a.temperature * a.temperature * (s_qlogq + c) : (status == ROW_BAD ? NAN : 0.0f);
+        if (a.unscale != nullptr && t == 0) *a.unscale = a.st->count > 0 ? 1.0f / store_scale(a) : 1.0f;
         if (a.loss != nullptr) {
           __threadfence();
           s_last = atomicAdd(&a.st->done, 1u) == static_cast<unsigned int>(a.T) - 1;
@@ -325,7 +335,7 @@ __global__ void __launch_bounds__((GRAD ? kGradThreads : kEvalThreads) + 32, GRA
     float w = 0.0f;
     if (live) {
       w = a.temperature;
-      if (a.mean) w /= static_cast<float>(a.st->count);
+      if (a.mean) w *= store_scale(a) / static_cast<float>(a.st->count);
       if (a.row_grad != nullptr) w *= a.row_grad[t];
     }
     const float ws = w / s;
@@ -472,6 +482,7 @@ extern "C" int po_distill_logits(const void* logits, long long ld, int dtype, lo
   a.index = index, a.index_ld = index_ld, a.teacher = teacher, a.teacher_ld = teacher_ld;
   a.teacher_dtype = teacher_dtype, a.top = static_cast<int>(top), a.temperature = temperature, a.mean = mean;
   a.row_grad = row_grad, a.loss_rows = loss_rows, a.loss = loss;
+  if (mean == PO_MEAN_SCALED && dtype == PO_F16 && dlogits != nullptr) a.unscale = loss_rows + tokens;
   if (loss != nullptr || mean) {
     if (workspace == nullptr || workspace_bytes < sizeof(DistillState))
       return set_error(PO_ERR_WORKSPACE, "distill_logits: workspace too small");

@@ -16,6 +16,7 @@ struct CallState {
   int counted_mean;  // rows that the mean divides by
   int done;          // blocks of the finishing launch that are through
   float alpha;       // factor of the gradient products
+  float alpha_dh, alpha_dw;  // the same, with the power of two that each is stored by
   float grad_max;    // max |row_grad|
   int splits;        // of K in the next dH product
 };
@@ -59,6 +60,9 @@ struct FinishArgs {
   long long T;
   int mean, final_launch;
   CallState* st;
+  const float* rowmax;  // fp16, scaled gradients (else null): max |h| of each packed row
+  float* unscale;       // receives the inverses of the powers of two
+  float margin;         // what else may make dZ larger than softmax
   uint4* packed;       // 16-byte words of H's packed rows of this launch (and of their low halves, nullable)
   uint4* packed_lo;
   int row_words;

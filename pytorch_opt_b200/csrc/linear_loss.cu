@@ -166,6 +166,8 @@ struct PackArgs {
   unsigned int* sched;
   float alpha;
   int mean, has_row_grad;
+  float* rowmax;   // nullable: max |h| of each packed row
+  float* unscale;
 };
 
 __device__ __forceinline__ int row_status(const PackArgs& a, long long t, int& target) {
@@ -222,6 +224,13 @@ __device__ __forceinline__ void copy_row16(const T* src, T* dst, int D, int lane
   for (int i = 8 * whole + lane; i < D; i += 32) dst[i] = src[i];
 }
 
+// Eight fp16 values.
+__device__ __forceinline__ float max_abs(const uint4& v) {
+  const __half2* h = reinterpret_cast<const __half2*>(&v);
+  const float2 f = __half22float2(__hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3]))));
+  return fmaxf(f.x, f.y);
+}
+
 constexpr int kPackWarps = 8;
 
 // A warp copies a row; a block takes `groups` times 8 consecutive rows. Their
@@ -275,6 +284,7 @@ __global__ void __launch_bounds__(32 * kPackWarps) pack_kernel(PackArgs a, int g
     T* dst = static_cast<T*>(a.packed) + static_cast<long long>(place) * a.ldp;
     float* lo = DT == PO_F32 ? a.packed_lo + static_cast<long long>(place) * a.ldp : nullptr;
     constexpr int VEC = 16 / sizeof(T);
+    float top = 0.0f;
     if (a.vec) {
       const int n = a.D / VEC;
       for (int i0 = lane; i0 < n; i0 += 128) {  // four loads in flight
@@ -285,6 +295,7 @@ __global__ void __launch_bounds__(32 * kPackWarps) pack_kernel(PackArgs a, int g
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           if (i0 + 32 * u >= n) continue;
+          if (DT == PO_F16 && a.rowmax != nullptr) top = fmaxf(top, max_abs(v[u]));
           if (DT == PO_F32) split_vec(v[u], reinterpret_cast<float4*>(dst) + i0 + 32 * u, reinterpret_cast<float4*>(lo) + i0 + 32 * u);
           else reinterpret_cast<uint4*>(dst)[i0 + 32 * u] = v[u];
         }
@@ -298,6 +309,12 @@ __global__ void __launch_bounds__(32 * kPackWarps) pack_kernel(PackArgs a, int g
       }
     } else {
       copy_row16(src, dst, a.D, lane);
+      if (DT == PO_F16 && a.rowmax != nullptr)
+        for (int i = lane; i < a.D; i += 32) top = fmaxf(top, fabsf(to_f32(src[i])));
+    }
+    if (DT == PO_F16 && a.rowmax != nullptr) {
+      top = warp_max(top);
+      if (lane == 0) a.rowmax[place] = top;
     }
   }
   if (last && threadIdx.x == 0) {
@@ -308,7 +325,8 @@ __global__ void __launch_bounds__(32 * kPackWarps) pack_kernel(PackArgs a, int g
     float alpha = a.alpha;
     if (a.mean) alpha /= static_cast<float>(all > 0 ? all : 1);
     if (a.has_row_grad) alpha *= a.st->grad_max;
-    a.st->alpha = alpha;
+    a.st->alpha = a.st->alpha_dh = a.st->alpha_dw = alpha;
+    if (a.unscale != nullptr) a.unscale[0] = a.unscale[1] = 1.0f;
   }
 }
 
@@ -384,6 +402,26 @@ __device__ __forceinline__ void choose_splits(const FinishArgs& a, int left, int
   if (lane == 0) a.st->splits = best;
 }
 
+// One block: the powers of two that fp16 gradients of a mean are stored by. A
+// mean's gradients may lie below fp16's range until the caller's loss scale
+// lifts them, which comes after the rounding here. With dZ's row at most 2 in
+// sum of magnitudes, |dH| <= 2 max|W| / n and |dW| <= 2 max|h|: neither leaves
+// the range by its factor (n / 2 at most, and half the room that max|h| leaves).
+__device__ __forceinline__ void choose_scales(const FinishArgs& a, float* buf) {
+  float top = 0.0f;
+  for (int i = threadIdx.x; i < a.st->count; i += blockDim.x) top = fmaxf(top, a.rowmax[i]);
+  top = fmaxf(block_max(top, buf), 1e-4f) * a.margin;
+  if (threadIdx.x != 0) return;
+  const int n = a.st->counted_mean;
+  const float dh = n > 1 ? exp2f(floorf(log2f(static_cast<float>(n) / a.margin)) - 1.0f) : 1.0f;
+  const float dw = exp2f(floorf(log2f(16384.0f / top)));
+  const float sh = fminf(fmaxf(dh, 1.0f), 65536.0f), sw = fminf(fmaxf(dw, 1.0f), 65536.0f);
+  a.st->alpha_dh = a.st->alpha * sh;
+  a.st->alpha_dw = a.st->alpha * sw;
+  a.unscale[0] = 1.0f / sh;
+  a.unscale[1] = 1.0f / sw;
+}
+
 __global__ void __launch_bounds__(32 * kFinishWarps) finish_kernel(FinishArgs a) {
   grid_launch_next();
   grid_wait();
@@ -395,6 +433,7 @@ __global__ void __launch_bounds__(32 * kFinishWarps) finish_kernel(FinishArgs a)
   if (row < left && row < a.rows) finish_row(a, row, lane);
   else if (left > 0 && row < (left + kRowPad - 1) / kRowPad * kRowPad && row < (a.rows + kRowPad - 1) / kRowPad * kRowPad)
     zero_row(a, row, lane);
+  if (a.rowmax != nullptr && blockIdx.x == 0) choose_scales(a, reinterpret_cast<float*>(dbuf));
   if (a.split.nkb > 0 && blockIdx.x == 0 && threadIdx.x < 32) choose_splits(a, left, lane);
   if (a.loss == nullptr || !a.final_launch) return;
   __threadfence();
@@ -659,6 +698,7 @@ struct Plan {
   int nparts;
   long long e_ld;
   int bk;
+  float* rowmax;
   int splits_dh, splits_dw;
   int dh_blocks, split_units;  // dH's splits are chosen on the device (0: they are not)
   bool dw_acc;
@@ -744,6 +784,7 @@ int make_plan(Plan& p, const void* weight, long long w_ld, int dtype, long long 
   p.st = static_cast<CallState*>(ar.take(sizeof(CallState)));
   p.sched = static_cast<unsigned int*>(ar.take(8));
   p.rowmap = i32(T);
+  if (dtype == PO_F16) p.rowmax = f32(T);
   p.ent = i32(T * top);
   p.zpick = f32(T * top);
   if (soft) {
@@ -776,11 +817,11 @@ int make_plan(Plan& p, const void* weight, long long w_ld, int dtype, long long 
   return ar.overflow() ? set_error(PO_ERR_WORKSPACE, "linear_loss: workspace too small") : PO_OK;
 }
 
-int join(int dtype, const float* partial, int splits, const int* splits_at, int M, long long pld, int N, const Plan& p, int row0,
+int join(int dtype, const float* alpha, const float* partial, int splits, const int* splits_at, int M, long long pld, int N, const Plan& p, int row0,
          bool limit_rows, const int* rows, void* out, long long ld, cudaStream_t s) {
   const dim3 grid(M, N > 4096 ? 4 : 1);
   const auto kern = dtype == PO_F32 ? join_kernel<PO_F32> : dtype == PO_BF16 ? join_kernel<PO_BF16> : join_kernel<PO_F16>;
-  return launch_next(false, kern, grid, 256, 0, s, "linear_loss join", partial, splits, splits_at, M, pld, N, &p.st->alpha, &p.st->count,
+  return launch_next(false, kern, grid, 256, 0, s, "linear_loss join", partial, splits, splits_at, M, pld, N, alpha, &p.st->count,
                      row0, limit_rows, rows, out, ld);
 }
 
@@ -912,6 +953,8 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
   pa.packed = p.packed, pa.packed_lo = p.packed_lo;
   pa.dhidden = dhidden, pa.dh_ld = dh_ld, pa.loss_rows = loss_rows, pa.st = p.st, pa.sched = p.sched;
   pa.alpha = temperature / gscale, pa.mean = mean, pa.has_row_grad = row_grad != nullptr;
+  float* unscale = mean == PO_MEAN_SCALED && p.grads ? loss_rows + tokens : nullptr;
+  pa.unscale = unscale, pa.rowmax = unscale != nullptr && dtype == PO_F16 && !p.few ? p.rowmax : nullptr;
   const int groups = cdiv(T, 2048 * kPackWarps), pblocks = cdiv(T, groups * kPackWarps);
   const auto pack = dtype == PO_F32 ? pack_kernel<PO_F32> : dtype == PO_BF16 ? pack_kernel<PO_BF16> : pack_kernel<PO_F16>;
   if ((r = launch_next(first, pack, pblocks, 32 * kPackWarps, 0, s, "linear_loss pack", pa, groups))) return r;
@@ -949,6 +992,8 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
       fa.row_words = static_cast<int>(p.ldp * p.es / 16);
     }
     fa.rows = rows;
+    fa.rowmax = pa.rowmax, fa.unscale = unscale;
+    fa.margin = fmaxf(temperature, 1.0f) * (1.0f + 128.0f * fabsf(z_loss));
     if (p.split_units > 0) fa.split = {p.dh_blocks, cdiv(D, 256), D, sm_count() / 2, p.split_units};
     if (p.few) {
       FewParams P{};
@@ -996,14 +1041,14 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
       memset(&P, 0, sizeof(P));
       P.M = rows, P.N = D, P.K = V, P.limit = LIMIT_M, P.row0 = static_cast<int>(row0), P.band = 8;
       P.chunk = p.f32 ? kChunkGrad32 : kChunkGrad16;
-      P.alpha = &p.st->alpha, P.out = dhidden, P.out_ld = dh_ld, P.out_dtype = dtype, P.vec = vec32(dhidden, dh_ld, p.es);
+      P.alpha = &p.st->alpha_dh, P.out = dhidden, P.out_ld = dh_ld, P.out_dtype = dtype, P.vec = vec32(dhidden, dh_ld, p.es);
       P.out_rows = p.rowmap, P.partial = p.partial, P.part_ld = pld;
       const HeadOperand A{{p.e, p.e_lo}, dtype, rows, vocab, p.e_ld, true};
       const HeadOperand B{{w, p.w_lo}, dtype, vocab, dim, wld, false};
       P.splits_at = p.split_units > 0 ? &p.st->splits : nullptr;
       if ((r = run_head(p, HEAD_DHIDDEN, P, A, B, p.splits_dh, s))) return r;
       if ((p.splits_dh > 1 || P.splits_at != nullptr) &&
-          (r = join(dtype, p.partial, p.splits_dh, P.splits_at, rows, pld, D, p, static_cast<int>(row0), true, p.rowmap, dhidden, dh_ld, s)))
+          (r = join(dtype, P.alpha, p.partial, p.splits_dh, P.splits_at, rows, pld, D, p, static_cast<int>(row0), true, p.rowmap, dhidden, dh_ld, s)))
         return r;
     }
     if (p.want_dw) {
@@ -1011,7 +1056,7 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
       memset(&P, 0, sizeof(P));
       P.M = V, P.N = D, P.K = rows, P.limit = LIMIT_K, P.row0 = static_cast<int>(row0), P.band = 8;
       P.chunk = p.f32 ? kChunkGrad32 : kChunkGrad16;
-      P.alpha = &p.st->alpha, P.partial = p.partial, P.part_ld = pld;
+      P.alpha = &p.st->alpha_dw, P.partial = p.partial, P.part_ld = pld;
       const bool to_acc = p.dw_acc && !p.f32;  // fp32 gradients add up in place
       const bool last = c == p.nchunks - 1;
       float* acc = to_acc ? p.dw_accum : static_cast<float*>(dweight);
@@ -1027,7 +1072,7 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
       const HeadOperand A{{p.e, p.e_lo}, dtype, krows, vocab, p.e_ld, false};
       const HeadOperand B{{hp, hlo}, dtype, p.rows_alloc - row0 < krows ? p.rows_alloc - row0 : krows, dim, p.ldp, false};
       if ((r = run_head(p, HEAD_DWEIGHT, P, A, B, p.splits_dw, s))) return r;
-      if (p.splits_dw > 1 && (r = join(dtype, p.partial, p.splits_dw, nullptr, V, pld, D, p, 0, false, nullptr, dweight, dw_ld, s)))
+      if (p.splits_dw > 1 && (r = join(dtype, P.alpha, p.partial, p.splits_dw, nullptr, V, pld, D, p, 0, false, nullptr, dweight, dw_ld, s)))
         return r;
     }
   }

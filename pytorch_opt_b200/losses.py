@@ -16,7 +16,8 @@ Three functions of CUDA tensors (bf16, fp16 or fp32), differentiable by
 Rows that count for nothing (``ignore_index``, no teacher's entry) have loss
 and gradient 0, are left out of the mean, and cost no product. With a scalar
 reduction the gradients are made together with the loss (the softmax is not
-computed a second time) whenever an input requires grad; with
+computed a second time) whenever an input requires grad (fp16 ones of a mean by
+powers of two, so that a loss scale does not come too late); with
 ``reduction="none"`` they are made in the backward pass from the upstream
 gradient of each row. Errors are ``RuntimeError`` as in ``native``; there is no
 CPU path.
@@ -33,6 +34,7 @@ from . import _lib
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _REDUCTIONS = ("mean", "sum", "none")
 MAX_TOP = 1024
+_MEAN_SCALED = 2  # PO_MEAN_SCALED
 
 
 def _check_tensors(name: str, first, *others) -> None:
@@ -77,17 +79,24 @@ def _workspace_bytes(aligned: bool, *args) -> int:
 
 def _linear_loss(hidden, weight, index, teacher, ignore_index, smoothing, z_loss, temperature, mean, scalar, row_grad,
                  want_dh, want_dw, chunk_rows):
-    """One call of po_linear_loss: (per-row losses or None, scalar loss or None, dhidden, dweight)."""
+    """One call of po_linear_loss: (per-row losses or None, scalar loss or None, dhidden, dweight, unscale).
+
+    ``unscale`` (or None): the factors that dhidden and dweight are still to be multiplied by.
+    """
     tokens, dim = hidden.shape
     vocab, top = weight.shape[0], index.shape[1]
     dev, dtype = hidden.device, hidden.dtype
     code, w_ptr, w_ld = _lib.DTYPE_CODE[dtype], weight.data_ptr(), _pitch(weight)
+    unscale = None
     with _lib.on_device(dev):
         nbytes = _workspace_bytes(w_ptr % 16 == 0, w_ld, code, tokens, dim, vocab, top, want_dh, want_dw, chunk_rows)
         if scalar:  # the per-row losses are the call's own: 4 bytes a row at the end of its workspace
             loss = torch.empty((), dtype=torch.float32, device=dev)
             ws = _lib.workspace(nbytes + 4 * tokens, dev)
             losses, rows_ptr = None, ws.data_ptr() + nbytes
+            if mean and dtype is torch.float16 and (want_dh or want_dw) and tokens:
+                mean, rows = _MEAN_SCALED, torch.empty(tokens + 2, dtype=torch.float32, device=dev)
+                rows_ptr, unscale = rows.data_ptr(), rows[tokens:]
         else:
             loss, losses = None, torch.empty(tokens, dtype=torch.float32, device=dev)
             ws, rows_ptr = _lib.workspace(nbytes, dev), losses.data_ptr()
@@ -105,21 +114,25 @@ def _linear_loss(hidden, weight, index, teacher, ignore_index, smoothing, z_loss
             ws.data_ptr(), nbytes, _lib.stream_ptr(dev))
         if status:
             _lib.check(status, "po_linear_loss")
-    return losses, loss, dh, dw
+    return losses, loss, dh, dw, unscale
 
 
 def _distill_logits(logits, index, teacher, temperature, mean, scalar, row_grad, want_grad):
-    """One call of po_distill_logits: (per-row losses or None, scalar loss or None, dlogits)."""
+    """One call of po_distill_logits: (per-row losses or None, scalar loss or None, dlogits, unscale), as above."""
     tokens, vocab = logits.shape
     dev, dtype = logits.device, logits.dtype
     with _lib.on_device(dev):
         lib = _lib.load()
         dz = logits.new_empty((tokens, vocab)) if want_grad else None
+        unscale = None
         if scalar:
             nbytes = (lib.po_distill_logits_workspace_bytes(tokens) + 15) // 16 * 16
             loss, losses = torch.empty((), dtype=torch.float32, device=dev), None
             ws = _lib.workspace(nbytes + 4 * tokens, dev)
             rows_ptr = ws.data_ptr() + nbytes
+            if mean and dtype is torch.float16 and want_grad and tokens:
+                mean, rows = _MEAN_SCALED, torch.empty(tokens + 1, dtype=torch.float32, device=dev)
+                rows_ptr, unscale = rows.data_ptr(), rows[tokens:]
         else:
             nbytes, ws, loss = 0, None, None
             losses = torch.empty(tokens, dtype=torch.float32, device=dev)
@@ -132,7 +145,7 @@ def _distill_logits(logits, index, teacher, temperature, mean, scalar, row_grad,
             _lib.stream_ptr(dev))
         if status:
             _lib.check(status, "po_distill_logits")
-    return losses, loss, dz
+    return losses, loss, dz, unscale
 
 
 def _upstream(up: torch.Tensor) -> torch.Tensor:
@@ -152,6 +165,15 @@ def _scale(factor: torch.Tensor, *grads) -> None:
                                                 factor.data_ptr(), _lib.stream_ptr(dev)), "po_scale_inplace")
 
 
+def _chain(up: torch.Tensor, unscale, *grads) -> None:
+    """Stored gradients to those of the upstream factor: fp16 ones of a mean each have a factor of their own."""
+    if unscale is None:
+        _scale(up, *grads)
+    else:
+        for factor, g in zip((up * unscale).unbind(), grads):
+            _scale(factor, g)
+
+
 def _records(*tensors) -> bool:
     """Whether autograd would record a function of these."""
     if torch.is_grad_enabled():
@@ -167,11 +189,11 @@ class _LinearLoss(torch.autograd.Function):
         reduction, chunk_rows, *terms = opts
         scalar = reduction != "none"
         want = ctx.needs_input_grad[:2] if scalar else (False, False)
-        losses, loss, dh, dw = _linear_loss(hidden, weight, index, teacher, *terms, reduction == "mean", scalar, None,
+        losses, loss, dh, dw, unscale = _linear_loss(hidden, weight, index, teacher, *terms, reduction == "mean", scalar, None,
                                             *want, chunk_rows)
         ctx.opts = opts
         if scalar:
-            ctx.grads = (dh, dw)
+            ctx.grads, ctx.unscale = (dh, dw), unscale
             return loss
         ctx.save_for_backward(hidden, weight, index, teacher)
         return losses
@@ -188,10 +210,10 @@ class _LinearLoss(torch.autograd.Function):
             if ctx.grads is None:
                 raise RuntimeError("the gradients of this loss were handed out already: one backward pass per loss")
             (dh, dw), ctx.grads = ctx.grads, None
-            _scale(up, dh, dw)
+            _chain(up, ctx.unscale, dh, dw)
             return dh, dw, None, None, None
         hidden, weight, index, teacher = ctx.saved_tensors
-        _, _, dh, dw = _linear_loss(hidden, weight, index, teacher, *terms, False, False, up, *ctx.needs_input_grad[:2],
+        _, _, dh, dw, _ = _linear_loss(hidden, weight, index, teacher, *terms, False, False, up, *ctx.needs_input_grad[:2],
                                     chunk_rows)
         return dh, dw, None, None, None
 
@@ -202,11 +224,11 @@ class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, index, teacher, reduction, temperature):
         scalar = reduction != "none"
-        losses, loss, dz = _distill_logits(logits, index, teacher, temperature, reduction == "mean", scalar, None,
+        losses, loss, dz, unscale = _distill_logits(logits, index, teacher, temperature, reduction == "mean", scalar, None,
                                            scalar and ctx.needs_input_grad[0])
         ctx.scalar, ctx.temperature = scalar, temperature
         if scalar:
-            ctx.grad = dz
+            ctx.grad, ctx.unscale = dz, unscale
             return loss
         ctx.save_for_backward(logits, index, teacher)
         return losses
@@ -222,7 +244,7 @@ class _Distillation(torch.autograd.Function):
             if ctx.grad is None:
                 raise RuntimeError("the gradient of this loss was handed out already: one backward pass per loss")
             dz, ctx.grad = ctx.grad, None
-            _scale(up, dz)
+            _chain(up, ctx.unscale, dz)
             return dz, None, None, None, None
         logits, index, teacher = ctx.saved_tensors
         return _distill_logits(logits, index, teacher, ctx.temperature, False, False, up, True)[2], None, None, None, None
@@ -236,7 +258,7 @@ def _head_loss(hidden, weight, index, teacher, reduction, chunk_rows, *terms):
     if _records(hidden, weight):
         out = _LinearLoss.apply(rows, head, index, teacher, (reduction, chunk_rows, *terms))
     else:
-        each, scalar, _, _ = _linear_loss(rows, head, index, teacher, *terms, reduction == "mean", reduction != "none",
+        each, scalar, *_ = _linear_loss(rows, head, index, teacher, *terms, reduction == "mean", reduction != "none",
                                           None, False, False, chunk_rows)
         out = each if scalar is None else scalar
     return out.reshape(lead) if reduction == "none" and len(lead) != 1 else out
@@ -333,7 +355,7 @@ def distillation(logits: torch.Tensor, teacher_index: torch.Tensor, teacher_logi
     if _records(logits):
         out = _Distillation.apply(rows, index, teacher, reduction, float(temperature))
     else:
-        each, mean, _ = _distill_logits(rows, index, teacher, float(temperature), reduction == "mean",
+        each, mean, *_ = _distill_logits(rows, index, teacher, float(temperature), reduction == "mean",
                                         reduction != "none", None, False)
         out = each if mean is None else mean
     return out.reshape(lead) if reduction == "none" and len(lead) != 1 else out

@@ -671,6 +671,40 @@ def test_distillation_empty():
     assert losses.distillation(z, i, t, reduction="none").shape == (0,)
 
 
+def test_fp16_gradients_of_a_mean_keep_their_digits_under_a_loss_scale():
+    """p / n is far below fp16's smallest value; a loss scale lifts it back, as with gradients made after it."""
+    T, D, V, K, up = 600, 64, 40000, 4, 2.0**14
+    h, w, y = _head(T, D, V, torch.float16)
+    want, dh, dw = ref_ce(h, w, y, up=torch.full((T,), up / T, device="cuda"))
+    h.requires_grad_(), w.requires_grad_()
+    gh, gw = _grads(losses.linear_cross_entropy(h, w, y) * up, h, w)
+    rare = torch.ones(V, dtype=torch.bool, device="cuda")
+    rare[y] = False  # rows of W that are nobody's target: p alone
+    assert _rel(gh, dh) < GRAD_TOL[h.dtype] and _rel(gw, dw) < GRAD_TOL[h.dtype]
+    assert float(dw[rare].abs().max()) / up < 2.0**-14 and _rel(gw[rare], dw[rare]) < 2.0**-7
+    z, index, teacher = (torch.randn(T, V, generator=_gen(5), device="cuda").half(), *_teacher(T, V, K, 6))
+    want, dz, counts = ref_distill(z, index, teacher, 2.0)
+    dz *= up / int(counts.sum())
+    z.requires_grad_()
+    gz, = _grads(losses.distillation(z, index, teacher, temperature=2.0) * up, z)
+    rest = torch.ones_like(z, dtype=torch.bool).scatter_(1, index.clamp(min=0), False)
+    assert _rel(gz, dz) < 2.0**-9 and _rel(gz[rest], dz[rest]) < 2.0**-8
+
+
+@pytest.mark.parametrize("size", [1.0, 40.0, 3000.0])
+def test_fp16_gradients_of_a_mean_stay_in_range(size):
+    """Every row the same large state and target: the largest gradients that states of this size can have."""
+    T, D, V = 500, 64, 300
+    h = torch.full((T, D), size, device="cuda", dtype=torch.float16)
+    w = torch.zeros(V, D, device="cuda", dtype=torch.float16)
+    w[1] = -0.25  # unlikely
+    y = torch.ones(T, dtype=torch.long, device="cuda")
+    want, dh, dw = ref_ce(h, w, y, up=torch.full((T,), 1 / T, device="cuda"))
+    h.requires_grad_(), w.requires_grad_()
+    gh, gw = _grads(losses.linear_cross_entropy(h, w, y), h, w)
+    assert _rel(gh, dh) < GRAD_TOL[h.dtype] and _rel(gw, dw) < GRAD_TOL[h.dtype]
+
+
 def test_scale_of_gradients_is_skipped_for_one():
     x = torch.randn(1001, device="cuda")
     lib = _lib.load()
