@@ -33,8 +33,8 @@ __host__ __device__ inline float split_cost(int s, int tiles, int nkb, float val
 
 // The split of dH's K is chosen again from the counted rows, which fill fewer
 // tiles than the rows the host knows of. A pass of 50257 x 768, the host's
-// choice against this one: bf16, 410 of 2048 rows 233 / 183 us, 410 of 1024 183
-// / 171, fp32, 400 of 1000 740 / 662; all rows counted: the same.
+// choice against this one: bf16, 410 of 2048 rows 233 / 186 us, 410 of 1024 186
+// / 176, fp32, 400 of 1000 757 / 680; all rows counted: the same.
 struct SplitArgs {
   int nkb;     // K blocks (0: the host's choice stays)
   int tiles_n, dim, pairs;

@@ -296,7 +296,8 @@ __global__ void __launch_bounds__(32 * kPackWarps) pack_kernel(PackArgs a, int g
         for (int u = 0; u < 4; ++u) {
           if (i0 + 32 * u >= n) continue;
           if (DT == PO_F16 && a.rowmax != nullptr) top = fmaxf(top, max_abs(v[u]));
-          if (DT == PO_F32) split_vec(v[u], reinterpret_cast<float4*>(dst) + i0 + 32 * u, reinterpret_cast<float4*>(lo) + i0 + 32 * u);
+          if (DT == PO_F32)
+            split_vec(v[u], reinterpret_cast<float4*>(dst) + i0 + 32 * u, reinterpret_cast<float4*>(lo) + i0 + 32 * u);
           else reinterpret_cast<uint4*>(dst)[i0 + 32 * u] = v[u];
         }
       }
@@ -575,24 +576,25 @@ __global__ void __launch_bounds__(256) join_kernel(const float* partial, int spl
   grid_wait();
   if (splits_at != nullptr) splits = *splits_at;
   if (limit_rows) M = min(M, *count - row0);
-  const int r = blockIdx.x;
-  if (r >= M || splits == 1) return;  // (one split wrote the output itself)
+  if (splits == 1) return;  // (it wrote the output itself)
   const float al = *alpha;
-  typename ElemOf<DT>::T* o =
-      static_cast<typename ElemOf<DT>::T*>(out) + (rows != nullptr ? rows[row0 + r] : r) * ld;
-  for (int c = (blockIdx.y * 256 + threadIdx.x) * 4; c < N; c += gridDim.y * 1024) {
-    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k = 0; k < splits; ++k) {
-      const float4 v = *reinterpret_cast<const float4*>(partial + (static_cast<long long>(k) * M + r) * pld + c);
-      s.x += v.x;
-      s.y += v.y;
-      s.z += v.z;
-      s.w += v.w;
-    }
-    const float x[4] = {s.x * al, s.y * al, s.z * al, s.w * al};
+  for (int r = blockIdx.x; r < M; r += gridDim.x) {
+    typename ElemOf<DT>::T* o =
+        static_cast<typename ElemOf<DT>::T*>(out) + (rows != nullptr ? rows[row0 + r] : r) * ld;
+    for (int c = (blockIdx.y * 256 + threadIdx.x) * 4; c < N; c += gridDim.y * 1024) {
+      float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int k = 0; k < splits; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(partial + (static_cast<long long>(k) * M + r) * pld + c);
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+      }
+      const float x[4] = {s.x * al, s.y * al, s.z * al, s.w * al};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c + i < N) from_f32(x[i], o[c + i]);
+      for (int i = 0; i < 4; ++i)
+        if (c + i < N) from_f32(x[i], o[c + i]);
+    }
   }
 }
 
@@ -769,11 +771,11 @@ int make_plan(Plan& p, const void* weight, long long w_ld, int dtype, long long 
   const auto blocks = [&](long long k) { return p.f32 ? cdiv(3LL * cdiv(k, p.bk), 2) : cdiv(k, p.bk); };
   p.splits_dh = want_dh ? choose_splits(mt * nd, blocks(V), p.chunk, D) : 1;
   // Fewer rows may count, and fewer tiles then take more splits: the finishing
-  // kernel chooses, within 256 KB a tile and split and four units a pair of SMs.
+  // kernel chooses, within 256 KB a tile and split and two units a pair of SMs.
   if (want_dh && mt > 1 && mt * nd <= 16 * (sm_count() / 2)) {
     p.dh_blocks = blocks(V);
     const long long units = mt * nd * p.splits_dh;
-    p.split_units = static_cast<int>(units > 4 * (sm_count() / 2) ? units : 4 * (sm_count() / 2));
+    p.split_units = static_cast<int>(units > 2 * (sm_count() / 2) ? units : 2 * (sm_count() / 2));
   }
   p.dw_acc = want_dw && p.nchunks > 1;
   p.splits_dw = want_dw && !p.dw_acc ? choose_splits(nv * nd, blocks(p.chunk), V, D) : 1;
@@ -817,12 +819,13 @@ int make_plan(Plan& p, const void* weight, long long w_ld, int dtype, long long 
   return ar.overflow() ? set_error(PO_ERR_WORKSPACE, "linear_loss: workspace too small") : PO_OK;
 }
 
-int join(int dtype, const float* alpha, const float* partial, int splits, const int* splits_at, int M, long long pld, int N, const Plan& p, int row0,
-         bool limit_rows, const int* rows, void* out, long long ld, cudaStream_t s) {
-  const dim3 grid(M, N > 4096 ? 4 : 1);
+int join(int dtype, const float* alpha, const float* partial, int splits, const int* splits_at, int M, long long pld,
+         int N, const Plan& p, int row0, bool limit_rows, const int* rows, void* out, long long ld, cudaStream_t s) {
+  // Blocks that fit at once: the launch costs little where there is one split.
+  const dim3 grid(M < 8 * sm_count() ? M : 8 * sm_count(), N > 4096 ? 4 : 1);
   const auto kern = dtype == PO_F32 ? join_kernel<PO_F32> : dtype == PO_BF16 ? join_kernel<PO_BF16> : join_kernel<PO_F16>;
-  return launch_next(false, kern, grid, 256, 0, s, "linear_loss join", partial, splits, splits_at, M, pld, N, alpha, &p.st->count,
-                     row0, limit_rows, rows, out, ld);
+  return launch_next(false, kern, grid, 256, 0, s, "linear_loss join", partial, splits, splits_at, M, pld, N, alpha,
+                     &p.st->count, row0, limit_rows, rows, out, ld);
 }
 
 int run_head(const Plan& p, int product, HeadParams& P, const HeadOperand& A, const HeadOperand& B, int splits,
