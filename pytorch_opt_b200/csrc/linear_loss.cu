@@ -894,12 +894,13 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
   if (tokens < 0 || dim <= 0 || vocab <= 0) return set_error(PO_ERR_ARG, "linear_loss: bad size");
   if (tokens > (1 << 26) || dim > (1 << 24) || vocab > (1 << 28))
     return set_error(PO_ERR_ARG, "linear_loss: size too large");
-  const bool soft = teacher != nullptr;
-  if (top < 1 || top > kMaxTop || (!soft && top != 1))
+  // An empty call reads no targets, and its teacher may have no address: it may be of either kind.
+  const bool soft = teacher != nullptr, hard = !soft && tokens > 0;
+  if (top < 1 || top > kMaxTop || (hard && top != 1))
     return set_error(PO_ERR_ARG, "linear_loss: top must be 1 to 1024 (1 without a teacher)");
   if (soft && teacher_dtype != PO_F32 && teacher_dtype != PO_BF16 && teacher_dtype != PO_F16)
     return set_error(PO_ERR_ARG, "linear_loss: teacher dtype must be fp32, bf16 or fp16");
-  if (!(temperature > 0.0f) || !std::isfinite(temperature) || (!soft && temperature != 1.0f))
+  if (!(temperature > 0.0f) || !std::isfinite(temperature) || (hard && temperature != 1.0f))
     return set_error(PO_ERR_ARG, "linear_loss: temperature must be positive (1 without a teacher)");
   if (!(smoothing >= 0.0f && smoothing <= 1.0f) || !std::isfinite(z_loss) || (soft && (smoothing != 0.0f || z_loss != 0.0f)))
     return set_error(PO_ERR_ARG, "linear_loss: smoothing must be in [0, 1] and z_loss finite (both 0 with a teacher)");

@@ -1,0 +1,17 @@
+"""Host-side checks of the loss operators at the edges of their arguments (no GPU)."""
+
+import ctypes
+
+import pytest
+
+from pytorch_opt_b200 import _lib
+
+P = ctypes.c_void_p(256)  # never followed: every call below is refused or empty
+
+
+@pytest.mark.parametrize("top,temperature", [(1, 1.0), (3, 1.0), (3, 2.0)])
+def test_linear_loss_abi_takes_an_empty_call_of_either_kind(top, temperature):
+    """No token, so no index, no hidden row, no teacher has an address, and nothing is left to launch."""
+    status = _lib.load().po_linear_loss(None, 8, P, 8, 0, 0, 8, 16, None, top, None, top, 0, top, -100, 0.0, 0.0,
+                                        temperature, 1, None, None, None, None, 8, None, 8, 0, None, 0, None)
+    assert status == 0, _lib.last_error()
