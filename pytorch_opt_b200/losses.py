@@ -19,8 +19,9 @@ reduction the gradients are made together with the loss (the softmax is not
 computed a second time) whenever an input requires grad (fp16 ones of a mean by
 powers of two, so that a loss scale does not come too late); with
 ``reduction="none"`` they are made in the backward pass from the upstream
-gradient of each row. Errors are ``RuntimeError`` as in ``native``; there is no
-CPU path.
+gradient of each row. Derivatives are first order and reverse mode only: a dual
+tensor of forward mode is refused. Errors are ``RuntimeError`` as in ``native``;
+there is no CPU path.
 """
 
 from __future__ import annotations
@@ -28,6 +29,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -175,7 +177,10 @@ def _chain(up: torch.Tensor, unscale, *grads) -> None:
 
 
 def _records(*tensors) -> bool:
-    """Whether autograd would record a function of these."""
+    """Whether the call goes through autograd's function: where it would be recorded, and inside a dual level, where
+    a tensor may carry a tangent without requires_grad (also under no_grad): the function refuses those."""
+    if forward_ad._current_level >= 0:
+        return True
     if torch.is_grad_enabled():
         for t in tensors:
             if t.requires_grad:

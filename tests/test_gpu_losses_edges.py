@@ -36,3 +36,22 @@ def test_linear_distillation_empty(top, temperature, reduction):
         assert loss.shape == (0,)
     else:
         assert float(loss.detach()) == 0.0
+
+
+def test_forward_mode_is_refused():
+    """No tangent is lost silently: a dual tensor without requires_grad is refused like any other."""
+    h, w, y = _head(20, 64, 300, torch.float32, seed=1)
+    index, teacher = _teacher(20, 300, 3, 2)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(h, torch.ones_like(h))
+        for reduction in ("mean", "none"):
+            for call in (lambda a: losses.linear_cross_entropy(a, w, y, reduction=reduction),
+                         lambda a: losses.linear_cross_entropy(h, torch.autograd.forward_ad.make_dual(w, w), y),
+                         lambda a: losses.linear_distillation(a, w, index, teacher, reduction=reduction),
+                         lambda a: losses.distillation(a, index.clamp(max=63), teacher, reduction=reduction)):
+                with pytest.raises(RuntimeError):  # (NotImplementedError is one)
+                    call(dual)
+                with torch.no_grad(), pytest.raises(RuntimeError):  # which does not stop forward mode
+                    call(dual)
+        plain = losses.linear_cross_entropy(h, w, y)  # no dual among its inputs
+    assert torch.equal(plain, losses.linear_cross_entropy(h, w, y))

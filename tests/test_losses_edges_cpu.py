@@ -3,8 +3,9 @@
 import ctypes
 
 import pytest
+import torch
 
-from pytorch_opt_b200 import _lib
+from pytorch_opt_b200 import _lib, losses
 
 P = ctypes.c_void_p(256)  # never followed: every call below is refused or empty
 
@@ -15,3 +16,12 @@ def test_linear_loss_abi_takes_an_empty_call_of_either_kind(top, temperature):
     status = _lib.load().po_linear_loss(None, 8, P, 8, 0, 0, 8, 16, None, top, None, top, 0, top, -100, 0.0, 0.0,
                                         temperature, 1, None, None, None, None, 8, None, 8, 0, None, 0, None)
     assert status == 0, _lib.last_error()
+
+
+def test_dual_tensors_go_through_autograd():
+    """Which refuses them; past it their tangent would be lost without a word."""
+    x = torch.ones(2)
+    assert not losses._records(x) and losses._records(x.clone().requires_grad_())
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        assert losses._records(torch.autograd.forward_ad.make_dual(x, x))
+    assert not losses._records(x)
