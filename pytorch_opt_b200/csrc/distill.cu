@@ -196,7 +196,9 @@ struct Segment {
 // In each of a row's CTAs
 //   the last warp takes the teacher's entries, their distribution and the
 //   logits there (three dependent loads, which would hold up the row if a
-//   warp with a share of the segment made them);
+//   warp with a share of the segment made them); whether the row has mass goes
+//   by the entries as they are, as in the counting kernel, and their maximum
+//   is subtracted before the scaling, as the student's is;
 //   the others run over their vectors of the segment (each thread its own)
 //   and hand each warp's (max, sum) to every CTA of the row;
 //   after one barrier of the row's CTAs every thread joins the row's pairs in
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__((GRAD ? kGradThreads : kEvalThreads) + 32, GRA
 #pragma unroll 4
     for (int k = lane; k < a.top; k += 32) {
       const long long x = a.index[t * a.index_ld + k];
-      const float l = load_as_f32(a.teacher, a.teacher_dtype, t * a.teacher_ld + k) * inv_temp;
+      const float l = load_as_f32(a.teacher, a.teacher_dtype, t * a.teacher_ld + k);
       const bool there = x >= 0 && x < a.V;
       bad |= x >= a.V;
       mass |= there && !(l == -INFINITY);
@@ -251,7 +253,7 @@ __global__ void __launch_bounds__((GRAD ? kGradThreads : kEvalThreads) + 32, GRA
     tm = warp_max(tm);
     float sum = 0.0f;
     for (int k = lane; k < a.top; k += 32) {
-      const float e = si[k] >= 0 ? expf(sq[k] - tm) : 0.0f;
+      const float e = si[k] >= 0 ? expf((sq[k] - tm) * inv_temp) : 0.0f;
       sum += e;
     }
     sum = warp_sum(sum);
@@ -260,8 +262,9 @@ __global__ void __launch_bounds__((GRAD ? kGradThreads : kEvalThreads) + 32, GRA
     for (int k = lane; k < a.top; k += 32) {
       float q = 0.0f;
       if (si[k] >= 0) {
-        q = expf(sq[k] - tm) * inv_sum;
-        if (q != 0.0f) c += q * (sq[k] - tm - logsum);
+        const float d = (sq[k] - tm) * inv_temp;
+        q = expf(d) * inv_sum;
+        if (q != 0.0f) c += q * (d - logsum);
       }
       sq[k] = q;
     }

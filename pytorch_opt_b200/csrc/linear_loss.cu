@@ -57,7 +57,9 @@ struct Targets {
 // ---------------------------------------------------------------- targets
 // One block a row: q = softmax(teacher / a) over the entries with index >= 0,
 // sum q log q, and (index, q) sorted by index (a bitonic network over `width`
-// = the next power of two; empty entries sort last as INT_MAX, q = 0).
+// = the next power of two; empty entries sort last as INT_MAX, q = 0). The
+// maximum is subtracted before the scaling: entries of the type's lowest value
+// stay finite at temperatures below 1, count, and share equally.
 __global__ void teacher_targets_kernel(Targets tg, long long V, float inv_temp, int width, int* status,
                                        int* ent, float* q, float* qlogq) {
   grid_launch_next();
@@ -77,7 +79,7 @@ __global__ void teacher_targets_kernel(Targets tg, long long V, float inv_temp, 
       if (x >= V) bad = true;
       else if (x >= 0) {
         i = static_cast<int>(x);
-        l = load_as_f32(tg.teacher, tg.teacher_dtype, t * tg.teacher_ld + k) * inv_temp;
+        l = load_as_f32(tg.teacher, tg.teacher_dtype, t * tg.teacher_ld + k);
         nan |= isnan(l);
       }
     }
@@ -91,16 +93,16 @@ __global__ void teacher_targets_kernel(Targets tg, long long V, float inv_temp, 
   const int st = bad ? ROW_BAD : (m > -INFINITY || nan ? ROW_COUNTED : ROW_IGNORED);
   float sum = 0.0f;
   for (int k = threadIdx.x; k < width; k += blockDim.x)
-    if (si[k] != INT_MAX) sum += expf(sl[k] - m);
+    if (si[k] != INT_MAX) sum += expf((sl[k] - m) * inv_temp);
   sum = block_sum(sum, buf);
   const float logsum = logf(sum);
   float c = 0.0f;
   for (int k = threadIdx.x; k < width; k += blockDim.x) {
     float p = 0.0f;
     if (si[k] != INT_MAX && st == ROW_COUNTED) {
-      const float lq = sl[k] - m - logsum;
-      p = expf(sl[k] - m) / sum;
-      if (p != 0.0f) c += p * lq;  // NaN passes
+      const float d = (sl[k] - m) * inv_temp;
+      p = expf(d) / sum;
+      if (p != 0.0f) c += p * (d - logsum);  // NaN passes
     }
     sl[k] = p;
   }

@@ -55,3 +55,33 @@ def test_forward_mode_is_refused():
                     call(dual)
         plain = losses.linear_cross_entropy(h, w, y)  # no dual among its inputs
     assert torch.equal(plain, losses.linear_cross_entropy(h, w, y))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("temperature", [0.5, 0.125, 2.0])
+def test_teacher_entries_of_the_lowest_value(dtype, temperature):
+    """Entries of the type's lowest value alone share equally at every temperature, and the row counts; beside
+    others they have no mass; -inf has none. Both forms agree on what a mean divides by."""
+    dt = DTYPES[dtype]
+    T, V, K = 6, 64, 4
+    z = torch.randn(T, V, generator=_gen(41), device="cuda")
+    index = torch.stack([torch.randperm(V, generator=_gen(s), device="cuda")[:K] for s in range(T)])
+    teacher = torch.randn(T, K, generator=_gen(42), device="cuda").to(dt)
+    teacher[0] = torch.finfo(dt).min
+    teacher[1, 1:] = torch.finfo(dt).min
+    teacher[2] = -math.inf
+    teacher[3, :2] = -math.inf
+    teacher[3, 2:] = torch.finfo(dt).min
+    teacher[4] = torch.finfo(dt).max
+    want, dz, counts = ref_distill(z, index, teacher, temperature)
+    assert counts.tolist() == [True, True, False, True, True, True]
+    n, eye = int(counts.sum()), torch.eye(V, device="cuda")
+    for form in (lambda a, r: losses.distillation(a, index, teacher, temperature=temperature, reduction=r),
+                 lambda a, r: losses.linear_distillation(a, eye, index, teacher, temperature=temperature, reduction=r)):
+        a = z.clone().requires_grad_()
+        rows = form(a, "none")
+        assert ((rows - want).abs() <= max(1.0, temperature**2) * 2.0**-16).all()
+        assert _rel(_grads(rows, a, up=torch.ones_like(rows))[0], dz) <= 2.0**-16
+        loss = form(a, "mean")
+        assert abs(float(loss.detach()) - float(want.sum()) / n) <= max(1.0, temperature**2) * 2.0**-16
+        assert _rel(_grads(loss, a)[0], dz / n) <= 2.0**-16
