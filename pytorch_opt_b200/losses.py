@@ -317,7 +317,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
         raise RuntimeError(f"{name}: label_smoothing must be in [0, 1] and z_loss finite")
     if chunk_rows < 0:
         raise RuntimeError(f"{name}: chunk_rows must not be negative")
-    return _head_loss(hidden, weight, target.long().reshape(-1, 1), None, reduction, int(chunk_rows),
+    return _head_loss(hidden, weight, _rows(target.long().reshape(-1, 1)), None, reduction, int(chunk_rows),
                       int(ignore_index), float(label_smoothing), float(z_loss), 1.0)
 
 

@@ -85,3 +85,19 @@ def test_teacher_entries_of_the_lowest_value(dtype, temperature):
         loss = form(a, "mean")
         assert abs(float(loss.detach()) - float(want.sum()) / n) <= max(1.0, temperature**2) * 2.0**-16
         assert _rel(_grads(loss, a)[0], dz / n) <= 2.0**-16
+
+
+def test_targets_of_one_value_expanded():
+    """A target that is a broadcast view, as a constant one often is."""
+    T, D, V = 37, 64, 300
+    h, w, _ = _head(T, D, V, torch.bfloat16, seed=3)
+    y = torch.full((1,), 7, device="cuda").expand(T)
+    want, dh, dw = ref_ce(h, w, y)
+    rows = losses.linear_cross_entropy(h, w, y, reduction="none")
+    assert ((rows - want).abs() <= _loss_bound(h, w)).all()
+    a = h.reshape(1, T, D).expand(2, T, D)
+    both = losses.linear_cross_entropy(a, w, y.expand(2, T).int(), reduction="none")
+    assert torch.equal(both[0], rows) and torch.equal(both[1], rows)
+    index, teacher = y[:1, None].expand(T, 1), torch.zeros(1, 1, device="cuda").expand(T, 1)
+    same = losses.linear_distillation(h, w, index, teacher, reduction="none")  # all mass on one entry
+    assert ((same - want).abs() <= _loss_bound(h, w) + 2.0**-17).all()
