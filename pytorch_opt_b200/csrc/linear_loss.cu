@@ -136,17 +136,6 @@ __global__ void teacher_targets_kernel(Targets tg, long long V, float inv_temp, 
   }
 }
 
-// max |row_grad| into state->grad_max (1 when there is nothing to scale by).
-__global__ void grad_max_kernel(const float* g, long long T, CallState* st) {
-  grid_launch_next();
-  grid_wait();
-  __shared__ float buf[32];
-  float m = 0.0f;
-  for (long long t = threadIdx.x; t < T; t += blockDim.x) m = fmaxf(m, fabsf(g[t]));
-  m = block_max(m, buf);
-  if (threadIdx.x == 0) st->grad_max = (m > 0.0f && m < INFINITY) ? m : 1.0f;
-}
-
 // ------------------------------------------------------------------- pack
 struct PackArgs {
   const void* hidden;
@@ -179,6 +168,23 @@ __device__ __forceinline__ int row_status(const PackArgs& a, long long t, int& t
   if (y < 0 || y >= a.V) return ROW_BAD;
   target = static_cast<int>(y);
   return ROW_COUNTED;
+}
+
+// Largest finite |row_grad| of the counted rows into state->grad_max (1 when
+// there is none): what stands beside the others, or one row's infinity, must not
+// move the scale that all counted rows are rounded at. One block.
+__global__ void grad_max_kernel(PackArgs a, const float* g) {
+  grid_launch_next();
+  grid_wait();
+  __shared__ float buf[32];
+  float m = 0.0f;
+  int y;
+  for (long long t = threadIdx.x; t < a.T; t += blockDim.x) {
+    const float x = fabsf(g[t]);
+    if (x < INFINITY && row_status(a, t, y) == ROW_COUNTED) m = fmaxf(m, x);
+  }
+  m = block_max(m, buf);
+  if (threadIdx.x == 0) a.st->grad_max = m > 0.0f ? m : 1.0f;
 }
 
 __device__ __forceinline__ float tf32_rna(float v) {
@@ -947,10 +953,6 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
       return r;
     first = false;
   }
-  if (row_grad != nullptr) {
-    if ((r = launch_next(first, grad_max_kernel, 1, 1024, 0, s, "linear_loss grad_max", row_grad, tokens, p.st))) return r;
-    first = false;
-  }
   const float gscale = dtype == PO_F16 ? kF16Scale : 1.0f;
   PackArgs pa{};
   pa.hidden = hidden, pa.h_ld = h_ld, pa.T = tokens, pa.D = D, pa.ldp = static_cast<int>(p.ldp);
@@ -961,6 +963,10 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
   pa.alpha = temperature / gscale, pa.mean = mean, pa.has_row_grad = row_grad != nullptr;
   float* unscale = mean == PO_MEAN_SCALED && p.grads ? loss_rows + tokens : nullptr;
   pa.unscale = unscale, pa.rowmax = unscale != nullptr && dtype == PO_F16 && !p.few ? p.rowmax : nullptr;
+  if (row_grad != nullptr) {
+    if ((r = launch_next(first, grad_max_kernel, 1, 1024, 0, s, "linear_loss grad_max", pa, row_grad))) return r;
+    first = false;
+  }
   const int groups = cdiv(T, 2048 * kPackWarps), pblocks = cdiv(T, groups * kPackWarps);
   const auto pack = dtype == PO_F32 ? pack_kernel<PO_F32> : dtype == PO_BF16 ? pack_kernel<PO_BF16> : pack_kernel<PO_F16>;
   if ((r = launch_next(first, pack, pblocks, 32 * kPackWarps, 0, s, "linear_loss pack", pa, groups))) return r;

@@ -101,3 +101,41 @@ def test_targets_of_one_value_expanded():
     index, teacher = y[:1, None].expand(T, 1), torch.zeros(1, 1, device="cuda").expand(T, 1)
     same = losses.linear_distillation(h, w, index, teacher, reduction="none")  # all mass on one entry
     assert ((same - want).abs() <= _loss_bound(h, w) + 2.0**-17).all()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan, 1e30])
+@pytest.mark.parametrize("form", ["ce", "distil"])
+def test_upstream_of_rows_that_count_for_nothing_is_not_looked_at(form, value, dtype):
+    """A division by a masked row's weight leaves anything as its upstream gradient."""
+    T, D, V = 70, 64, 300
+    dt = DTYPES[dtype]
+    h, w, y = _head(T, D, V, dt, seed=4)
+    up = 100.0 * torch.rand(T, generator=_gen(5), device="cuda")
+    index, teacher = _teacher(T, V, 4, 6, holes=False)
+    off = torch.zeros(T, dtype=torch.bool, device="cuda")
+    off[3::4] = True
+    y[off], index[off] = -100, -1
+    if form == "ce":
+        _, dh, dw = ref_ce(h, w, y, up=up)
+    else:
+        _, dz, _ = ref_distill(h.double() @ w.double().t(), index, teacher, 1.0, up)
+        dh, dw = dz @ w.double(), dz.t() @ h.double()
+    up[off] = value
+    h.requires_grad_(), w.requires_grad_()
+    rows = (losses.linear_cross_entropy(h, w, y, reduction="none") if form == "ce" else
+            losses.linear_distillation(h, w, index, teacher, reduction="none"))
+    gh, gw = _grads(rows, h, w, up=up)
+    assert _rel(gh, dh) <= GRAD_TOL[dt] and _rel(gw, dw) <= GRAD_TOL[dt]
+
+
+def test_upstream_of_one_row_that_is_infinite_stays_there():
+    T, D, V = 70, 64, 300
+    h, w, y = _head(T, D, V, torch.float16, seed=4)
+    up = 100.0 + torch.rand(T, generator=_gen(5), device="cuda")
+    _, dh, _ = ref_ce(h, w, y, up=up)
+    up[9] = math.inf
+    rest = torch.arange(T, device="cuda") != 9
+    h.requires_grad_()
+    gh, = _grads(losses.linear_cross_entropy(h, w, y, reduction="none"), h, up=up)
+    assert _rel(gh[rest], dh[rest]) <= GRAD_TOL[h.dtype] and not torch.isfinite(gh[9]).any()
