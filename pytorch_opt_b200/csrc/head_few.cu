@@ -103,9 +103,9 @@ __global__ void __launch_bounds__(kFewThreads, TT == 8 ? 4 : 0) few_rows_kernel(
   for (int r = warp; r < count; r += kFewThreads / 32) {
     const int c = 2 * lane, t = F.rowmap[r];
     const float z0 = n0 + c < P.V ? s_z[t][c] : -INFINITY, z1 = n0 + c + 1 < P.V ? s_z[t][c + 1] : -INFINITY;
-    const float m = warp_max(fmaxf(z0, z1)) * P.scale2;
+    const float m = warp_max(fmaxf(z0, z1));
     const float off = m == -INFINITY ? 0.0f : -m;
-    const float e0 = ex2(fmaf(z0, P.scale2, off)), e1 = ex2(fmaf(z1, P.scale2, off));
+    const float e0 = ex2((z0 + off) * P.scale2), e1 = ex2((z1 + off) * P.scale2);
     const float s = warp_sum(e0 + e1);
     const long long at = static_cast<long long>(r) * F.nparts + blockIdx.x;
     if (lane == 0) P.part[at] = make_float2(m, s);

@@ -54,7 +54,7 @@ struct FinishArgs {
   const float* qlogq;
   int top;
   float smoothing, z_loss, temperature, inv_vocab, scale2;
-  float4* stat;        // [row of this launch] max, 1 / sum, log2 sum 2^z2
+  float4* stat;        // [row of this launch] max, 1 / sum, log sum exp at temperature 1
   float* loss_rows;
   float* loss;         // nullable; written by the last block of the last launch
   long long T;
@@ -68,8 +68,9 @@ struct FinishArgs {
   int row_words;
 };
 
-// One warp: log2 sum 2^z2 of a packed row from its partial statistics, and its
-// loss. (Loads bypass L1: other SMs wrote, perhaps in this launch.)
+// One warp: maximum and sum of a packed row from its partial statistics, and its
+// loss. The statistics' maxima are the logits' own; a difference of two logits
+// is scaled, never a logit. (Loads bypass L1: other SMs wrote, perhaps in this launch.)
 __device__ __forceinline__ void finish_row(const FinishArgs& a, int row, int lane) {
   const float2* p = a.part + static_cast<long long>(row) * a.nparts;
   float m = -INFINITY, s = 0.0f;
@@ -83,16 +84,16 @@ __device__ __forceinline__ void finish_row(const FinishArgs& a, int row, int lan
       c = fmaxf(c, v[u].x);
     }
     if (c > m) {
-      s *= ex2(m - c);
+      s *= ex2((m - c) * a.scale2);
       m = c;
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      s += v[u].x == -INFINITY ? v[u].y : v[u].y * ex2(v[u].x - m);  // an empty part holds 0, or a NaN to keep
+      s += v[u].x == -INFINITY ? v[u].y : v[u].y * ex2((v[u].x - m) * a.scale2);  // an empty part holds 0, or a NaN to keep
   }
   const float mm = warp_max(m);
-  s = warp_sum(m == -INFINITY ? s : s * ex2(m - mm));
-  const float log2s = log2f(s), lse2 = mm + log2s;
+  s = warp_sum(m == -INFINITY ? s : s * ex2((m - mm) * a.scale2));
+  const float logs = kLn2 * log2f(s), lse = mm + logs;
   const long long t = a.rowmap[a.row0 + row];
   float zs = 0.0f;
   if (a.zsum != nullptr) {
@@ -101,20 +102,20 @@ __device__ __forceinline__ void finish_row(const FinishArgs& a, int row, int lan
   }
   float loss;
   if (a.q == nullptr) {
-    const float lse = lse2 * kLn2, zy = __ldcg(a.zpick + t);
-    loss = kLn2 * (log2s - fmaf(zy, a.scale2, -mm)) + a.z_loss * lse * lse;
+    const float zy = __ldcg(a.zpick + t);
+    loss = logs + (mm - zy) + a.z_loss * lse * lse;
     if (a.smoothing != 0.0f) loss += a.smoothing * (zy - zs * a.inv_vocab);
   } else {
     float c = 0.0f;
     for (int k = lane; k < a.top; k += 32) {
       const float q = a.q[t * a.top + k];
-      if (q != 0.0f) c += q * (log2s - fmaf(__ldcg(a.zpick + t * a.top + k), a.scale2, -mm));
+      if (q != 0.0f) c += q * (logs + (mm - __ldcg(a.zpick + t * a.top + k)) / a.temperature);
     }
     c = warp_sum(c);
-    loss = a.temperature * a.temperature * (a.qlogq[t] + kLn2 * c);
+    loss = a.temperature * a.temperature * (a.qlogq[t] + c);
   }
   if (lane == 0) {
-    a.stat[row] = make_float4(mm, 1.0f / s, lse2, 0.0f);
+    a.stat[row] = make_float4(mm, 1.0f / s, lse, 0.0f);
     a.loss_rows[t] = loss;
   }
 }

@@ -75,15 +75,15 @@ struct alignas(64) HeadParams {
   int* err;
   // HEAD_STATS
   float scale2;       // log2(e) / temperature
-  float2* part;       // [row][nparts] (max, sum of 2^(z2 - max)) over 256 columns, z2 = scale2 * logit
+  float2* part;       // [row][nparts] (max, sum of 2^(scale2 (z - max))) over 256 columns, z the logits
   int nparts;
   float* zsum;        // [row][nparts] sum of the logits (nullable)
-  void* e;            // [row][e_ld] 2^(z2 - max) (nullable)
+  void* e;            // [row][e_ld] 2^(scale2 (z - max)) (nullable)
   long long e_ld;
   const int* rowmap;  // packed row -> row of the call
   const int* ent;     // [row of the call][top] ascending target indices
   int top;
-  float* zpick;       // [row of the call][top] logits at those indices, scaled only with the maximum taken off
+  float* zpick;       // [row of the call][top] logits at those indices
   // HEAD_STORE
   const float* alpha;  // device scalar
   const float* cin;    // fp32, added to row r (nullable)
@@ -335,13 +335,15 @@ __device__ __forceinline__ void stats_epilogue(const HeadParams& P, float (&x)[H
   // The four warps of this lane quarter share the row's maximum over the tile.
   share[group * 32 + lane] = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
   bar_sync(1 + q, 128);
-  const float m = fmaxf(fmaxf(share[lane], share[32 + lane]), fmaxf(share[64 + lane], share[96 + lane])) * P.scale2;
+  const float m = fmaxf(fmaxf(share[lane], share[32 + lane]), fmaxf(share[64 + lane], share[96 + lane]));
+  // The maximum is subtracted before the scaling: exact where it matters, and
+  // neither logits near the type's limit nor low temperatures overflow.
   const float off = m == -INFINITY ? 0.0f : -m;
   uint64_t sum2[2] = {0, 0};
   const uint64_t scale2 = pack2(P.scale2, P.scale2), off2 = pack2(off, off);
 #pragma unroll
   for (int j = 0; j < HC; j += 2) {
-    const float2 a = unpack2(fma2(pack2(x[j], x[j + 1]), scale2, off2));
+    const float2 a = unpack2(mul2(add2(pack2(x[j], x[j + 1]), off2), scale2));
     x[j] = ex2(a.x);
     x[j + 1] = ex2(a.y);
     sum2[(j / 2) & 1] = add2(sum2[(j / 2) & 1], pack2(x[j], x[j + 1]));

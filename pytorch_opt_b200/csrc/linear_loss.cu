@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
   const float4 stat = a.stat[row];
   const float mm = stat.x;
   const float w = a.scale * (a.row_grad != nullptr ? a.row_grad[t] / a.st->grad_max : 1.0f);
-  const float coef = w * (1.0f + 2.0f * a.z_loss * kLn2 * stat.z);
+  const float coef = w * (1.0f + 2.0f * a.z_loss * stat.z);
   const float pcoef = coef * stat.y;
   const float flat = w * a.smoothing * a.inv_vocab;
   const float2* part = a.part + static_cast<long long>(row) * a.nparts;
@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
 #pragma unroll 2
     for (int c = c0 + threadIdx.x * 4; c < c1; c += 256 * 4) {
       const float m = part[c / a.part_cols].x;
-      const float f = m == -INFINITY ? (pcoef == pcoef ? 0.0f : pcoef) : pcoef * ex2(m - mm);
+      const float f = m == -INFINITY ? (pcoef == pcoef ? 0.0f : pcoef) : pcoef * ex2((m - mm) * a.scale2);
       const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(a.e) + base + c);
       const float x[4] = {fmaf(v.x, f, -flat), fmaf(v.y, f, -flat), fmaf(v.z, f, -flat), fmaf(v.w, f, -flat)};
       float4 h, l;
@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
       const int c = c0 + (i * 256 + static_cast<int>(threadIdx.x)) * 8;
       if (c >= c1) break;
       const float m = ms[i];
-      const float f = m == -INFINITY ? (pcoef == pcoef ? 0.0f : pcoef) : pcoef * ex2(m - mm);
+      const float f = m == -INFINITY ? (pcoef == pcoef ? 0.0f : pcoef) : pcoef * ex2((m - mm) * a.scale2);
       const __half2* hv = reinterpret_cast<const __half2*>(&raw[i]);
       uint32_t o[4];
 #pragma unroll
@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
     if (a.q == nullptr) goal = 1.0f - a.smoothing;
     else
       for (int j = k; j < a.top && ent[j] == c; ++j) goal += a.q[t * a.top + j];
-    put_dz<DT>(a, base + c, pcoef * ex2(fmaf(a.zpick[t * a.top + k], a.scale2, -mm)) - flat - w * goal);
+    put_dz<DT>(a, base + c, pcoef * ex2((a.zpick[t * a.top + k] - mm) * a.scale2) - flat - w * goal);
   }
 }
 

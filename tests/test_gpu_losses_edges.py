@@ -139,3 +139,35 @@ def test_upstream_of_one_row_that_is_infinite_stays_there():
     h.requires_grad_()
     gh, = _grads(losses.linear_cross_entropy(h, w, y, reduction="none"), h, up=up)
     assert _rel(gh[rest], dh[rest]) <= GRAD_TOL[h.dtype] and not torch.isfinite(gh[9]).any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("copies", [1, 5])  # up to two rows (eight in fp32) go to the CUDA cores
+@pytest.mark.parametrize("temperature", [1.0, 0.5])
+def test_linear_logits_near_the_largest_value(temperature, copies, dtype):
+    """Finite logits of 3e38 at temperature 1 and 1.5e38 at 0.5: only differences from the row's maximum are scaled."""
+    dt = DTYPES[dtype]
+    V = 96
+    big = 3e38 * temperature
+    z = torch.zeros(2, V, device="cuda")
+    z[0] = -big                                  # masked throughout: equal shares
+    z[1, :4], z[1, 4:] = big, torch.randn(V - 4, generator=_gen(51), device="cuda")
+    z = z.repeat(copies, 1).to(dt)
+    y = torch.tensor([3, 1], device="cuda").repeat(copies)
+    want = torch.tensor([math.log(V), math.log(4.0)], dtype=torch.float64, device="cuda").repeat(copies)
+    p = torch.zeros(2, V, dtype=torch.float64, device="cuda")
+    p[0], p[1, :4] = 1 / V, 0.25
+    dz = p.repeat(copies, 1)
+    dz[torch.arange(2 * copies), y] -= 1
+    eye = torch.eye(V, device="cuda", dtype=dt)
+    index, teacher = y[:, None], torch.zeros(2 * copies, 1, device="cuda")  # all mass on the target
+    calls = [lambda a, r: losses.linear_distillation(a, eye, index, teacher, temperature=temperature, reduction=r)]
+    if temperature == 1.0:
+        calls.append(lambda a, r: losses.linear_cross_entropy(a, eye, y, reduction=r))
+    for call in calls:
+        a = z.clone().requires_grad_()
+        rows = call(a, "none")
+        # log and exponentials of equal logits: a few roundings of numbers below 8, times a^2.
+        assert ((rows - temperature**2 * want).abs() <= 2.0**-20).all()
+        assert _rel(_grads(rows, a, up=torch.ones_like(rows))[0], temperature * dz) <= GRAD_TOL[dt]
+        assert _rel(_grads(call(a, "sum"), a)[0], temperature * dz) <= GRAD_TOL[dt]
