@@ -290,7 +290,7 @@ int po_matmul(const void* A, long long lda, long long sa, int trans_a, const voi
  *   dz = (1 + 2 z_loss lse(z)) softmax(z) - (1 - s) onehot(y) - s / vocab
  * Rows with y == ignore_index count for nothing.
  * A teacher's top logits (teacher != NULL), over the entries k of the row
- * with index[t][k] >= 0, a = temperature:
+ * with index[t][k] >= 0, a = temperature (2^-60 to 2^60):
  *   q  = softmax(teacher / a)
  *   l  = a^2 sum_k q_k (log q_k - log softmax(z / a)[i_k])
  *   dz = a (softmax(z / a) - q scattered to i)

@@ -908,8 +908,8 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
     return set_error(PO_ERR_ARG, "linear_loss: top must be 1 to 1024 (1 without a teacher)");
   if (soft && teacher_dtype != PO_F32 && teacher_dtype != PO_BF16 && teacher_dtype != PO_F16)
     return set_error(PO_ERR_ARG, "linear_loss: teacher dtype must be fp32, bf16 or fp16");
-  if (!(temperature > 0.0f) || !std::isfinite(temperature) || (hard && temperature != 1.0f))
-    return set_error(PO_ERR_ARG, "linear_loss: temperature must be positive (1 without a teacher)");
+  if (!temperature_ok(temperature) || (hard && temperature != 1.0f))
+    return set_error(PO_ERR_ARG, "linear_loss: temperature must be 2^-60 to 2^60 (1 without a teacher)");
   if (!(smoothing >= 0.0f && smoothing <= 1.0f) || !std::isfinite(z_loss) || (soft && (smoothing != 0.0f || z_loss != 0.0f)))
     return set_error(PO_ERR_ARG, "linear_loss: smoothing must be in [0, 1] and z_loss finite (both 0 with a teacher)");
   if (row_grad != nullptr && (mean || (dhidden == nullptr && dweight == nullptr)))

@@ -170,6 +170,10 @@ int launch_next(bool first, void (*kern)(Params...), dim3 grid, int block, size_
   return check_cuda(cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...), what);
 }
 
+// Temperatures a teacher's form takes: a^2 (the loss's factor) and log2(e) / a
+// (the exponents') are ordinary fp32 numbers.
+inline bool temperature_ok(float a) { return a >= 0x1p-60f && a <= 0x1p60f; }
+
 // What a row is to the loss.
 enum RowStatus : int { ROW_IGNORED = 0, ROW_COUNTED = 1, ROW_BAD = 2 };
 

@@ -288,8 +288,8 @@ def _check_teacher(name: str, lead, index: torch.Tensor, teacher: torch.Tensor, 
                            f"{tuple(index.shape)} and {tuple(teacher.shape)} for {tuple(lead)}")
     if not 1 <= index.shape[-1] <= MAX_TOP:
         raise RuntimeError(f"{name}: 1 to {MAX_TOP} entries a token, got {index.shape[-1]}")
-    if not (temperature > 0 and temperature < float("inf")):
-        raise RuntimeError(f"{name}: temperature must be positive, got {temperature}")
+    if not 2.0**-60 <= temperature <= 2.0**60:  # its square and its reciprocal are fp32 numbers
+        raise RuntimeError(f"{name}: temperature must be 2^-60 to 2^60, got {temperature}")
     return _rows(index.long()), _rows(teacher.detach() if teacher.requires_grad else teacher)
 
 

@@ -171,3 +171,17 @@ def test_linear_logits_near_the_largest_value(temperature, copies, dtype):
         assert ((rows - temperature**2 * want).abs() <= 2.0**-20).all()
         assert _rel(_grads(rows, a, up=torch.ones_like(rows))[0], temperature * dz) <= GRAD_TOL[dt]
         assert _rel(_grads(call(a, "sum"), a)[0], temperature * dz) <= GRAD_TOL[dt]
+
+
+def test_temperatures_whose_square_has_no_fp32():
+    """Losses have the factor a^2 and exponents 1 / a: beyond 2^-60 .. 2^60 one of them leaves fp32's range."""
+    h, w, _ = _head(4, 8, 16, torch.bfloat16)
+    i, t = torch.zeros(4, 2, dtype=torch.long, device="cuda"), torch.zeros(4, 2, device="cuda")
+    for a in (1e-39, 2.0**-61, 2.0**61, 1e30):
+        with pytest.raises(RuntimeError, match="temperature"):
+            losses.linear_distillation(h, w, i, t, temperature=a)
+        with pytest.raises(RuntimeError, match="temperature"):
+            losses.distillation(torch.randn(4, 16, device="cuda"), i, t, temperature=a)
+    for a in (2.0**-60, 2.0**60):
+        assert torch.isfinite(losses.linear_distillation(h, w, i, t, temperature=a))
+        assert torch.isfinite(losses.distillation(torch.randn(4, 16, device="cuda"), i, t, temperature=a))

@@ -25,3 +25,14 @@ def test_dual_tensors_go_through_autograd():
     with torch.autograd.forward_ad.dual_level(), torch.no_grad():
         assert losses._records(torch.autograd.forward_ad.make_dual(x, x))
     assert not losses._records(x)
+
+
+@pytest.mark.parametrize("temperature", [0.0, -1.0, float("nan"), float("inf"), 1e-39, 2.0**-61, 2.0**61])
+def test_abi_refuses_temperatures_outside_fp32(temperature):
+    lib = _lib.load()
+    assert lib.po_linear_loss(P, 8, P, 8, 0, 4, 8, 16, P, 2, P, 2, 0, 2, -100, 0.0, 0.0, temperature, 1, None, P, P,
+                              None, 8, None, 8, 0, P, 1 << 30, None) == 1
+    assert "temperature" in _lib.last_error()
+    assert lib.po_distill_logits(P, 16, 0, 4, 16, P, 2, P, 2, 0, 2, temperature, 1, None, P, P, None, 16, P, 8,
+                                 None) == 1
+    assert "temperature" in _lib.last_error()
