@@ -15,9 +15,13 @@ struct CallState {
   int count;         // counted rows
   int counted_mean;  // rows that the mean divides by
   int done;          // blocks of the finishing launch that are through
-  float alpha;       // factor of the gradient products
-  float alpha_dh, alpha_dw;  // the same, with the power of two that each is stored by
+  float alpha;       // the upstream factor that all rows share
+  float alpha_dh, alpha_dw;  // the products' factors: it, with the powers of two of operand and result
   float grad_max;    // max |row_grad|
+  // fp16 gradients:
+  float coef_max;    // largest |1 + 2 z_loss lse| of the rows finished so far, 1 at least
+  float store_dh, store_dw;  // powers of two that the gradients of a mean are stored by (0: not chosen yet)
+  float redo_dh, redo_dw;    // what earlier launches' gradients are multiplied by to agree with these
   int splits;        // of K in the next dH product
 };
 
@@ -60,9 +64,6 @@ struct FinishArgs {
   long long T;
   int mean, final_launch;
   CallState* st;
-  const float* rowmax;  // fp16, scaled gradients (else null): max |h| of each packed row
-  float* unscale;       // receives the inverses of the powers of two
-  float margin;         // what else may make dZ larger than softmax
   uint4* packed;       // 16-byte words of H's packed rows of this launch (and of their low halves, nullable)
   uint4* packed_lo;
   int row_words;
@@ -115,6 +116,9 @@ __device__ __forceinline__ void finish_row(const FinishArgs& a, int row, int lan
     loss = a.temperature * a.temperature * (a.qlogq[t] + c);
   }
   if (lane == 0) {
+    // (fp16 operands are scaled by it; a row without a finite one has no finite gradient)
+    const float coef = fabsf(1.0f + 2.0f * a.z_loss * lse);
+    if (a.z_loss != 0.0f && coef < INFINITY) atomicMax(reinterpret_cast<int*>(&a.st->coef_max), __float_as_int(coef));
     a.stat[row] = make_float4(mm, 1.0f / s, lse, 0.0f);
     a.loss_rows[t] = loss;
   }

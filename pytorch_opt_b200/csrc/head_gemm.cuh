@@ -88,6 +88,7 @@ struct alignas(64) HeadParams {
   const float* alpha;  // device scalar
   const float* cin;    // fp32, added to row r (nullable)
   long long cin_ld;
+  const float* cin_scale;  // device scalar that cin is multiplied by (nullable)
   void* out;           // row r of the product goes to out row (rows ? rows[row0 + r] : r)
   long long out_ld;
   int out_dtype;       // PO_F32 / PO_BF16 / PO_F16
@@ -400,19 +401,20 @@ __device__ __forceinline__ void store_epilogue(const HeadParams& P, float (&x)[H
   }
   if (P.cin != nullptr && live) {
     const float* ci = P.cin + static_cast<long long>(row) * P.cin_ld + n0;
+    const float cs = P.cin_scale != nullptr ? *P.cin_scale : 1.0f;
     if (P.vec && ncols == HC) {
 #pragma unroll
       for (int j = 0; j < HC; j += 4) {
         const float4 f = *reinterpret_cast<const float4*>(ci + j);
-        x[j] += f.x;
-        x[j + 1] += f.y;
-        x[j + 2] += f.z;
-        x[j + 3] += f.w;
+        x[j] = fmaf(f.x, cs, x[j]);
+        x[j + 1] = fmaf(f.y, cs, x[j + 1]);
+        x[j + 2] = fmaf(f.z, cs, x[j + 2]);
+        x[j + 3] = fmaf(f.w, cs, x[j + 3]);
       }
     } else {
 #pragma unroll
       for (int j = 0; j < HC; ++j)
-        if (j < ncols) x[j] += ci[j];
+        if (j < ncols) x[j] = fmaf(ci[j], cs, x[j]);
     }
   }
   const bool bf = P.out_dtype == PO_BF16;

@@ -39,10 +39,14 @@
 namespace po {
 namespace {
 
-// Values of the fp16 gradient operand are 2^10 of dZ / upstream: |dZ| is at
-// most 1 + 2 z_loss lse, and softmax values down to 6e-8 stay normal. bf16
-// and tf32 have fp32's range and need no factor.
-constexpr float kF16Scale = 1024.0f;
+// The fp16 gradient operand is dZ / upstream times this power of two: |dZ| is at
+// most 1 + |1 + 2 z_loss lse|, whose largest second term is `coef`; 2^10 keeps
+// softmax values down to 6e-8 normal, and a large z-loss takes less (60000 leaves
+// fp16's range a margin for the logarithm's rounding). bf16 and tf32 have fp32's
+// range and need no factor.
+__device__ __forceinline__ float f16_scale(float coef) {
+  return fminf(1024.0f, exp2f(floorf(log2f(60000.0f / (coef + 1.0f)))));
+}
 
 struct Targets {
   const long long* index;
@@ -335,6 +339,8 @@ __global__ void __launch_bounds__(32 * kPackWarps) pack_kernel(PackArgs a, int g
     if (a.mean) alpha /= static_cast<float>(all > 0 ? all : 1);
     if (a.has_row_grad) alpha *= a.st->grad_max;
     a.st->alpha = a.st->alpha_dh = a.st->alpha_dw = alpha;
+    a.st->coef_max = 1.0f;
+    a.st->store_dh = a.st->store_dw = 0.0f;
     if (a.unscale != nullptr) a.unscale[0] = a.unscale[1] = 1.0f;
   }
 }
@@ -411,26 +417,6 @@ __device__ __forceinline__ void choose_splits(const FinishArgs& a, int left, int
   if (lane == 0) a.st->splits = best;
 }
 
-// One block: the powers of two that fp16 gradients of a mean are stored by. A
-// mean's gradients may lie below fp16's range until the caller's loss scale
-// lifts them, which comes after the rounding here. With dZ's row at most 2 in
-// sum of magnitudes, |dH| <= 2 max|W| / n and |dW| <= 2 max|h|: neither leaves
-// the range by its factor (n / 2 at most, and half the room that max|h| leaves).
-__device__ __forceinline__ void choose_scales(const FinishArgs& a, float* buf) {
-  float top = 0.0f;
-  for (int i = threadIdx.x; i < a.st->count; i += blockDim.x) top = fmaxf(top, a.rowmax[i]);
-  top = fmaxf(block_max(top, buf), 1e-4f) * a.margin;
-  if (threadIdx.x != 0) return;
-  const int n = a.st->counted_mean;
-  const float dh = n > 1 ? exp2f(floorf(log2f(static_cast<float>(n) / a.margin)) - 1.0f) : 1.0f;
-  const float dw = exp2f(floorf(log2f(16384.0f / top)));
-  const float sh = fminf(fmaxf(dh, 1.0f), 65536.0f), sw = fminf(fmaxf(dw, 1.0f), 65536.0f);
-  a.st->alpha_dh = a.st->alpha * sh;
-  a.st->alpha_dw = a.st->alpha * sw;
-  a.unscale[0] = 1.0f / sh;
-  a.unscale[1] = 1.0f / sw;
-}
-
 __global__ void __launch_bounds__(32 * kFinishWarps) finish_kernel(FinishArgs a) {
   grid_launch_next();
   grid_wait();
@@ -442,7 +428,6 @@ __global__ void __launch_bounds__(32 * kFinishWarps) finish_kernel(FinishArgs a)
   if (row < left && row < a.rows) finish_row(a, row, lane);
   else if (left > 0 && row < (left + kRowPad - 1) / kRowPad * kRowPad && row < (a.rows + kRowPad - 1) / kRowPad * kRowPad)
     zero_row(a, row, lane);
-  if (a.rowmax != nullptr && blockIdx.x == 0) choose_scales(a, reinterpret_cast<float*>(dbuf));
   if (a.split.nkb > 0 && blockIdx.x == 0 && threadIdx.x < 32) choose_splits(a, left, lane);
   if (a.loss == nullptr || !a.final_launch) return;
   __threadfence();
@@ -470,8 +455,11 @@ struct RescaleArgs {
   const float* zpick;
   int top;
   const float* row_grad;  // nullable
-  float smoothing, z_loss, inv_vocab, scale, scale2;
-  const CallState* st;
+  float smoothing, z_loss, inv_vocab, scale2;
+  const float* rowmax;  // fp16 gradients of a mean (else null): max |h| of each packed row
+  float* unscale;       // receives the inverses of the powers of two
+  float room;           // max(temperature, 1)
+  CallState* st;
 };
 
 constexpr int kSegment = 8192;  // columns a block rescales
@@ -489,6 +477,52 @@ __device__ __forceinline__ void put_dz(const RescaleArgs& a, long long off, floa
   }
 }
 
+// One block: the factors of the fp16 products, and the powers of two that
+// gradients of a mean are stored by. A mean's gradients may lie below fp16's
+// range until the caller's loss scale lifts them, which comes after the rounding
+// here. With dZ's row at most 2 m in sum of magnitudes, m = coef_max times room,
+// |dH| <= 2 m max|W| / n and |dW| <= 2 m max|h|: neither leaves the range by its
+// factor (n / 2m at most, and half the room that max|h| leaves). Where a later
+// chunk of rows has a larger coef, the factors shrink, and what earlier chunks
+// left is multiplied by redo_dh and redo_dw.
+__device__ __forceinline__ void choose_scales(const RescaleArgs& a, float* buf) {
+  CallState& st = *a.st;
+  const float m = a.room * st.coef_max;
+  float sh = 1.0f, sw = 1.0f;
+  if (a.rowmax != nullptr) {
+    float top = 0.0f;
+    for (int i = threadIdx.x; i < st.count; i += blockDim.x) top = fmaxf(top, a.rowmax[i]);
+    top = fmaxf(block_max(top, buf), 1e-4f) * m;
+    const float n = static_cast<float>(st.counted_mean);
+    sh = fminf(fmaxf(exp2f(floorf(log2f(n / m)) - 1.0f), 1.0f), 65536.0f);
+    sw = fminf(fmaxf(exp2f(floorf(log2f(16384.0f / top))), 1.0f), 65536.0f);
+  }
+  if (threadIdx.x != 0) return;
+  const bool fresh = st.store_dh == 0.0f;
+  if (!fresh) sh = fminf(sh, st.store_dh), sw = fminf(sw, st.store_dw);
+  st.redo_dh = fresh ? 1.0f : sh / st.store_dh;
+  st.redo_dw = fresh ? 1.0f : sw / st.store_dw;
+  st.store_dh = sh, st.store_dw = sw;
+  const float alpha = st.alpha / f16_scale(st.coef_max);
+  st.alpha_dh = alpha * sh;
+  st.alpha_dw = alpha * sw;
+  if (a.rowmax != nullptr) a.unscale[0] = 1.0f / sh, a.unscale[1] = 1.0f / sw;
+}
+
+// dH rows of earlier chunks brought to the factor of this one.
+__global__ void __launch_bounds__(256) redo_rows_kernel(const CallState* st, const int* rowmap, int row0, __half* dh,
+                                                        long long ld, int D) {
+  grid_launch_next();
+  grid_wait();
+  const float f = st->redo_dh;
+  if (f == 1.0f) return;
+  const int rows = min(row0, st->count), lane = threadIdx.x & 31;
+  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) {
+    __half* x = dh + rowmap[r] * ld;
+    for (int i = lane; i < D; i += 32) x[i] = __float2half_rn(__half2float(x[i]) * f);
+  }
+}
+
 // dZ = w ((1 + 2 c lse) p - s/V - target distribution), w the row's share of
 // the upstream gradient; the constant upstream factor is in the products'
 // alpha, so that rounding dZ to 16 bits sees w = 1 in all but the per-row
@@ -497,6 +531,8 @@ template <int DT>
 __global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
   grid_launch_next();
   grid_wait();
+  __shared__ float buf[32];
+  if (DT == PO_F16 && blockIdx.x == 0) choose_scales(a, buf);
   const int row = blockIdx.x / nseg;
   const int seg = blockIdx.x - row * nseg;
   const int left = a.st->count - a.row0;
@@ -511,7 +547,8 @@ __global__ void __launch_bounds__(256) rescale_kernel(RescaleArgs a, int nseg) {
   const long long t = a.rowmap[a.row0 + row];
   const float4 stat = a.stat[row];
   const float mm = stat.x;
-  const float w = a.scale * (a.row_grad != nullptr ? a.row_grad[t] / a.st->grad_max : 1.0f);
+  const float w =
+      (DT == PO_F16 ? f16_scale(a.st->coef_max) : 1.0f) * (a.row_grad != nullptr ? a.row_grad[t] / a.st->grad_max : 1.0f);
   const float coef = w * (1.0f + 2.0f * a.z_loss * stat.z);
   const float pcoef = coef * stat.y;
   const float flat = w * a.smoothing * a.inv_vocab;
@@ -953,14 +990,13 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
       return r;
     first = false;
   }
-  const float gscale = dtype == PO_F16 ? kF16Scale : 1.0f;
   PackArgs pa{};
   pa.hidden = hidden, pa.h_ld = h_ld, pa.T = tokens, pa.D = D, pa.ldp = static_cast<int>(p.ldp);
   pa.vec = D * p.es % 16 == 0 && reinterpret_cast<uintptr_t>(hidden) % 16 == 0 && h_ld * p.es % 16 == 0;
   pa.tg = tg, pa.V = vocab, pa.status = p.status, pa.ent = p.ent, pa.rowmap = p.rowmap;
   pa.packed = p.packed, pa.packed_lo = p.packed_lo;
   pa.dhidden = dhidden, pa.dh_ld = dh_ld, pa.loss_rows = loss_rows, pa.st = p.st, pa.sched = p.sched;
-  pa.alpha = temperature / gscale, pa.mean = mean, pa.has_row_grad = row_grad != nullptr;
+  pa.alpha = temperature, pa.mean = mean, pa.has_row_grad = row_grad != nullptr;
   float* unscale = mean == PO_MEAN_SCALED && p.grads ? loss_rows + tokens : nullptr;
   pa.unscale = unscale, pa.rowmax = unscale != nullptr && dtype == PO_F16 && !p.few ? p.rowmax : nullptr;
   if (row_grad != nullptr) {
@@ -1004,8 +1040,6 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
       fa.row_words = static_cast<int>(p.ldp * p.es / 16);
     }
     fa.rows = rows;
-    fa.rowmax = pa.rowmax, fa.unscale = unscale;
-    fa.margin = fmaxf(temperature, 1.0f) * (1.0f + 128.0f * fabsf(z_loss));
     if (p.split_units > 0) fa.split = {p.dh_blocks, cdiv(D, 256), D, sm_count() / 2, p.split_units};
     if (p.few) {
       FewParams P{};
@@ -1039,7 +1073,8 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
     ra.e = p.e, ra.lo = p.e_lo, ra.e_ld = p.e_ld, ra.V = vocab, ra.part = p.part, ra.nparts = p.nparts, ra.part_cols = p.part_cols, ra.stat = p.stat;
     ra.row0 = static_cast<int>(row0), ra.rows = rows, ra.rowmap = p.rowmap, ra.ent = p.ent, ra.q = soft ? p.q : nullptr;
     ra.scale2 = kLog2e / temperature, ra.zpick = p.zpick, ra.top = static_cast<int>(top), ra.row_grad = row_grad, ra.smoothing = smoothing;
-    ra.z_loss = z_loss, ra.inv_vocab = 1.0f / static_cast<float>(vocab), ra.scale = gscale, ra.st = p.st;
+    ra.z_loss = z_loss, ra.inv_vocab = 1.0f / static_cast<float>(vocab), ra.st = p.st;
+    ra.rowmax = pa.rowmax, ra.unscale = unscale, ra.room = fmaxf(temperature, 1.0f);
     const int nseg = cdiv(p.e_ld, kSegment);
     const long long rblocks = krows * nseg;
     if (rblocks > INT_MAX) return set_error(PO_ERR_ARG, "linear_loss: chunk too large");
@@ -1048,6 +1083,11 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
     if ((r = launch_next(false, rescale, static_cast<int>(rblocks), 256, 0, s, "linear_loss rescale", ra, nseg))) return r;
 
     const long long pld = round_up(dim, 256);
+    const bool redo = pa.rowmax != nullptr && z_loss != 0.0f && c > 0;  // (without a z-loss the factors stay)
+    if (redo && p.want_dh &&
+        (r = launch_next(false, redo_rows_kernel, sms, 256, 0, s, "linear_loss redo", p.st, p.rowmap,
+                         static_cast<int>(row0), static_cast<__half*>(dhidden), dh_ld, D)))
+      return r;
     if (p.want_dh) {
       HeadParams P;
       memset(&P, 0, sizeof(P));
@@ -1075,6 +1115,7 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
       const long long acc_ld = to_acc ? round_up(dim, 8) : dw_ld;
       P.cin = p.dw_acc && c > 0 ? acc : nullptr;
       P.cin_ld = acc_ld;
+      P.cin_scale = redo ? &p.st->redo_dw : nullptr;
       const bool mid = to_acc && !last;
       P.out = mid ? static_cast<void*>(acc) : dweight;
       P.out_ld = mid ? acc_ld : dw_ld;

@@ -185,3 +185,42 @@ def test_temperatures_whose_square_has_no_fp32():
     for a in (2.0**-60, 2.0**60):
         assert torch.isfinite(losses.linear_distillation(h, w, i, t, temperature=a))
         assert torch.isfinite(losses.distillation(torch.randn(4, 16, device="cuda"), i, t, temperature=a))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("T,chunk", [(2, 0), (300, 0), (900, 0), (900, 256)])
+@pytest.mark.parametrize("z_loss,top,shared", [(0.5, 120.0, 0.25), (2.0, 250.0, 4.0), (-0.5, 120.0, 0.25)])
+def test_fp16_gradients_of_a_large_z_loss(z_loss, top, shared, T, chunk, reduction):
+    """(1 + 2 c lse) softmax reaches a thousand times softmax, later rows the most; the gradients fit fp16."""
+    D, V = 64, 500
+    h, w, y = _head(T, D, V, torch.float16, seed=T, scale=0.5)
+    w[:, 0] = shared
+    h[:, 0] = torch.linspace(2.0, top, T, device="cuda") / shared  # adds 2 .. top to every logit of a row
+    w[:, 1] = 0
+    w[:7, 1] = 2.0
+    h[:, 1] = 4.0                                             # and 8 to seven of them: some p are large
+    y[5::9] = -100
+    n = int((y != -100).sum())
+    up = torch.full((T,), 1 / n if reduction == "mean" else 2.0**-6, device="cuda")
+    want, dh, dw = ref_ce(h, w, y, 0.0, z_loss, -100, up)
+    assert max(float(dh.abs().max()), float(dw.abs().max())) < 60000
+    h.requires_grad_(), w.requires_grad_()
+    loss = losses.linear_cross_entropy(h, w, y, z_loss=z_loss, reduction=reduction, chunk_rows=chunk)
+    if reduction == "none":
+        gh, gw = _grads(loss, h, w, up=up)
+    else:
+        gh, gw = _grads(loss, h, w, up=torch.tensor(1.0 if reduction == "mean" else 2.0**-6, device="cuda"))
+    assert _rel(gh, dh) <= GRAD_TOL[h.dtype] and _rel(gw, dw) <= GRAD_TOL[h.dtype]
+
+
+def test_fp16_gradients_of_a_large_z_loss_under_a_loss_scale():
+    """As without z-loss, rare rows of W keep their digits until the loss scale comes, in chunks or not."""
+    T, D, V, up = 600, 64, 20000, 2.0**10
+    h, w, y = _head(T, D, V, torch.float16)
+    w[:, 0] = 1.0
+    h[:, 0] = torch.linspace(0.0, 90.0, T, device="cuda")
+    _, dh, dw = ref_ce(h, w, y, 0.0, 0.5, -100, torch.full((T,), up / T, device="cuda"))
+    h.requires_grad_(), w.requires_grad_()
+    for chunk in (0, 256):
+        gh, gw = _grads(losses.linear_cross_entropy(h, w, y, z_loss=0.5, chunk_rows=chunk) * up, h, w)
+        assert _rel(gh, dh) < GRAD_TOL[h.dtype] and _rel(gw, dw) < GRAD_TOL[h.dtype]
