@@ -998,7 +998,7 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
   pa.dhidden = dhidden, pa.dh_ld = dh_ld, pa.loss_rows = loss_rows, pa.st = p.st, pa.sched = p.sched;
   pa.alpha = temperature, pa.mean = mean, pa.has_row_grad = row_grad != nullptr;
   float* unscale = mean == PO_MEAN_SCALED && p.grads ? loss_rows + tokens : nullptr;
-  pa.unscale = unscale, pa.rowmax = unscale != nullptr && dtype == PO_F16 && !p.few ? p.rowmax : nullptr;
+  pa.unscale = unscale, pa.rowmax = unscale != nullptr && dtype == PO_F16 ? p.rowmax : nullptr;
   if (row_grad != nullptr) {
     if ((r = launch_next(first, grad_max_kernel, 1, 1024, 0, s, "linear_loss grad_max", pa, row_grad))) return r;
     first = false;

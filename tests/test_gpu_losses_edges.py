@@ -224,3 +224,17 @@ def test_fp16_gradients_of_a_large_z_loss_under_a_loss_scale():
     for chunk in (0, 256):
         gh, gw = _grads(losses.linear_cross_entropy(h, w, y, z_loss=0.5, chunk_rows=chunk) * up, h, w)
         assert _rel(gh, dh) < GRAD_TOL[h.dtype] and _rel(gw, dw) < GRAD_TOL[h.dtype]
+
+
+@pytest.mark.parametrize("T", [1, 2])
+def test_fp16_gradients_of_few_rows_keep_their_digits_under_a_loss_scale(T):
+    """As those of many: rows of W that are nobody's target have p h, far below fp16's smallest normal value."""
+    D, V, up = 64, 128256, 2.0**16
+    h, w, y = _head(T, D, V, torch.float16, seed=9, scale=0.1)
+    _, dh, dw = ref_ce(h, w, y, up=torch.full((T,), up / T, device="cuda"))
+    h.requires_grad_(), w.requires_grad_()
+    gh, gw = _grads(losses.linear_cross_entropy(h, w, y) * up, h, w)
+    rare = torch.ones(V, dtype=torch.bool, device="cuda")
+    rare[y] = False
+    assert _rel(gh, dh) < GRAD_TOL[h.dtype] and _rel(gw, dw) < GRAD_TOL[h.dtype]
+    assert _rel(gw[rare], dw[rare]) < 2.0**-7
