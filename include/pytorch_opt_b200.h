@@ -312,16 +312,18 @@ int po_matmul(const void* A, long long lda, long long sa, int trans_a, const voi
  * dweight (pitch dw_ld), nullable, receive the gradients of that loss in
  * `dtype`; with row_grad (fp32 [tokens], nullable) the gradients of
  * sum_t row_grad[t] l_t instead (`mean` must be 0).
- * `mean` PO_MEAN_SCALED: the gradients are stored multiplied by powers of two
- * chosen from the data, so that fp16 ones keep their digits until a loss scale
- * is applied; loss_rows then has two more elements, which receive the inverse
- * factors of dhidden and dweight (one, of dlogits, from po_distill_logits).
+ * `mean` PO_MEAN_SCALED, or PO_SUM_SCALED for the sum: the gradients are stored
+ * multiplied by powers of two chosen from the data, so that fp16 ones keep their
+ * digits until a loss scale is applied, and those of a sum stay in range until
+ * the caller's division; loss_rows then has two more elements, which receive the
+ * inverse factors of dhidden and dweight (PO_MEAN_SCALED of po_distill_logits:
+ * one more, of dlogits; it has no PO_SUM_SCALED).
  * The logits are never stored: without gradients each tile of them (256
  * columns, 64 for a few rows) leaves two numbers a row; with gradients at most chunk_rows rows at a time (0: a
  * default by the workspace it takes) leave their scaled exponentials in the
  * workspace, in 16 bits (32 for fp32).
  * ---------------------------------------------------------------------- */
-enum { PO_MEAN_SCALED = 2 };
+enum { PO_MEAN_SCALED = 2, PO_SUM_SCALED = 3 };
 size_t po_linear_loss_workspace_bytes(const void* weight, long long w_ld, int dtype, long long tokens, long long dim,
                                       long long vocab, long long top, int want_dhidden, int want_dweight,
                                       long long chunk_rows);

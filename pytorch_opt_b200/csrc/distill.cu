@@ -472,6 +472,7 @@ extern "C" int po_distill_logits(const void* logits, long long ld, int dtype, lo
   if (top < 1 || top > kMaxTop) return set_error(PO_ERR_ARG, "distill_logits: top must be 1 to 1024");
   if (!temperature_ok(temperature))
     return set_error(PO_ERR_ARG, "distill_logits: temperature must be 2^-60 to 2^60");
+  if (mean == PO_SUM_SCALED) return set_error(PO_ERR_ARG, "distill_logits: gradients of a sum need no scaling");
   if (row_grad != nullptr && (mean || dlogits == nullptr))
     return set_error(PO_ERR_ARG, "distill_logits: row_grad goes with gradients of the sum");
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -456,9 +456,10 @@ struct RescaleArgs {
   int top;
   const float* row_grad;  // nullable
   float smoothing, z_loss, inv_vocab, scale2;
-  const float* rowmax;  // fp16 gradients of a mean (else null): max |h| of each packed row
+  const float* rowmax;  // fp16 gradients of a scalar (else null): max |h| of each packed row
   float* unscale;       // receives the inverses of the powers of two
   float room;           // max(temperature, 1)
+  int mean;
   CallState* st;
 };
 
@@ -478,11 +479,13 @@ __device__ __forceinline__ void put_dz(const RescaleArgs& a, long long off, floa
 }
 
 // One block: the factors of the fp16 products, and the powers of two that
-// gradients of a mean are stored by. A mean's gradients may lie below fp16's
-// range until the caller's loss scale lifts them, which comes after the rounding
-// here. With dZ's row at most 2 m in sum of magnitudes, m = coef_max times room,
-// |dH| <= 2 m max|W| / n and |dW| <= 2 m max|h|: neither leaves the range by its
-// factor (n / 2m at most, and half the room that max|h| leaves). Where a later
+// gradients of a scalar are stored by. A mean's gradients may lie below fp16's
+// range until the caller's loss scale lifts them, a sum's above it until the
+// caller's division, and both come after the rounding here. With dZ's row at
+// most 2 m in sum of magnitudes, m = coef_max times room, the mean's have
+// |dH| <= 2 m max|W| / n and |dW| <= 2 m max|h|, the sum's n times as much:
+// neither leaves the range by its factor (dH's takes 2 m / n away, a sum's m;
+// dW's leaves half of what max|h| and a sum's n do). Where a later
 // chunk of rows has a larger coef, the factors shrink, and what earlier chunks
 // left is multiplied by redo_dh and redo_dw.
 __device__ __forceinline__ void choose_scales(const RescaleArgs& a, float* buf) {
@@ -494,8 +497,13 @@ __device__ __forceinline__ void choose_scales(const RescaleArgs& a, float* buf) 
     for (int i = threadIdx.x; i < st.count; i += blockDim.x) top = fmaxf(top, a.rowmax[i]);
     top = fmaxf(block_max(top, buf), 1e-4f) * m;
     const float n = static_cast<float>(st.counted_mean);
-    sh = fminf(fmaxf(exp2f(floorf(log2f(n / m)) - 1.0f), 1.0f), 65536.0f);
-    sw = fminf(fmaxf(exp2f(floorf(log2f(16384.0f / top))), 1.0f), 65536.0f);
+    if (a.mean) {
+      sh = fminf(fmaxf(exp2f(floorf(log2f(n / m)) - 1.0f), 1.0f), 65536.0f);
+      sw = fminf(fmaxf(exp2f(floorf(log2f(16384.0f / top))), 1.0f), 65536.0f);
+    } else {
+      sh = fmaxf(exp2f(floorf(log2f(1.0f / m))), 0x1p-40f);
+      sw = fminf(fmaxf(exp2f(floorf(log2f(16384.0f / (top * fmaxf(n, 1.0f))))), 0x1p-40f), 1.0f);
+    }
   }
   if (threadIdx.x != 0) return;
   const bool fresh = st.store_dh == 0.0f;
@@ -949,6 +957,7 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
     return set_error(PO_ERR_ARG, "linear_loss: temperature must be 2^-60 to 2^60 (1 without a teacher)");
   if (!(smoothing >= 0.0f && smoothing <= 1.0f) || !std::isfinite(z_loss) || (soft && (smoothing != 0.0f || z_loss != 0.0f)))
     return set_error(PO_ERR_ARG, "linear_loss: smoothing must be in [0, 1] and z_loss finite (both 0 with a teacher)");
+  const bool scaled = mean == PO_MEAN_SCALED || mean == PO_SUM_SCALED;
   if (row_grad != nullptr && (mean || (dhidden == nullptr && dweight == nullptr)))
     return set_error(PO_ERR_ARG, "linear_loss: row_grad goes with gradients of the sum");
   if (h_ld < dim || w_ld < dim || (tokens > 1 && (index_ld < top || (soft && teacher_ld < top))) ||
@@ -956,6 +965,7 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
     return set_error(PO_ERR_ARG, "linear_loss: a pitch is smaller than its row");
   if (weight == nullptr || (tokens > 0 && (hidden == nullptr || index == nullptr || loss_rows == nullptr)))
     return set_error(PO_ERR_ARG, "linear_loss: null operand");
+  if (mean == PO_SUM_SCALED) mean = 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int sms = sm_count();
   if (tokens == 0) {
@@ -997,7 +1007,7 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
   pa.packed = p.packed, pa.packed_lo = p.packed_lo;
   pa.dhidden = dhidden, pa.dh_ld = dh_ld, pa.loss_rows = loss_rows, pa.st = p.st, pa.sched = p.sched;
   pa.alpha = temperature, pa.mean = mean, pa.has_row_grad = row_grad != nullptr;
-  float* unscale = mean == PO_MEAN_SCALED && p.grads ? loss_rows + tokens : nullptr;
+  float* unscale = scaled && p.grads ? loss_rows + tokens : nullptr;
   pa.unscale = unscale, pa.rowmax = unscale != nullptr && dtype == PO_F16 ? p.rowmax : nullptr;
   if (row_grad != nullptr) {
     if ((r = launch_next(first, grad_max_kernel, 1, 1024, 0, s, "linear_loss grad_max", pa, row_grad))) return r;
@@ -1074,7 +1084,7 @@ extern "C" int po_linear_loss(const void* hidden, long long h_ld, const void* we
     ra.row0 = static_cast<int>(row0), ra.rows = rows, ra.rowmap = p.rowmap, ra.ent = p.ent, ra.q = soft ? p.q : nullptr;
     ra.scale2 = kLog2e / temperature, ra.zpick = p.zpick, ra.top = static_cast<int>(top), ra.row_grad = row_grad, ra.smoothing = smoothing;
     ra.z_loss = z_loss, ra.inv_vocab = 1.0f / static_cast<float>(vocab), ra.st = p.st;
-    ra.rowmax = pa.rowmax, ra.unscale = unscale, ra.room = fmaxf(temperature, 1.0f);
+    ra.rowmax = pa.rowmax, ra.unscale = unscale, ra.room = fmaxf(temperature, 1.0f), ra.mean = mean;
     const int nseg = cdiv(p.e_ld, kSegment);
     const long long rblocks = krows * nseg;
     if (rblocks > INT_MAX) return set_error(PO_ERR_ARG, "linear_loss: chunk too large");

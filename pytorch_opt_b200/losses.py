@@ -16,8 +16,8 @@ Three functions of CUDA tensors (bf16, fp16 or fp32), differentiable by
 Rows that count for nothing (``ignore_index``, no teacher's entry) have loss
 and gradient 0, are left out of the mean, and cost no product. With a scalar
 reduction the gradients are made together with the loss (the softmax is not
-computed a second time) whenever an input requires grad (fp16 ones of a mean by
-powers of two, so that a loss scale does not come too late); with
+computed a second time) whenever an input requires grad (fp16 ones by powers of
+two, so that neither a loss scale nor a division of the sum comes too late); with
 ``reduction="none"`` they are made in the backward pass from the upstream
 gradient of each row. Derivatives are first order and reverse mode only: a dual
 tensor of forward mode is refused. Errors are ``RuntimeError`` as in ``native``;
@@ -36,7 +36,7 @@ from . import _lib
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _REDUCTIONS = ("mean", "sum", "none")
 MAX_TOP = 1024
-_MEAN_SCALED = 2  # PO_MEAN_SCALED
+_MEAN_SCALED, _SUM_SCALED = 2, 3  # PO_MEAN_SCALED, PO_SUM_SCALED
 
 
 def _check_tensors(name: str, first, *others) -> None:
@@ -96,8 +96,8 @@ def _linear_loss(hidden, weight, index, teacher, ignore_index, smoothing, z_loss
             loss = torch.empty((), dtype=torch.float32, device=dev)
             ws = _lib.workspace(nbytes + 4 * tokens, dev)
             losses, rows_ptr = None, ws.data_ptr() + nbytes
-            if mean and dtype is torch.float16 and (want_dh or want_dw) and tokens:
-                mean, rows = _MEAN_SCALED, torch.empty(tokens + 2, dtype=torch.float32, device=dev)
+            if dtype is torch.float16 and (want_dh or want_dw) and tokens:
+                mean, rows = _MEAN_SCALED if mean else _SUM_SCALED, torch.empty(tokens + 2, dtype=torch.float32, device=dev)
                 rows_ptr, unscale = rows.data_ptr(), rows[tokens:]
         else:
             loss, losses = None, torch.empty(tokens, dtype=torch.float32, device=dev)
@@ -168,7 +168,7 @@ def _scale(factor: torch.Tensor, *grads) -> None:
 
 
 def _chain(up: torch.Tensor, unscale, *grads) -> None:
-    """Stored gradients to those of the upstream factor: fp16 ones of a mean each have a factor of their own."""
+    """Stored gradients to those of the upstream factor: fp16 ones each have a factor of their own."""
     if unscale is None:
         _scale(up, *grads)
     else:

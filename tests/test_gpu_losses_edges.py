@@ -187,7 +187,7 @@ def test_temperatures_whose_square_has_no_fp32():
         assert torch.isfinite(losses.distillation(torch.randn(4, 16, device="cuda"), i, t, temperature=a))
 
 
-@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 @pytest.mark.parametrize("T,chunk", [(2, 0), (300, 0), (900, 0), (900, 256)])
 @pytest.mark.parametrize("z_loss,top,shared", [(0.5, 120.0, 0.25), (2.0, 250.0, 4.0), (-0.5, 120.0, 0.25)])
 def test_fp16_gradients_of_a_large_z_loss(z_loss, top, shared, T, chunk, reduction):
@@ -238,3 +238,23 @@ def test_fp16_gradients_of_few_rows_keep_their_digits_under_a_loss_scale(T):
     rare[y] = False
     assert _rel(gh, dh) < GRAD_TOL[h.dtype] and _rel(gw, dw) < GRAD_TOL[h.dtype]
     assert _rel(gw[rare], dw[rare]) < 2.0**-7
+
+
+@pytest.mark.parametrize("form", ["ce", "distil"])
+@pytest.mark.parametrize("T", [2, 600, 4000])
+def test_fp16_gradients_of_a_sum_divided_afterwards_stay_in_range(T, form):
+    """loss_sum / n: the sum's own gradient of a frequent target's row may lie beyond fp16, the mean's does not."""
+    D, V = 64, 100
+    h = torch.full((T, D), 80000.0 / T if T > 2 else 40000.0, device="cuda", dtype=torch.float16)
+    w = torch.zeros(V, D, device="cuda", dtype=torch.float16)
+    y = torch.ones(T, dtype=torch.long, device="cuda")
+    _, dh, dw = ref_ce(h, w, y, up=torch.full((T,), 1 / T, device="cuda"))
+    assert float(dw.abs().max()) * T > 65504 > float(dw.abs().max())
+    h.requires_grad_(), w.requires_grad_()
+    for chunk in (0, 256):
+        loss = (losses.linear_cross_entropy(h, w, y, reduction="sum", chunk_rows=chunk) if form == "ce" else
+                losses.linear_distillation(h, w, y[:, None], torch.zeros(T, 1, device="cuda"), reduction="sum",
+                                           chunk_rows=chunk))
+        gh, gw = _grads(loss / T, h, w)
+        assert torch.isfinite(gw).all() and _rel(gw, dw) <= GRAD_TOL[h.dtype]
+        assert float(gh.abs().max()) == 0.0  # W is 0
