@@ -759,7 +759,7 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_gemm_kernel(const __grid
   }
 }
 
-// The tile counts here are upper bounds: the kernel reads the real extent.
+// `max_tiles` is an upper bound of tiles times splits: the kernel reads the real extent.
 template <int KIND, bool A_MN, bool B_MN, int EPI>
 int launch_head(const HeadParams& P, int max_tiles, cudaStream_t stream) {
   using C = HeadCfg<KIND>;

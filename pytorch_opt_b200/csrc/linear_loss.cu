@@ -894,7 +894,9 @@ int run_head(const Plan& p, int product, HeadParams& P, const HeadOperand& A, co
   P.splits = splits;
   P.tiles_n = cdiv(P.N, 256);
   const int tiles_m = cdiv(P.M, 256);
-  const long long tiles = static_cast<long long>(tiles_m) * P.tiles_n * splits;
+  // (splits chosen on the device may make more units of fewer tiles: as many as their workspace holds)
+  long long tiles = static_cast<long long>(tiles_m) * P.tiles_n * splits;
+  if (P.splits_at != nullptr && tiles < p.split_units) tiles = p.split_units;
   if (tiles > INT_MAX / 2) return set_error(PO_ERR_ARG, "linear_loss: too many tiles");
   return p.f32 ? dispatch_head<KIND_TF32>(product, P, static_cast<int>(tiles), s)
                : dispatch_head<KIND_BF16>(product, P, static_cast<int>(tiles), s);

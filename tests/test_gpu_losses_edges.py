@@ -258,3 +258,28 @@ def test_fp16_gradients_of_a_sum_divided_afterwards_stay_in_range(T, form):
         gh, gw = _grads(loss / T, h, w)
         assert torch.isfinite(gw).all() and _rel(gw, dw) <= GRAD_TOL[h.dtype]
         assert float(gh.abs().max()) == 0.0  # W is 0
+
+
+def test_splits_chosen_on_the_device_have_the_whole_gpu(tmp_path):
+    """Half of the rows count, so dH's 32 tiles take two splits or more: their launch has a pair of SMs for each
+    unit, although the host, which knows of 60 tiles, splits nothing."""
+    import json
+
+    T, D, V = 3840, 1024, 20000
+    h, w, y = _head(T, D, V, torch.bfloat16, seed=8)
+    y[::2] = -100
+    _, dh, _ = ref_ce(h, w, y)
+    h.requires_grad_()
+    loss = lambda: losses.linear_cross_entropy(h, w, y, reduction="sum")  # noqa: E731
+    gh, = _grads(loss(), h)
+    assert _rel(gh, dh) <= GRAD_TOL[h.dtype]
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        loss()
+        torch.cuda.synchronize()
+    prof.export_chrome_trace(str(tmp_path / "trace.json"))
+    events = json.loads((tmp_path / "trace.json").read_text())["traceEvents"]
+    heads = sorted((e["ts"], e["args"]["grid"][0]) for e in events
+                   if e.get("cat") == "kernel" and "head_gemm_kernel" in e["name"])
+    assert len(heads) == 2  # logits, dH
+    pairs = torch.cuda.get_device_properties(0).multi_processor_count // 2
+    assert heads[1][1] >= 2 * min(pairs, 64)
