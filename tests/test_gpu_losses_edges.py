@@ -283,3 +283,91 @@ def test_splits_chosen_on_the_device_have_the_whole_gpu(tmp_path):
     assert len(heads) == 2  # logits, dH
     pairs = torch.cuda.get_device_properties(0).multi_processor_count // 2
     assert heads[1][1] >= 2 * min(pairs, 64)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("form", ["ce", "linear", "logits"])
+def test_gradients_under_graph_capture(form, reduction, dtype):
+    """A step's loss and gradients captured once, replayed on other inputs."""
+    T, D, V, K = 100, 64, 1000, 5
+    dt = DTYPES[dtype]
+
+    def inputs(seed):
+        h, w, y = _head(T, D, V, dt, seed=seed)
+        y[seed % 7::7] = -100
+        return [h, w, y, *_teacher(T, V, K, seed), torch.rand(T, generator=_gen(seed), device="cuda")]
+
+    at = inputs(18)
+    h, w, y, index, teacher, up = at
+    leaves = [h.clone().requires_grad_(), w.clone().requires_grad_()]
+    z = (h @ w.t()).requires_grad_()
+
+    def step():
+        if form == "logits":
+            loss, xs = losses.distillation(z, index, teacher, reduction=reduction), [z]
+        elif form == "ce":
+            loss, xs = losses.linear_cross_entropy(*leaves, y, reduction=reduction), leaves
+        else:
+            loss, xs = losses.linear_distillation(*leaves, index, teacher, reduction=reduction), leaves
+        return (loss, *_grads(loss, *xs, up=up if reduction == "none" else None))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (19, 20):
+        with torch.no_grad():
+            for a, b in zip(at, inputs(seed)):
+                a.copy_(b)
+            leaves[0].copy_(h), leaves[1].copy_(w), z.copy_(h @ w.t())
+        graph.replay()
+        torch.cuda.synchronize()
+        n = int((y != -100).sum()) if form == "ce" else int((index >= 0).any(1).sum())
+        u = up if reduction == "none" else torch.full((T,), 1 / n, device="cuda")
+        if form == "ce":
+            want, dh, dw = ref_ce(h, w, y, up=u)
+        else:
+            zz = z.detach().double() if form == "logits" else h.double() @ w.double().t()
+            want, dz, _ = ref_distill(zz, index, teacher, 1.0, u)
+            dh, dw = dz @ w.double(), dz.t() @ h.double()
+        bound = _loss_bound(h, w) + 2.0**-17
+        if reduction == "none":
+            assert ((got[0].detach() - want).abs() <= bound).all()
+        else:
+            assert abs(float(got[0].detach()) - float(want.sum()) / n) <= float(bound.max())
+        grads = (dz,) if form == "logits" else (dh, dw)
+        for a, b in zip(got[1:], grads):
+            assert _rel(a, b) <= GRAD_TOL[dt]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("soft", [False, True])
+def test_masked_rows_among_many(soft, dtype):
+    """More than 16384 rows: a packing block takes several groups of eight."""
+    T, D, V = 33001, 72, 130
+    dt = DTYPES[dtype]
+    h, w, y = _head(T, D, V, dt, seed=30, scale=2.0)
+    drop = torch.rand(T, generator=_gen(31), device="cuda") < 0.4
+    drop[1000:9000] = True
+    drop[20000:28000] = False
+    y[drop] = -100
+    h[drop] = math.nan
+    if soft:
+        index, teacher = y[:, None].clone(), torch.zeros(T, 1, device="cuda")
+        index[drop] = -1
+    want, dh, dw = ref_ce(h, w, y)
+    call = lambda a, b, **k: (losses.linear_distillation(a, b, index, teacher, **k) if soft else  # noqa: E731
+                              losses.linear_cross_entropy(a, b, y, **k))
+    rows = call(h, w, reduction="none")
+    assert ((rows - want).abs() <= torch.where(drop, 0.0, _loss_bound(torch.where(drop[:, None], 0.0, h), w)) + 2.0**-17 * soft).all()
+    n = int((~drop).sum())
+    h.requires_grad_(), w.requires_grad_()
+    for chunk in (0, 8192):
+        gh, gw = _grads(call(h, w, chunk_rows=chunk), h, w)
+        assert (gh[drop] == 0).all()
+        assert _rel(gh, dh / n) <= GRAD_TOL[dt] and _rel(gw, dw / n) <= GRAD_TOL[dt]
