@@ -316,8 +316,8 @@ int po_matmul(const void* A, long long lda, long long sa, int trans_a, const voi
  * multiplied by powers of two chosen from the data, so that fp16 ones keep their
  * digits until a loss scale is applied, and those of a sum stay in range until
  * the caller's division; loss_rows then has two more elements, which receive the
- * inverse factors of dhidden and dweight (PO_MEAN_SCALED of po_distill_logits:
- * one more, of dlogits; it has no PO_SUM_SCALED).
+ * inverse factors of dhidden and dweight (one, of dlogits, from
+ * po_distill_logits).
  * The logits are never stored: without gradients each tile of them (256
  * columns, 64 for a few rows) leaves two numbers a row; with gradients at most chunk_rows rows at a time (0: a
  * default by the workspace it takes) leave their scaled exponentials in the

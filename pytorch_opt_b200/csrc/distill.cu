@@ -57,12 +57,13 @@ __device__ __forceinline__ int entry_status(const DistillArgs& a, long long t, i
   return l > -INFINITY || isnan(l) ? ROW_COUNTED : ROW_IGNORED;
 }
 
-// The power of two that fp16 gradients of a mean are stored by, so that the
+// The power of two that fp16 gradients of a scalar are stored by, so that the
 // rounding here comes above fp16's smallest values and the caller's loss scale
-// not too late: |dz| <= 2 a / n, times n 2^14 / max(a, 1) at most.
+// not too late: |dz| <= 2 a / n, times n 2^14 / max(a, 1) at most, n = 1 for a sum.
 __device__ __forceinline__ float store_scale(const DistillArgs& a) {
   if (a.unscale == nullptr) return 1.0f;
-  return exp2f(floorf(log2f(static_cast<float>(a.st->count) / fmaxf(a.temperature, 1.0f))) + 14.0f);
+  const float n = a.mean ? static_cast<float>(a.st->count) : 1.0f;
+  return exp2f(floorf(log2f(n / fmaxf(a.temperature, 1.0f))) + 14.0f);
 }
 
 // Rows that the mean divides by (counted ones and those with a bad index).
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__((GRAD ? kGradThreads : kEvalThreads) + 32, GRA
       c = warp_sum(c);
       if (lane == 0) {
         a.loss_rows[t] = live ? a.temperature * a.temperature * (s_qlogq + c) : (status == ROW_BAD ? NAN : 0.0f);
-        if (a.unscale != nullptr && t == 0) *a.unscale = a.st->count > 0 ? 1.0f / store_scale(a) : 1.0f;
+        if (a.unscale != nullptr && t == 0) *a.unscale = !a.mean || a.st->count > 0 ? 1.0f / store_scale(a) : 1.0f;
         if (a.loss != nullptr) {
           __threadfence();
           s_last = atomicAdd(&a.st->done, 1u) == static_cast<unsigned int>(a.T) - 1;
@@ -337,8 +338,8 @@ __global__ void __launch_bounds__((GRAD ? kGradThreads : kEvalThreads) + 32, GRA
     const bool vec = reinterpret_cast<uintptr_t>(out0) % 16 == 0;
     float w = 0.0f;
     if (live) {
-      w = a.temperature;
-      if (a.mean) w *= store_scale(a) / static_cast<float>(a.st->count);
+      w = a.temperature * store_scale(a);
+      if (a.mean) w /= static_cast<float>(a.st->count);
       if (a.row_grad != nullptr) w *= a.row_grad[t];
     }
     const float ws = w / s;
@@ -472,7 +473,6 @@ extern "C" int po_distill_logits(const void* logits, long long ld, int dtype, lo
   if (top < 1 || top > kMaxTop) return set_error(PO_ERR_ARG, "distill_logits: top must be 1 to 1024");
   if (!temperature_ok(temperature))
     return set_error(PO_ERR_ARG, "distill_logits: temperature must be 2^-60 to 2^60");
-  if (mean == PO_SUM_SCALED) return set_error(PO_ERR_ARG, "distill_logits: gradients of a sum need no scaling");
   if (row_grad != nullptr && (mean || dlogits == nullptr))
     return set_error(PO_ERR_ARG, "distill_logits: row_grad goes with gradients of the sum");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -484,9 +484,11 @@ extern "C" int po_distill_logits(const void* logits, long long ld, int dtype, lo
   DistillArgs a{};
   a.z = logits, a.ld = ld, a.dz = dlogits, a.dz_ld = dl_ld, a.T = tokens, a.V = static_cast<int>(vocab);
   a.index = index, a.index_ld = index_ld, a.teacher = teacher, a.teacher_ld = teacher_ld;
+  const bool scaled = mean == PO_MEAN_SCALED || mean == PO_SUM_SCALED;
+  if (mean == PO_SUM_SCALED) mean = 0;
   a.teacher_dtype = teacher_dtype, a.top = static_cast<int>(top), a.temperature = temperature, a.mean = mean;
   a.row_grad = row_grad, a.loss_rows = loss_rows, a.loss = loss;
-  if (mean == PO_MEAN_SCALED && dtype == PO_F16 && dlogits != nullptr) a.unscale = loss_rows + tokens;
+  if (scaled && dtype == PO_F16 && dlogits != nullptr) a.unscale = loss_rows + tokens;
   if (loss != nullptr || mean) {
     if (workspace == nullptr || workspace_bytes < sizeof(DistillState))
       return set_error(PO_ERR_WORKSPACE, "distill_logits: workspace too small");

@@ -479,9 +479,9 @@ __device__ __forceinline__ void put_dz(const RescaleArgs& a, long long off, floa
 }
 
 // One block: the factors of the fp16 products, and the powers of two that
-// gradients of a scalar are stored by. A mean's gradients may lie below fp16's
-// range until the caller's loss scale lifts them, a sum's above it until the
-// caller's division, and both come after the rounding here. With dZ's row at
+// gradients of a scalar are stored by. They may lie below fp16's range until the
+// caller's loss scale lifts them, a sum's also above it until the caller's
+// division, and both come after the rounding here. With dZ's row at
 // most 2 m in sum of magnitudes, m = coef_max times room, the mean's have
 // |dH| <= 2 m max|W| / n and |dW| <= 2 m max|h|, the sum's n times as much:
 // neither leaves the range by its factor (dH's takes 2 m / n away, a sum's m;
@@ -502,7 +502,7 @@ __device__ __forceinline__ void choose_scales(const RescaleArgs& a, float* buf) 
       sw = fminf(fmaxf(exp2f(floorf(log2f(16384.0f / top))), 1.0f), 65536.0f);
     } else {
       sh = fmaxf(exp2f(floorf(log2f(1.0f / m))), 0x1p-40f);
-      sw = fminf(fmaxf(exp2f(floorf(log2f(16384.0f / (top * fmaxf(n, 1.0f))))), 0x1p-40f), 1.0f);
+      sw = fminf(fmaxf(exp2f(floorf(log2f(16384.0f / (top * fmaxf(n, 1.0f))))), 0x1p-40f), 65536.0f);
     }
   }
   if (threadIdx.x != 0) return;

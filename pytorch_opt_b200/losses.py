@@ -132,8 +132,8 @@ def _distill_logits(logits, index, teacher, temperature, mean, scalar, row_grad,
             loss, losses = torch.empty((), dtype=torch.float32, device=dev), None
             ws = _lib.workspace(nbytes + 4 * tokens, dev)
             rows_ptr = ws.data_ptr() + nbytes
-            if mean and dtype is torch.float16 and want_grad and tokens:
-                mean, rows = _MEAN_SCALED, torch.empty(tokens + 1, dtype=torch.float32, device=dev)
+            if dtype is torch.float16 and want_grad and tokens:
+                mean, rows = _MEAN_SCALED if mean else _SUM_SCALED, torch.empty(tokens + 1, dtype=torch.float32, device=dev)
                 rows_ptr, unscale = rows.data_ptr(), rows[tokens:]
         else:
             nbytes, ws, loss = 0, None, None

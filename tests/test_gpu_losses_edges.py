@@ -371,3 +371,27 @@ def test_masked_rows_among_many(soft, dtype):
         gh, gw = _grads(call(h, w, chunk_rows=chunk), h, w)
         assert (gh[drop] == 0).all()
         assert _rel(gh, dh / n) <= GRAD_TOL[dt] and _rel(gw, dw / n) <= GRAD_TOL[dt]
+
+
+@pytest.mark.parametrize("T", [1, 2, 30, 600])
+def test_fp16_gradients_of_a_sum_keep_their_digits_under_a_loss_scale(T):
+    """Softmax itself is below fp16's smallest normal value in a large vocabulary; loss_sum / n times a scale lifts it."""
+    D, V, K, up = 64, 60000, 4, 2.0**12
+    h, w, y = _head(T, D, V, torch.float16, seed=10, scale=0.1)
+    _, dh, dw = ref_ce(h, w, y, up=torch.full((T,), up / T, device="cuda"))
+    h.requires_grad_(), w.requires_grad_()
+    gh, gw = _grads(losses.linear_cross_entropy(h, w, y, reduction="sum") / T * up, h, w)
+    rare = torch.ones(V, dtype=torch.bool, device="cuda")
+    rare[y] = False
+    assert _rel(gh, dh) < GRAD_TOL[h.dtype] and _rel(gw, dw) < GRAD_TOL[h.dtype]
+    # A division by T that is no power of two rounds once more; 2^-7 as for a mean.
+    assert _rel(gw[rare], dw[rare]) < 2.0**-7
+    z, index, teacher = (4 * torch.randn(T, V, generator=_gen(5), device="cuda").half(), *_teacher(T, V, K, 6))
+    _, dz, _ = ref_distill(z, index, teacher, 2.0, torch.full((T,), up / T, device="cuda"))
+    z.requires_grad_()
+    gz, = _grads(losses.distillation(z, index, teacher, temperature=2.0, reduction="sum") / T * up, z)
+    rest = torch.ones_like(z, dtype=torch.bool).scatter_(1, index.clamp(min=0), False)
+    rest &= dz.abs() > 2.0**-13  # what fp16 holds to 2^-11 once it is scaled
+    # Each value is rounded to 2^-11 twice.
+    assert _rel(gz, dz) < 2.0**-9
+    assert float(((gz.double() - dz).abs() / dz.abs().clamp_min(1e-30))[rest].max()) < 2.0**-9

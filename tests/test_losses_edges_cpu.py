@@ -38,10 +38,11 @@ def test_abi_refuses_temperatures_outside_fp32(temperature):
     assert "temperature" in _lib.last_error()
 
 
-def test_abi_knows_scaled_sums_of_linear_losses_only():
+def test_abi_refuses_row_grad_beside_a_scaled_scalar():
     lib = _lib.load()
-    assert lib.po_distill_logits(P, 16, 1, 4, 16, P, 2, P, 2, 0, 2, 1.0, 3, None, P, P, P, 16, P, 8, None) == 1
-    assert "sum" in _lib.last_error()
-    assert lib.po_linear_loss(P, 8, P, 8, 2, 4, 8, 16, P, 1, None, 1, 0, 1, -100, 0.0, 0.0, 1.0, 3, P, P, P, P, 8, None,
-                              8, 0, P, 1 << 30, None) == 1
-    assert "row_grad" in _lib.last_error()
+    for mode in (2, 3):
+        assert lib.po_distill_logits(P, 16, 1, 4, 16, P, 2, P, 2, 0, 2, 1.0, mode, P, P, P, P, 16, P, 8, None) == 1
+        assert "row_grad" in _lib.last_error()
+        assert lib.po_linear_loss(P, 8, P, 8, 2, 4, 8, 16, P, 1, None, 1, 0, 1, -100, 0.0, 0.0, 1.0, mode, P, P, P, P, 8,
+                                  None, 8, 0, P, 1 << 30, None) == 1
+        assert "row_grad" in _lib.last_error()
