@@ -94,7 +94,7 @@ __device__ __forceinline__ void finish_row(const FinishArgs& a, int row, int lan
   }
   const float mm = warp_max(m);
   s = warp_sum(m == -INFINITY ? s : s * ex2((m - mm) * a.scale2));
-  const float logs = kLn2 * log2f(s), lse = mm + logs;
+  const float logs = logf(s), lse = mm + logs;
   const long long t = a.rowmap[a.row0 + row];
   float zs = 0.0f;
   if (a.zsum != nullptr) {

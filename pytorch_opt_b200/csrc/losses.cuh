@@ -144,9 +144,10 @@ __device__ __forceinline__ T block_sum(T v, T* buf) {
 
 // Launches of one call follow one another closely: each may start (blocks
 // scheduled, barriers and tensor memory set up) while the one before it drains.
-// So every kernel of a call begins with grid_wait(), which returns when all
-// earlier work is done and visible, and lets its successor start with
-// grid_launch_next(). What an earlier launch of the call wrote is read with ordinary
+// So every thread of every kernel of a call passes grid_wait(), which returns
+// when all earlier work is done and visible, before it touches anything that a
+// launch of the call writes (what it does before that needs the caller's inputs
+// alone, or nothing), and lets its successor start with grid_launch_next(). What an earlier launch of the call wrote is read with ordinary
 // loads: the read-only path wants data that no kernel writes while this one is
 // resident.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -178,6 +179,5 @@ inline bool temperature_ok(float a) { return a >= 0x1p-60f && a <= 0x1p60f; }
 enum RowStatus : int { ROW_IGNORED = 0, ROW_COUNTED = 1, ROW_BAD = 2 };
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 }  // namespace po
