@@ -304,8 +304,9 @@ int po_matmul(const void* A, long long lda, long long sa, int trans_a, const voi
  * teacher's) has the loss NaN and gradient 0, and counts in the mean.
  *
  * hidden: tokens x dim, weight: vocab x dim, both of `dtype` (PO_BF16 /
- * PO_F16 / PO_F32: split-tf32 products, fp32-grade), rows contiguous with the
- * given pitches. index: tokens x top int64 (pitch index_ld); teacher: tokens
+ * PO_F16 / PO_F32: split-tf32 products, fp32-grade, for values below 3.4e38),
+ * rows contiguous with the given pitches. Gradients of 16-bit operands round
+ * dz to their type before the products, as a product of 16-bit operands must. index: tokens x top int64 (pitch index_ld); teacher: tokens
  * x top of teacher_dtype (PO_F32 / PO_BF16 / PO_F16). top <= 1024.
  * loss_rows (fp32 [tokens]) receives each row's loss; loss (nullable) their
  * sum, divided by the counted rows when `mean`. dhidden (pitch dh_ld) and
@@ -321,7 +322,7 @@ int po_matmul(const void* A, long long lda, long long sa, int trans_a, const voi
  * The logits are never stored: without gradients each tile of them (256
  * columns, 64 for a few rows) leaves two numbers a row; with gradients at most chunk_rows rows at a time (0: a
  * default by the workspace it takes) leave their scaled exponentials in the
- * workspace, in 16 bits (32 for fp32).
+ * workspace, in 16 bits (two times 32 for fp32).
  * ---------------------------------------------------------------------- */
 enum { PO_MEAN_SCALED = 2, PO_SUM_SCALED = 3 };
 size_t po_linear_loss_workspace_bytes(const void* weight, long long w_ld, int dtype, long long tokens, long long dim,
@@ -337,8 +338,10 @@ int po_linear_loss(const void* hidden, long long h_ld, const void* weight, long 
 
 /* The teacher's form of po_linear_loss on logits that are there: logits and
  * dlogits (nullable) tokens x vocab of `dtype` (PO_F32 / PO_BF16 / PO_F16)
- * with any pitches; the logits are read once and dlogits written once
- * (dlogits == logits, with equal pitches, is allowed). */
+ * with any pitches. Without gradients the logits are read once, with them a
+ * second time (from L2, where the rows in work fit), and dlogits is written
+ * once; dlogits == logits, with equal pitches, is allowed. Rows that count for
+ * nothing are read like the others. */
 size_t po_distill_logits_workspace_bytes(long long tokens);
 int po_distill_logits(const void* logits, long long ld, int dtype, long long tokens, long long vocab,
                       const long long* index, long long index_ld, const void* teacher, long long teacher_ld,
