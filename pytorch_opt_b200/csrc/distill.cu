@@ -44,6 +44,7 @@ struct DistillArgs {
   float* loss;
   DistillState* st;
   float* unscale;  // nullable: 1 / store_scale
+  int by_powers;   // gradients are stored by powers of two: fp16 ones beside an `unscale`
   int seg;  // elements a CTA takes
 };
 
@@ -61,7 +62,7 @@ __device__ __forceinline__ int entry_status(const DistillArgs& a, long long t, i
 // rounding here comes above fp16's smallest values and the caller's loss scale
 // not too late: |dz| <= 2 a / n, times n 2^14 / max(a, 1) at most, n = 1 for a sum.
 __device__ __forceinline__ float store_scale(const DistillArgs& a) {
-  if (a.unscale == nullptr) return 1.0f;
+  if (!a.by_powers) return 1.0f;
   const float n = a.mean ? static_cast<float>(a.st->count) : 1.0f;
   return exp2f(floorf(log2f(n / fmaxf(a.temperature, 1.0f))) + 14.0f);
 }
@@ -488,7 +489,7 @@ extern "C" int po_distill_logits(const void* logits, long long ld, int dtype, lo
   if (mean == PO_SUM_SCALED) mean = 0;
   a.teacher_dtype = teacher_dtype, a.top = static_cast<int>(top), a.temperature = temperature, a.mean = mean;
   a.row_grad = row_grad, a.loss_rows = loss_rows, a.loss = loss;
-  if (scaled && dtype == PO_F16 && dlogits != nullptr) a.unscale = loss_rows + tokens;
+  if (scaled && dlogits != nullptr) a.unscale = loss_rows + tokens, a.by_powers = dtype == PO_F16;
   if (loss != nullptr || mean) {
     if (workspace == nullptr || workspace_bytes < sizeof(DistillState))
       return set_error(PO_ERR_WORKSPACE, "distill_logits: workspace too small");

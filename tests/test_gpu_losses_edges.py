@@ -395,3 +395,37 @@ def test_fp16_gradients_of_a_sum_keep_their_digits_under_a_loss_scale(T):
     # Each value is rounded to 2^-11 twice.
     assert _rel(gz, dz) < 2.0**-9
     assert float(((gz.double() - dz).abs() / dz.abs().clamp_min(1e-30))[rest].max()) < 2.0**-9
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("mode", [2, 3])
+def test_c_functions_report_the_factors_they_store_by(mode, dtype):
+    """PO_MEAN_SCALED and PO_SUM_SCALED of every type: stored gradients times the reported factors are the gradients;
+    for bf16 and fp32 the factors are 1."""
+    dt, lib = DTYPES[dtype], _lib.load()
+    T, D, V, K = 40, 64, 300, 3
+    h, w, y = _head(T, D, V, dt, seed=12)
+    index, teacher = _teacher(T, V, K, 5)
+    n = T if mode == 2 else 1
+    _, dh, dw = ref_ce(h, w, y)
+    loss, code, stream = torch.empty((), device="cuda"), _lib.DTYPE_CODE[dt], _lib.stream_ptr(h.device)
+    rows = torch.full((T + 2,), math.nan, device="cuda")
+    gh, gw = torch.empty_like(h), torch.empty_like(w)
+    nbytes = lib.po_linear_loss_workspace_bytes(w.data_ptr(), D, code, T, D, V, 1, 1, 1, 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    _lib.check(lib.po_linear_loss(
+        h.data_ptr(), D, w.data_ptr(), D, code, T, D, V, y.data_ptr(), 1, None, 0, 0, 1, -100, 0.0, 0.0, 1.0, mode, None,
+        rows.data_ptr(), loss.data_ptr(), gh.data_ptr(), D, gw.data_ptr(), D, 0, ws.data_ptr(), nbytes, stream), "head")
+    assert _rel(gh.double() * rows[T].double(), dh / n) <= GRAD_TOL[dt]
+    assert _rel(gw.double() * rows[T + 1].double(), dw / n) <= GRAD_TOL[dt]
+    assert dtype == "fp16" or (rows[T:] == 1).all()
+    z = torch.randn(T, V, generator=_gen(13), device="cuda").to(dt)
+    _, dz, counts = ref_distill(z, index, teacher, 1.0)
+    n = int(counts.sum()) if mode == 2 else 1
+    rows, gz = torch.full((T + 1,), math.nan, device="cuda"), torch.empty_like(z)
+    ws = torch.empty(lib.po_distill_logits_workspace_bytes(T), dtype=torch.uint8, device="cuda")
+    _lib.check(lib.po_distill_logits(
+        z.data_ptr(), V, code, T, V, index.data_ptr(), K, teacher.data_ptr(), K, 0, K, 1.0, mode, None, rows.data_ptr(),
+        loss.data_ptr(), gz.data_ptr(), V, ws.data_ptr(), ws.numel(), stream), "logits")
+    assert _rel(gz.double() * rows[T].double(), dz / n) <= GRAD_TOL[dt]
+    assert dtype == "fp16" or float(rows[T]) == 1.0
